@@ -1,0 +1,816 @@
+"""Root-mean-square norm of rows: with the addition of a residual, with an
+output in 8 bits, and its gradient.
+
+With ``h = x + residual`` (``h = x`` without one) a row of ``width`` elements
+becomes ``y = h * r * weight``, ``r = 1 / sqrt(mean(h * h) + eps)``.  A row is
+read once: a group of lanes holds it in registers (packed, as it is stored),
+reduces, and writes from the same registers.  The reference has no such
+function; in its terms it is the row-wise fusion of
+cupy/_core/_fusion_kernel.pyx:99-115, which takes one kernel per reduction.
+"""
+import numpy
+
+from cupy_amd._core import _op_calls as _oc
+from cupy_amd._core._op_calls import Ref
+
+_SOURCE = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<X_T>::type A;
+typedef cupy::bits_of<A>::type Bits;
+
+struct Stat { A square; Bits top; };
+struct JoinStat {
+  _CUPY_DEV Stat operator()(const Stat& a, const Stat& b) const {
+    Stat r;
+    r.square = a.square + b.square;
+    r.top = a.top > b.top ? a.top : b.top;
+    return r;
+  }
+};
+
+#ifdef INT8
+typedef signed char Y_T;
+#else
+typedef X_T Y_T;
+#endif
+
+// What a row's statistics turn its elements h * weight into.
+struct Finish {
+  A r, inv, lift;
+  A scale;
+  _CUPY_DEV Finish(const Stat& s, int width, A eps) {
+    r = A(1) / cupy::sqrt_(s.square / A(width) + eps);
+#ifdef INT8
+    // max |y| = r * max |h w|, and q = y / scale = h w * (127 / max |h w|): r
+    // cancels.  Tiny rows are lifted by a power of two first, so that the
+    // quotient stays finite.
+    const A top = cupy::from_bits(s.top);
+    const bool tiny = top < A(1e-30);
+    lift = tiny ? A(1.2676506002282294e30) : A(1);     // 2^100
+    inv = top > A(0) ? A(127) / (top * lift) : A(0);
+    scale = top * r / A(127);
+#endif
+  }
+  _CUPY_DEV Y_T operator()(A hw) const {
+#ifdef INT8
+    // (a NaN compares false both ways and becomes 0; the row's scale is NaN)
+    const A q = cupy::rint_(hw * lift * inv);
+    return static_cast<signed char>(q >= A(-127) ? (q <= A(127) ? static_cast<int>(q) : 127)
+                                                 : (q < A(-127) ? -127 : 0));
+#else
+    return static_cast<Y_T>(hw * r);
+#endif
+  }
+};
+
+// h of one vector, from registers.  The sum is rounded to the type it is
+// stored in only on its way to memory: y follows from the unrounded sum.
+template <int N>
+_CUPY_DEV void sums_of(const cupy::Vec<X_T, N>& x, const cupy::Vec<R_T, N>& res, A (&h)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    h[e] = static_cast<A>(x.v[e]);
+#ifdef RESIDUAL
+    h[e] += static_cast<A>(res.v[e]);
+#endif
+  }
+}
+
+#if ITEMS > 0
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
+              const long long rows, const int width, const long long px, const long long pr,
+              const long long py, const long long ps, const double eps) {
+  constexpr int kRows = BLOCK / LANES;
+  __shared__ Stat lds[2][BLOCK / 64];
+  const int lane = threadIdx.x % LANES;
+  cupy::Vec<W_T, VEC> wv[ITEMS];
+#ifdef WEIGHT
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int c = (lane + k * LANES) * VEC;
+    if (c < width) wv[k] = cupy::load_part<W_T, VEC>(w + c, width - c);
+  }
+#endif
+  int flip = 0;
+  for (long long base = (long long)blockIdx.x * kRows; base < rows;
+       base += (long long)gridDim.x * kRows) {
+    const long long row = base + threadIdx.x / LANES;
+    const bool valid = kRows == 1 || row < rows;
+    cupy::Vec<X_T, VEC> xv[ITEMS];
+    cupy::Vec<R_T, VEC> rv[ITEMS];
+    if (valid) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int c = (lane + k * LANES) * VEC;
+        if (c < width) {
+          xv[k] = cupy::load_part<X_T, VEC, NT_IN>(x + row * px + c, width - c);
+#ifdef RESIDUAL
+          rv[k] = cupy::load_part<R_T, VEC, NT_IN>(res + row * pr + c, width - c);
+#endif
+        }
+      }
+    }
+    Stat s;
+    s.square = A(0);
+    s.top = 0;
+    if (valid) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        if ((lane + k * LANES) * VEC >= width) continue;
+        A h[VEC];
+        sums_of<VEC>(xv[k], rv[k], h);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s.square = cupy::fma_(h[e], h[e], s.square);
+#ifdef INT8
+#ifdef WEIGHT
+          // (a partial vector's tail is zeros)
+          const Bits b = cupy::abs_bits(h[e] * static_cast<A>(wv[k].v[e]));
+#else
+          const Bits b = cupy::abs_bits(h[e]);
+#endif
+          s.top = b > s.top ? b : s.top;
+#endif
+        }
+      }
+    }
+    s = cupy::row_allreduce<LANES, BLOCK>(s, JoinStat(), lds[flip]);
+    flip ^= 1;
+    if (!valid) continue;
+    const Finish fin(s, width, static_cast<A>(eps));
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int c = (lane + k * LANES) * VEC;
+      if (c >= width) continue;
+      A h[VEC];
+      sums_of<VEC>(xv[k], rv[k], h);
+#ifdef RESIDUAL
+      cupy::Vec<R_T, VEC> hv;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) hv.v[e] = static_cast<R_T>(h[e]);
+      cupy::store_part<R_T, VEC, NT_OUT>(sum + row * ps + c, hv, width - c);
+#endif
+      cupy::Vec<Y_T, VEC> yv;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+#ifdef WEIGHT
+        yv.v[e] = fin(h[e] * static_cast<A>(wv[k].v[e]));
+#else
+        yv.v[e] = fin(h[e]);
+#endif
+      }
+      cupy::store_part<Y_T, VEC, NT_OUT>(y + row * py + c, yv, width - c);
+    }
+#ifdef INT8
+    if (lane == 0) scale[row] = static_cast<float>(fin.scale);
+#endif
+  }
+}
+#else
+// Rows longer than the registers hold: a workgroup walks its row twice, the
+// second time out of the cache.  Every element is written by the thread that
+// read it, in the second walk only, so outputs may lie on the inputs here too.
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
+              const long long rows, const int width, const long long px, const long long pr,
+              const long long py, const long long ps, const double eps) {
+  __shared__ Stat lds[2][BLOCK / 64];
+  int flip = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    Stat s;
+    s.square = A(0);
+    s.top = 0;
+    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+      rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
+#endif
+      A h[VEC];
+      sums_of<VEC>(xv, rv, h);
+      cupy::Vec<W_T, VEC> wv;
+#if defined(INT8) && defined(WEIGHT)
+      wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        s.square = cupy::fma_(h[e], h[e], s.square);
+#ifdef INT8
+#ifdef WEIGHT
+        const Bits b = cupy::abs_bits(h[e] * static_cast<A>(wv.v[e]));
+#else
+        const Bits b = cupy::abs_bits(h[e]);
+#endif
+        s.top = b > s.top ? b : s.top;
+#endif
+      }
+    }
+    s = cupy::row_allreduce<BLOCK, BLOCK>(s, JoinStat(), lds[flip]);
+    flip ^= 1;
+    const Finish fin(s, width, static_cast<A>(eps));
+    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+      rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
+#endif
+      A h[VEC];
+      sums_of<VEC>(xv, rv, h);
+#ifdef RESIDUAL
+      cupy::Vec<R_T, VEC> hv;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) hv.v[e] = static_cast<R_T>(h[e]);
+      cupy::store_part<R_T, VEC>(sum + row * ps + c, hv, have);
+#endif
+      cupy::Vec<Y_T, VEC> yv;
+#ifdef WEIGHT
+      const cupy::Vec<W_T, VEC> wv = cupy::load_part<W_T, VEC>(w + c, have);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e] * static_cast<A>(wv.v[e]));
+#else
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e]);
+#endif
+      cupy::store_part<Y_T, VEC>(y + row * py + c, yv, have);
+    }
+#ifdef INT8
+    if (threadIdx.x == 0) scale[row] = static_cast<float>(fin.scale);
+#endif
+  }
+}
+#endif
+''')
+
+_GRAD_SOURCE = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<X_T>::type A;
+
+struct Pair { A square, dot; };
+struct JoinPair {
+  _CUPY_DEV Pair operator()(const Pair& a, const Pair& b) const {
+    Pair r;
+    r.square = a.square + b.square;
+    r.dot = a.dot + b.dot;
+    return r;
+  }
+};
+
+// With n = x r, a = g w and m = mean(a n):  dx = r (a - n m) = r a - x k,
+// k = r^3 sum(a x) / width;  dw = sum over the rows of g n.
+struct Factors {
+  A r, k;
+  _CUPY_DEV Factors(const Pair& s, int width, A eps) {
+    r = A(1) / cupy::sqrt_(s.square / A(width) + eps);
+    k = r * r * r * (s.dot / A(width));
+  }
+};
+
+#if ITEMS > 0
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
+                   A* partial, const long long rows, const int width, const long long pg,
+                   const long long px, const long long pr, const long long pd, const double eps) {
+  constexpr int kRows = BLOCK / LANES;
+  __shared__ Pair lds[2][BLOCK / 64];
+  const int lane = threadIdx.x % LANES;
+#ifdef WEIGHT
+  cupy::Vec<W_T, VEC> wv[ITEMS];
+  A dw[ITEMS][VEC];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int c = (lane + k * LANES) * VEC;
+    if (c < width) wv[k] = cupy::load_part<W_T, VEC>(w + c, width - c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[k][e] = A(0);
+  }
+#endif
+  int flip = 0;
+  for (long long base = (long long)blockIdx.x * kRows; base < rows;
+       base += (long long)gridDim.x * kRows) {
+    const long long row = base + threadIdx.x / LANES;
+    const bool valid = kRows == 1 || row < rows;
+    cupy::Vec<X_T, VEC> xv[ITEMS], gv[ITEMS];
+    cupy::Vec<R_T, VEC> rv[ITEMS];
+    if (valid) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int c = (lane + k * LANES) * VEC;
+        if (c < width) {
+          xv[k] = cupy::load_part<X_T, VEC, NT_IN>(x + row * px + c, width - c);
+          gv[k] = cupy::load_part<X_T, VEC, NT_IN>(g + row * pg + c, width - c);
+#ifdef RESIDUAL
+          rv[k] = cupy::load_part<R_T, VEC, NT_IN>(dres + row * pr + c, width - c);
+#endif
+        }
+      }
+    }
+    Pair s;
+    s.square = s.dot = A(0);
+    if (valid) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        if ((lane + k * LANES) * VEC >= width) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const A xe = static_cast<A>(xv[k].v[e]);
+          A a = static_cast<A>(gv[k].v[e]);
+#ifdef WEIGHT
+          a *= static_cast<A>(wv[k].v[e]);
+#endif
+          s.square = cupy::fma_(xe, xe, s.square);
+          s.dot = cupy::fma_(a, xe, s.dot);
+        }
+      }
+    }
+    s = cupy::row_allreduce<LANES, BLOCK>(s, JoinPair(), lds[flip]);
+    flip ^= 1;
+    if (!valid) continue;
+    const Factors f(s, width, static_cast<A>(eps));
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int c = (lane + k * LANES) * VEC;
+      if (c >= width) continue;
+      cupy::Vec<X_T, VEC> d;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A xe = static_cast<A>(xv[k].v[e]), ge = static_cast<A>(gv[k].v[e]);
+        A a = ge;
+#ifdef WEIGHT
+        a *= static_cast<A>(wv[k].v[e]);
+        dw[k][e] = cupy::fma_(ge, xe * f.r, dw[k][e]);
+#endif
+        A v = cupy::fma_(-xe, f.k, a * f.r);
+#ifdef RESIDUAL
+        v += static_cast<A>(rv[k].v[e]);
+#endif
+        d.v[e] = static_cast<X_T>(v);
+      }
+      cupy::store_part<X_T, VEC, NT_OUT>(dx + row * pd + c, d, width - c);
+    }
+  }
+#ifdef WEIGHT
+  // the workgroup's share of dw: its groups of lanes are added in order
+  if (kRows == 1) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int c = (lane + k * LANES) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (c + e < width) partial[(long long)blockIdx.x * width + c + e] = dw[k][e];
+    }
+  } else {
+    __shared__ A shares[kRows == 1 ? 1 : BLOCK * VEC];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) shares[threadIdx.x * VEC + e] = dw[k][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < LANES * VEC; i += BLOCK) {
+        A t = A(0);
+        for (int q = 0; q < kRows; ++q) t += shares[q * LANES * VEC + i];
+        const int c = k * LANES * VEC + i;
+        if (c < width) partial[(long long)blockIdx.x * width + c] = t;
+      }
+    }
+  }
+#endif
+}
+#else
+// Rows longer than the registers hold: walked twice; every row's r is kept
+// for the sums down the columns, which a kernel of their own makes.
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
+                   A* row_r, const long long rows, const int width, const long long pg,
+                   const long long px, const long long pr, const long long pd, const double eps) {
+  __shared__ Pair lds[2][BLOCK / 64];
+  int flip = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    Pair s;
+    s.square = s.dot = A(0);
+    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
+      cupy::Vec<W_T, VEC> wv;
+#ifdef WEIGHT
+      wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A xe = static_cast<A>(xv.v[e]);
+        A a = static_cast<A>(gv.v[e]);
+#ifdef WEIGHT
+        a *= static_cast<A>(wv.v[e]);
+#endif
+        s.square = cupy::fma_(xe, xe, s.square);
+        s.dot = cupy::fma_(a, xe, s.dot);
+      }
+    }
+    s = cupy::row_allreduce<BLOCK, BLOCK>(s, JoinPair(), lds[flip]);
+    flip ^= 1;
+    const Factors f(s, width, static_cast<A>(eps));
+#ifdef WEIGHT
+    if (threadIdx.x == 0) row_r[row] = f.r;
+#endif
+    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
+      cupy::Vec<W_T, VEC> wv;
+#ifdef WEIGHT
+      wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+      cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+      rv = cupy::load_part<R_T, VEC>(dres + row * pr + c, have);
+#endif
+      cupy::Vec<X_T, VEC> d;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A xe = static_cast<A>(xv.v[e]);
+        A a = static_cast<A>(gv.v[e]);
+#ifdef WEIGHT
+        a *= static_cast<A>(wv.v[e]);
+#endif
+        A v = cupy::fma_(-xe, f.k, a * f.r);
+#ifdef RESIDUAL
+        v += static_cast<A>(rv.v[e]);
+#endif
+        d.v[e] = static_cast<X_T>(v);
+      }
+      cupy::store_part<X_T, VEC>(dx + row * pd + c, d, have);
+    }
+  }
+}
+#endif
+
+// Partial sum of dw over the p-th run of rows, a thread per column: the first
+// `skip` words of `temp` are the rows' r, the partial sums follow.
+extern "C" __global__ void __launch_bounds__(256)
+cupy_rms_norm_columns(const X_T* g, const X_T* x, A* temp, const long long rows,
+                      const int width, const long long pg, const long long px,
+                      const long long run, const long long skip) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= width) return;
+  const long long r0 = blockIdx.y * run;
+  const long long r1 = r0 + run < rows ? r0 + run : rows;
+  A t = A(0);
+  for (long long r = r0; r < r1; ++r)
+    t = cupy::fma_(static_cast<A>(g[r * pg + c]), static_cast<A>(x[r * px + c]) * temp[r], t);
+  temp[skip + (long long)blockIdx.y * width + c] = t;
+}
+
+// dw = the sum of the partial rows: 16 columns by 64 slices of the partial
+// rows to a workgroup; a slice is summed in order, the slices by a tree.
+extern "C" __global__ void __launch_bounds__(1024)
+cupy_rms_norm_join(const A* temp, W_T* dw, const long long skip, const int n, const int width) {
+  const A* partial = temp + skip;
+  __shared__ A lds[64][17];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + tx;
+  A t = A(0);
+  if (c < width) {
+    int p = ty;
+    for (; p + 192 < n; p += 256) {
+      const A a = partial[(long long)p * width + c], b = partial[(long long)(p + 64) * width + c];
+      const A d = partial[(long long)(p + 128) * width + c], e = partial[(long long)(p + 192) * width + c];
+      t += a; t += b; t += d; t += e;
+    }
+    for (; p < n; p += 64) t += partial[(long long)p * width + c];
+  }
+  lds[ty][tx] = t;
+  __syncthreads();
+#pragma unroll
+  for (int half = 32; half > 0; half >>= 1) {
+    if (ty < half) lds[ty][tx] += lds[ty + half][tx];
+    __syncthreads();
+  }
+  if (ty == 0 && c < width) dw[c] = static_cast<W_T>(lds[0][tx]);
+}
+''')
+
+_plans = {}
+_plans_int8 = {}
+_plans_grad = {}
+
+# threads of a workgroup a CU may hold
+_THREADS_PER_CU = 2048
+
+
+def _geometry(width, itemsize, rows, most_items):
+    """(lanes per row, threads of a workgroup, vectors per lane, elements per
+    vector) of rows held in registers; 0 vectors: too long for them."""
+    vec = 16 // itemsize
+    n = (width + vec - 1) // vec
+    if n <= 64:
+        lanes = max(4, _oc.clp2(n))
+        return lanes, 256, 1, vec
+    if n <= 256:
+        lanes = 256 if rows < 1024 else 64
+        return lanes, 256, -(-n // lanes), vec
+    # few rows: the whole row at once, as many lanes as it has vectors
+    items = 1 if rows < 512 else 2
+    lanes = 256
+    while lanes < 1024 and lanes * items < n:
+        lanes *= 2
+    items = -(-n // lanes)
+    if items > most_items:
+        return 1024, 1024, 0, vec
+    return lanes, lanes, items, vec
+
+
+def _grid(rows, lanes, block):
+    per = block // lanes
+    return max(1, min(-(-rows // per), _oc.compute_units() * (_THREADS_PER_CU // block)))
+
+
+def _check(x, weight, residual, what):
+    _oc.check_float(x, 'x')
+    if x.ndim == 0:
+        raise ValueError('%s takes arrays of at least one dimension' % what)
+    if x._shape[-1] >= 1 << 31:
+        raise ValueError('%s: rows of 2**31 elements and more are not supported' % what)
+    if weight is not None:
+        _oc.check_float(weight, 'weight')
+        if weight._shape != x._shape[-1:]:
+            raise ValueError('weight has the wrong shape: %r, expected %r'
+                             % (weight._shape, x._shape[-1:]))
+        _check_mix(weight.dtype, x.dtype, 'weight')
+    if residual is not None:
+        _oc.check_float(residual, 'residual')
+        if residual._shape != x._shape:
+            raise ValueError('residual has the wrong shape: %r, expected %r'
+                             % (residual._shape, x._shape))
+        _check_mix(residual.dtype, x.dtype, 'residual')
+
+
+def _check_mix(dtype, base, name):
+    if dtype != base and not (base.char == 'e' and dtype.char == 'f'):
+        raise TypeError('%s of type %s does not go with x of type %s: the type of x, or float32 '
+                        'with float16' % (name, dtype, base))
+
+
+def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
+    eps = float(eps)
+    arrays = [x]
+    flags = 0
+    if weight is not None:
+        arrays.append(weight)
+        flags = 1
+    if residual is not None:
+        arrays.append(residual)
+        flags |= 2
+    if out is not None:
+        arrays.append(out)
+        flags |= 4
+    if scale_out is not None:
+        arrays.append(scale_out)
+        flags |= 8
+    if residual_out is not None:
+        arrays.append(residual_out)
+        flags |= 16
+    result, key = _oc.replay(plans, arrays, (flags, eps))
+    if result is not _oc._NOTHING:
+        return result
+    _check(x, weight, residual, 'rms_norm')
+    if residual_out is not None and residual is None:
+        raise ValueError('residual_out without residual')
+    y_dtype = numpy.dtype(numpy.int8) if int8 else x.dtype
+    if out is not None:
+        _oc.check_out(out, x._shape, y_dtype)
+    if scale_out is not None:
+        _oc.check_out(scale_out, x._shape[:-1], numpy.dtype(numpy.float32), 'scale_out')
+    if residual_out is not None:
+        _oc.check_out(residual_out, x._shape, residual.dtype, 'residual_out')
+    n_in = 1 + (weight is not None) + (residual is not None)
+    i_w = 1 if weight is not None else None
+    i_r = n_in - 1 if residual is not None else None
+    at = n_in
+    i_y = i_s = i_h = None
+    if out is not None:
+        i_y, at = at, at + 1
+    if scale_out is not None:
+        i_s, at = at, at + 1
+    if residual_out is not None:
+        i_h, at = at, at + 1
+    # a row is read whole before any of it is written, and a thread writes what
+    # it read: the outputs may take the place of x and the residual
+    places = [(i, o) for i in (0, i_r) if i is not None for o in (i_y, i_h) if o is not None]
+    call = _oc.Call(plans, key, arrays, n_in, places)
+    if i_y is None:
+        i_y = call.allocate(x._shape, y_dtype)
+    if int8 and i_s is None:
+        i_s = call.allocate(x._shape[:-1], numpy.float32)
+    if residual is not None and i_h is None:
+        i_h = call.allocate(x._shape, residual.dtype)
+    ret = (i_y,) + ((i_s,) if int8 else ()) + ((i_h,) if residual is not None else ())
+    width = x._shape[-1]
+    if x.size == 0:
+        call.key = None
+        if int8:
+            call.refs[i_s].fill(0)
+        call.begin()
+        out = call.finish(ret)
+        return out if len(out) > 1 else out[0]
+    rows = x.size // width
+    px = call.rows(0)
+    pr = call.rows(i_r) if i_r is not None else 0
+    py = call.rows(i_y)
+    ps = call.rows(i_h) if i_h is not None else 0
+    if i_w is not None:
+        call.dense(i_w)
+    if int8:
+        call.dense(i_s)
+    call.begin()
+    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, rows, 4)
+    nt_in, nt_out = _oc.stream_hints(
+        x.nbytes + (residual.nbytes if residual is not None else 0),
+        x.size * y_dtype.itemsize + (residual.nbytes if residual is not None else 0))
+    defines = dict(X_T=x.dtype, R_T=x.dtype if residual is None else residual.dtype,
+                   W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
+                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out)
+    for name, on in (('INT8', int8), ('WEIGHT', weight is not None),
+                     ('RESIDUAL', residual is not None)):
+        if on:
+            defines[name] = 1
+    fn = _SOURCE.function('cupy_rms_norm', **defines)
+    call.launch(fn, (_grid(rows, lanes, block), 1, 1), block, 'PPPPPPqiqqqqd',
+                Ref(0), Ref(i_r) if i_r is not None else 0, Ref(i_w) if i_w is not None else 0,
+                Ref(i_y), Ref(i_s) if int8 else 0, Ref(i_h) if i_h is not None else 0,
+                rows, width, px, pr, py, ps, eps)
+    out = call.finish(ret if len(ret) > 1 else ret[0])
+    return out
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6, *, out=None, residual_out=None):
+    """Root-mean-square norm along the last axis.
+
+    ``y = h / sqrt(mean(h * h) + eps) * weight`` with ``h = x + residual``
+    (``h = x`` without a residual).  Sums are held in 32 bits for float16 and
+    float32 (64 for float64); ``y`` is rounded once, from the unrounded ``h``.
+
+    Args:
+        x (cupy.ndarray): float16, float32 or float64, of one dimension or more.
+        weight (cupy.ndarray): one factor per column; of the type of ``x``, or
+            float32 with float16.
+        residual (cupy.ndarray): added to ``x`` first; shaped like ``x``, of its
+            type, or float32 with float16.
+        eps (float): added to the mean square.
+        out (cupy.ndarray): receives ``y``.
+        residual_out (cupy.ndarray): receives ``h``, in the residual's type.
+
+    ``out`` and ``residual_out`` may be ``x`` or ``residual`` themselves.
+
+    Returns:
+        ``y``, or ``(y, h)`` with a residual.
+    """
+    return _norm(_plans, False, x, weight, residual, eps, out, None, residual_out)
+
+
+def rms_norm_int8(x, weight=None, residual=None, eps=1e-6, *, out=None, scale_out=None,
+                  residual_out=None):
+    """:func:`rms_norm` with its result in 8 bits and a scale per row.
+
+    ``scale = max(|y|) / 127`` over the row (float32) and
+    ``q = rint(y / scale)``, ties to even: ``q * scale`` is ``y`` to half a
+    step.  A row of zeros has the scale 0; in a row with a NaN or an infinity
+    the scale is NaN.
+
+    Returns:
+        ``(q, scale)``, or ``(q, scale, h)`` with a residual: int8 shaped like
+        ``x``, float32 of the shape without the last axis, the sum.
+    """
+    return _norm(_plans_int8, True, x, weight, residual, eps, out, scale_out, residual_out)
+
+
+def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=None,
+                  weight_out=None):
+    """Gradients of :func:`rms_norm` with respect to its input and weight.
+
+    With ``n = x / sqrt(mean(x * x) + eps)`` and ``a = grad * weight``:
+    ``dx = (a - n * mean(a * n)) / sqrt(mean(x * x) + eps) + residual_grad`` and
+    ``dw = sum of grad * n`` over all rows, in an order that does not change
+    from call to call.
+
+    Args:
+        grad (cupy.ndarray): gradient of ``y``, of the shape and type of ``x``.
+        x (cupy.ndarray): what was normalised (``h`` where there was a residual).
+        weight (cupy.ndarray): as in the forward call.
+        residual_grad (cupy.ndarray): gradient that reaches ``h`` past the norm;
+            of the type of ``x``, or float32 with float16.
+        out (cupy.ndarray): receives ``dx``; may be ``grad``, ``x`` or
+            ``residual_grad``.
+        weight_out (cupy.ndarray): receives ``dw``.
+
+    Returns:
+        ``dx``, or ``(dx, dw)`` with a weight.  ``dx`` is the gradient of ``x``
+        and of the residual alike.
+    """
+    eps = float(eps)
+    arrays = [grad, x]
+    flags = 0
+    if weight is not None:
+        arrays.append(weight)
+        flags = 1
+    if residual_grad is not None:
+        arrays.append(residual_grad)
+        flags |= 2
+    if out is not None:
+        arrays.append(out)
+        flags |= 4
+    if weight_out is not None:
+        arrays.append(weight_out)
+        flags |= 8
+    result, key = _oc.replay(_plans_grad, arrays, (flags, eps))
+    if result is not _oc._NOTHING:
+        return result
+    _check(x, weight, None, 'rms_norm_grad')
+    _oc.check_float(grad, 'grad')
+    if grad._shape != x._shape or grad.dtype != x.dtype:
+        raise ValueError('grad has to have the shape and type of x: %r %s, expected %r %s'
+                         % (grad._shape, grad.dtype, x._shape, x.dtype))
+    if residual_grad is not None:
+        _oc.check_float(residual_grad, 'residual_grad')
+        if residual_grad._shape != x._shape:
+            raise ValueError('residual_grad has the wrong shape: %r, expected %r'
+                             % (residual_grad._shape, x._shape))
+        _check_mix(residual_grad.dtype, x.dtype, 'residual_grad')
+    if weight_out is not None and weight is None:
+        raise ValueError('weight_out without weight')
+    if out is not None:
+        _oc.check_out(out, x._shape, x.dtype)
+    if weight_out is not None:
+        _oc.check_out(weight_out, weight._shape, weight.dtype, 'weight_out')
+    n_in = 2 + (weight is not None) + (residual_grad is not None)
+    i_w = 2 if weight is not None else None
+    i_r = n_in - 1 if residual_grad is not None else None
+    at = n_in
+    i_d = i_dw = None
+    if out is not None:
+        i_d, at = at, at + 1
+    if weight_out is not None:
+        i_dw, at = at, at + 1
+    width = x._shape[-1]
+    rows = x.size // width if width else 0
+    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, rows,
+                                         2 if x.dtype.char == 'd' else 4)
+    # rows in registers: written by the threads that have read them.  (Rows
+    # that are walked are read again for dw.)
+    places = [(i, i_d) for i in (0, 1, i_r) if i is not None and i_d is not None
+              and (items or weight is None)]
+    call = _oc.Call(_plans_grad, key, arrays, n_in, places)
+    if i_d is None:
+        i_d = call.allocate(x._shape, x.dtype)
+    if weight is not None and i_dw is None:
+        i_dw = call.allocate(weight._shape, weight.dtype)
+    ret = (i_d, i_dw) if weight is not None else i_d
+    if x.size == 0:
+        call.key = None
+        if weight is not None:
+            call.refs[i_dw].fill(0)
+        call.begin()
+        return call.finish(ret)
+    pg, px = call.rows(0), call.rows(1)
+    pr = call.rows(i_r) if i_r is not None else 0
+    pd = call.rows(i_d)
+    if i_w is not None:
+        call.dense(i_w)
+        call.dense(i_dw)
+    call.begin()
+    nt_in, nt_out = _oc.stream_hints(3 * x.nbytes, x.nbytes)
+    defines = dict(X_T=x.dtype, R_T=x.dtype if residual_grad is None else residual_grad.dtype,
+                   W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
+                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out)
+    for name, on in (('WEIGHT', weight is not None), ('RESIDUAL', residual_grad is not None)):
+        if on:
+            defines[name] = 1
+    acc = _oc.acc_dtype(x.dtype).itemsize
+    grid = _grid(rows, lanes, block)
+    fn = _GRAD_SOURCE.function('cupy_rms_norm_grad', **defines)
+    # the temporary: the rows' r (walked rows only), then the partial sums of dw
+    n_partial, skip, run = grid, 0, 0
+    i_t = None
+    if weight is not None:
+        if not items:
+            # runs of rows, about as many as keep the device busy
+            blocks = -(-width // 256)
+            run = -(-rows // max(1, min(rows, -(-_oc.compute_units() * 8 // blocks), 65535)))
+            n_partial, skip = -(-rows // run), rows
+        i_t = call.temp((skip + n_partial * width) * acc)
+    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
+                Ref(0), Ref(1), Ref(i_w) if i_w is not None else 0,
+                Ref(i_r) if i_r is not None else 0, Ref(i_d), Ref(i_t) if i_t is not None else 0,
+                rows, width, pg, px, pr, pd, eps)
+    if weight is not None:
+        if not items:
+            fn = _GRAD_SOURCE.function('cupy_rms_norm_columns', **defines)
+            call.launch(fn, (blocks, n_partial, 1), 256, 'PPPqiqqqq',
+                        Ref(0), Ref(1), Ref(i_t), rows, width, pg, px, run, skip)
+        fn = _GRAD_SOURCE.function('cupy_rms_norm_join', **defines)
+        call.launch(fn, (-(-width // 16), 1, 1), 1024, 'PPqii',
+                    Ref(i_t), Ref(i_dw), skip, n_partial, width)
+    return call.finish(ret)

@@ -25,6 +25,9 @@ static PyObject* str_dtype;
 static PyObject* str_shape;
 static PyObject* str_strides;
 static PyObject* str_device_id;
+static PyObject* str_size;
+static PyObject* str_c_contiguous;
+static PyObject* str_f_contiguous;
 static PyTypeObject* array_type;      /* the package's ndarray, set by setup() */
 static PyTypeObject* generic_type;    /* numpy.generic */
 
@@ -366,7 +369,139 @@ static PyObject* hp_signature(PyObject* self, PyObject* const* args, Py_ssize_t 
   return sig;
 }
 
+/* overlap(arrays: tuple or list, spec: bytes) -> True if any listed pair of
+ * arrays shares memory.  spec: u32 n_arrays, u32 n_pairs, per array the lowest
+ * and one-past-highest byte it touches relative to its address (i64 each; both
+ * 0: it touches nothing), per pair two u32 positions; the top bit of the second
+ * says that the pair may start at the very same address (the same memory, laid
+ * out alike).  Reads addresses only. */
+static PyObject* hp_overlap(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 2 || !(PyTuple_Check(args[0]) || PyList_Check(args[0])) || !PyBytes_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "overlap(arrays: tuple or list, spec: bytes)");
+    return NULL;
+  }
+  const unsigned char* spec = (const unsigned char*)PyBytes_AS_STRING(args[1]);
+  const size_t size = (size_t)PyBytes_GET_SIZE(args[1]);
+  uint32_t n, pairs;
+  if (size < 8) goto malformed;
+  memcpy(&n, spec, 4);
+  memcpy(&pairs, spec + 4, 4);
+  if (size != 8 + 16 * (size_t)n + 8 * (size_t)pairs ||
+      (Py_ssize_t)n > PySequence_Fast_GET_SIZE(args[0]))
+    goto malformed;
+  uint64_t stack_at[64];
+  uint64_t* at = stack_at;
+  if (n > 64) {
+    at = (uint64_t*)PyMem_Malloc((size_t)n * 8);
+    if (!at) return PyErr_NoMemory();
+  }
+  int found = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    if (address_of(PySequence_Fast_GET_ITEM(args[0], i), 1, &at[i]) < 0) {
+      found = -1;
+      break;
+    }
+  }
+  for (uint32_t k = 0; k < pairs && found == 0; ++k) {
+    uint32_t a, b;
+    memcpy(&a, spec + 8 + 16 * (size_t)n + 8 * (size_t)k, 4);
+    memcpy(&b, spec + 12 + 16 * (size_t)n + 8 * (size_t)k, 4);
+    const int same = b >> 31;
+    b &= 0x7fffffffu;
+    if (a >= n || b >= n) {
+      found = -2;
+      break;
+    }
+    int64_t alo, ahi, blo, bhi;
+    memcpy(&alo, spec + 8 + 16 * (size_t)a, 8);
+    memcpy(&ahi, spec + 16 + 16 * (size_t)a, 8);
+    memcpy(&blo, spec + 8 + 16 * (size_t)b, 8);
+    memcpy(&bhi, spec + 16 + 16 * (size_t)b, 8);
+    if (alo == ahi || blo == bhi || (same && at[a] == at[b])) continue;
+    if (at[a] + (uint64_t)alo < at[b] + (uint64_t)bhi &&
+        at[b] + (uint64_t)blo < at[a] + (uint64_t)ahi)
+      found = 1;
+  }
+  if (at != stack_at) PyMem_Free(at);
+  if (found == -1) return NULL;
+  if (found == -2) goto malformed;
+  return PyBool_FromLong(found);
+malformed:
+  PyErr_SetString(PyExc_ValueError, "malformed overlap specification");
+  return NULL;
+}
+
+/* describe(arrays: list, types: list of dtypes) -> bytes, per array: u64 address,
+ * u64 elements, u32 position of its dtype in `types` (their number: none of
+ * them), u32 1 if stored in C order | 2 if in Fortran order, i64 device. */
+static PyObject* hp_describe(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 2 || !PyList_Check(args[0]) || !PyList_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "describe(arrays: list, types: list)");
+    return NULL;
+  }
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  PyObject* out = PyBytes_FromStringAndSize(NULL, n * 32);
+  if (!out) return NULL;
+  unsigned char* to = (unsigned char*)PyBytes_AS_STRING(out);
+  for (Py_ssize_t i = 0; i < n; ++i, to += 32) {
+    if (i >= PyList_GET_SIZE(args[0])) break;
+    PyObject* a = PyList_GET_ITEM(args[0], i);
+    PyObject *data = NULL, *ptr = NULL, *dev = NULL, *size = NULL, *dtype = NULL;
+    PyObject *c_order = NULL, *f_order = NULL;
+    int ok = 0;
+    uint64_t address, elements;
+    data = PyObject_GetAttr(a, str_data);
+    if (data) {
+      ptr = PyObject_GetAttr(data, str_ptr);
+      dev = PyObject_GetAttr(data, str_device_id);
+    }
+    size = PyObject_GetAttr(a, str_size);
+    dtype = PyObject_GetAttr(a, str_dtype);
+    c_order = PyObject_GetAttr(a, str_c_contiguous);
+    f_order = PyObject_GetAttr(a, str_f_contiguous);
+    if (ptr && dev && size && dtype && c_order && f_order && as_u64(ptr, &address) == 0 &&
+        as_u64(size, &elements) == 0) {
+      uint32_t type = 0;
+      const Py_ssize_t n_types = PyList_GET_SIZE(args[1]);
+      for (; (Py_ssize_t)type < n_types; ++type) {
+        const int same = PyObject_RichCompareBool(dtype, PyList_GET_ITEM(args[1], type), Py_EQ);
+        if (same != 0) break;          /* the same, or an error */
+      }
+      const int c = PyObject_IsTrue(c_order), f = PyObject_IsTrue(f_order);
+      const int64_t device = (int64_t)PyLong_AsLongLong(dev);
+      if (!PyErr_Occurred()) {
+        const uint32_t dense = (c ? 1u : 0u) | (f ? 2u : 0u);
+        memcpy(to, &address, 8);
+        memcpy(to + 8, &elements, 8);
+        memcpy(to + 16, &type, 4);
+        memcpy(to + 20, &dense, 4);
+        memcpy(to + 24, &device, 8);
+        ok = 1;
+      }
+    }
+    Py_XDECREF(data);
+    Py_XDECREF(ptr);
+    Py_XDECREF(dev);
+    Py_XDECREF(size);
+    Py_XDECREF(dtype);
+    Py_XDECREF(c_order);
+    Py_XDECREF(f_order);
+    if (!ok) {
+      Py_DECREF(out);
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "describe: no array");
+      return NULL;
+    }
+  }
+  return out;
+}
+
 static PyMethodDef methods[] = {
+    {"describe", (PyCFunction)(void (*)(void))hp_describe, METH_FASTCALL,
+     "describe(arrays, types) -> addresses, sizes, types and layouts as bytes"},
+    {"overlap", (PyCFunction)(void (*)(void))hp_overlap, METH_FASTCALL,
+     "overlap(arrays, spec) -> whether a listed pair of arrays shares memory"},
     {"get_device", hp_get_device, METH_NOARGS, "get_device() -> device index or -status"},
     {"setup", (PyCFunction)(void (*)(void))hp_setup, METH_FASTCALL,
      "setup(array type, numpy.generic)"},
@@ -395,7 +530,11 @@ PyMODINIT_FUNC PyInit__hotpath(void) {
   str_shape = PyUnicode_InternFromString("_shape");
   str_strides = PyUnicode_InternFromString("_strides");
   str_device_id = PyUnicode_InternFromString("device_id");
-  if (!str_data || !str_ptr || !str_dtype || !str_shape || !str_strides || !str_device_id)
+  str_size = PyUnicode_InternFromString("size");
+  str_c_contiguous = PyUnicode_InternFromString("_c_contiguous");
+  str_f_contiguous = PyUnicode_InternFromString("_f_contiguous");
+  if (!str_data || !str_ptr || !str_dtype || !str_shape || !str_strides || !str_device_id ||
+      !str_size || !str_c_contiguous || !str_f_contiguous)
     return NULL;
   return PyModule_Create(&module);
 }

@@ -1,0 +1,281 @@
+"""rms_norm, rms_norm_int8 and rms_norm_grad against the formula in float64.
+
+Bounds, with u = eps / 2 of the type sums are held in and ``terms`` the longest
+chain of additions one lane makes: a sum of squares is off by at most
+``terms * u`` relative to itself, its root by half of that, and each further
+operation adds u; the result is rounded once more, to its own type."""
+import numpy as np
+import pytest
+
+import cupy_amd as cp
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ['float16', 'float32', 'float64']
+SHAPES = [(1, 1), (3, 5), (7, 8), (300, 64), (65, 127), (1030, 513), (9, 2047), (2, 8192),
+          (600, 4100), (3, 16385), (2, 40001), (1500, 1000), (2, 3, 48), (96,)]
+
+
+def half_step(dtype):
+    return np.finfo(dtype).eps / 2
+
+
+def acc_step(dtype):
+    return half_step('float64' if np.dtype(dtype) == np.float64 else 'float32')
+
+
+def tiny(dtype):
+    # half of the smallest subnormal: what rounding below the normal range costs
+    return float(np.finfo(dtype).smallest_subnormal) / 2
+
+
+def terms(width):
+    # a lane adds at most 32 elements of a row in registers, width / 1024 + 8 of a
+    # longer one; the lanes are joined in at most 10 steps
+    return 42 + width / 1024 + 8
+
+
+def inputs(shape, dtype, seed=0, spread=1.0):
+    rng = np.random.default_rng(seed)
+    return (rng.standard_normal(shape) * spread).astype(dtype)
+
+
+def norm64(h, w, eps):
+    h = h.astype(np.float64)
+    r = 1 / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+    y = h * r
+    return y if w is None else y * w.astype(np.float64)
+
+
+def check_norm(y, want, width, dtype):
+    bound = (half_step(dtype) + (terms(width) / 2 + 8) * acc_step(dtype)) * np.abs(want) + tiny(dtype)
+    assert y.dtype == dtype
+    assert np.all(np.abs(y.astype(np.float64) - want) <= bound)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_norm(shape, dtype):
+    x, w, r = inputs(shape, dtype, 1), inputs(shape[-1:], dtype, 2), inputs(shape, dtype, 3, 3.0)
+    for weight in (None, w):
+        got = cp.rms_norm(cp.asarray(x), None if weight is None else cp.asarray(weight), eps=1e-5)
+        check_norm(got.get(), norm64(x, weight, 1e-5), shape[-1], dtype)
+    y, h = cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r), 1e-5)
+    h64 = x.astype(np.float64) + r.astype(np.float64)
+    check_norm(y.get(), norm64(h64, w, 1e-5), shape[-1], dtype)
+    assert h.dtype == dtype
+    assert np.all(np.abs(h.get().astype(np.float64) - h64) <= half_step(dtype) * np.abs(h64) * 1.001)
+
+
+@pytest.mark.parametrize('shape', [(5, 96), (700, 1001), (2, 33000)])
+def test_float32_weight_and_residual_with_float16(shape):
+    x, w, r = inputs(shape, 'float16', 1), inputs(shape[-1:], 'float32', 2), inputs(shape, 'float32', 3)
+    y, h = cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r))
+    h64 = x.astype(np.float64) + r.astype(np.float64)
+    check_norm(y.get(), norm64(h64, w, 1e-6), shape[-1], 'float16')
+    assert h.dtype == np.float32
+    assert np.all(np.abs(h.get() - h64) <= half_step('float32') * np.abs(h64) * 1.001)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_norm_to_int8(shape, dtype):
+    x, w, r = inputs(shape, dtype, 4), inputs(shape[-1:], dtype, 5), inputs(shape, dtype, 6)
+    q, s, h = cp.rms_norm_int8(cp.asarray(x), cp.asarray(w), cp.asarray(r))
+    want = norm64(x.astype(np.float64) + r.astype(np.float64), w, 1e-6)
+    step = np.abs(want).max(-1) / 127
+    assert q.dtype == np.int8 and s.dtype == np.float32 and s.shape == shape[:-1]
+    off = (terms(shape[-1]) / 2 + 10) * acc_step(dtype)
+    s_, q_ = s.get().astype(np.float64), q.get().astype(np.float64)
+    assert np.all(np.abs(s_ - step) <= (off + half_step('float32')) * step)
+    # half a step, and what the quotient (at most 127) is off by
+    assert np.all(np.abs(q_ - want / np.where(step > 0, step, 1)[..., None]) <= 0.5 + 127 * off)
+    assert np.all(np.abs(q_).max(-1) == 127)
+    h64 = x.astype(np.float64) + r.astype(np.float64)
+    assert np.all(np.abs(h.get().astype(np.float64) - h64) <= half_step(dtype) * np.abs(h64) * 1.001)
+
+
+def test_int8_rows_of_zeros_of_tiny_and_of_huge_values():
+    x = np.zeros((6, 40), np.float32)
+    x[1] = 1e-37 * np.linspace(-1, 1, 40)
+    x[2] = 1e15 * np.linspace(-1, 1, 40)
+    x[3, 7] = np.inf
+    x[4, 9] = np.nan
+    x[5, 3] = -2.5
+    q, s = cp.rms_norm_int8(cp.asarray(x))
+    q, s = q.get(), s.get()
+    assert np.all(q[0] == 0) and s[0] == 0
+    for row in (1, 2):
+        assert np.all(np.abs(q[row] - 127 * np.linspace(-1, 1, 40)) <= 0.5 + 1e-3)
+    assert np.isnan(s[3]) and np.isnan(s[4])
+    assert q[5, 3] == -127 and np.all(np.delete(q[5], 3) == 0)
+    y = cp.rms_norm(cp.asarray(x)).get()
+    assert np.all(y[0] == 0) and np.isnan(y[3, 7]) and np.all(np.delete(y[3], 7) == 0)
+    assert np.all(np.isnan(y[4]))
+
+
+def grad64(g, x, w, eps):
+    g, x = g.astype(np.float64), x.astype(np.float64)
+    a = g if w is None else g * w.astype(np.float64)
+    r = 1 / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+    n = x * r
+    dx = r * (a - n * (a * n).mean(-1, keepdims=True))
+    lead = tuple(range(x.ndim - 1))
+    # and the sizes of what is added up, for the bounds
+    size = np.abs(r * a) + np.abs(n) * r * np.abs(a * n).mean(-1, keepdims=True)
+    return dx, (g * n).sum(lead), size, np.abs(g * n).sum(lead)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_gradient(shape, dtype):
+    g, x = inputs(shape, dtype, 7), inputs(shape, dtype, 8, 2.0)
+    w, d = inputs(shape[-1:], dtype, 9), inputs(shape, dtype, 10)
+    u, out = acc_step(dtype), half_step(dtype)
+    rows = x.size // shape[-1]
+    off = 1.5 * terms(shape[-1]) + 10
+    for weight, extra in ((None, None), (w, None), (w, d), (None, d)):
+        got = cp.rms_norm_grad(cp.asarray(g), cp.asarray(x),
+                               None if weight is None else cp.asarray(weight), 1e-5,
+                               residual_grad=None if extra is None else cp.asarray(extra))
+        dx, dw, size, dw_size = grad64(g, x, weight, 1e-5)
+        if extra is not None:
+            dx = dx + extra.astype(np.float64)
+            size = size + np.abs(extra.astype(np.float64))
+        if weight is not None:
+            got, got_w = got
+            assert got_w.dtype == dtype
+            bound = out * np.abs(dw) + (rows + off) * u * dw_size + tiny(dtype)
+            assert np.all(np.abs(got_w.get().astype(np.float64) - dw) <= bound)
+        bound = out * np.abs(dx) + off * u * size + tiny(dtype)
+        assert np.all(np.abs(got.get().astype(np.float64) - dx) <= bound)
+
+
+@pytest.mark.parametrize('shape', [(4, 7), (3, 300), (2, 9000)])
+def test_gradient_against_differences(shape):
+    """f = sum(c * y) in float64: (f(x + h e) - f(x - h e)) / 2h, h = 1e-5, is off
+    by h^2 times a third derivative of order one and by 1e-16 |f| / h."""
+    x, w, c = inputs(shape, 'float64', 1), inputs(shape[-1:], 'float64', 2), inputs(shape, 'float64', 3)
+    r = inputs(shape, 'float64', 4)
+    dh = inputs(shape, 'float64', 5)
+
+    def loss(x, w):
+        y, h = cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r))
+        return float((y.get() * c).sum() + (h.get() * dh).sum())
+    _, h = cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r))
+    dx, dw = cp.rms_norm_grad(cp.asarray(c), h, cp.asarray(w), residual_grad=cp.asarray(dh))
+    dx, dw = dx.get(), dw.get()
+    step = 1e-5
+    rng = np.random.default_rng(0)
+    for _ in range(6):
+        at = tuple(rng.integers(0, n) for n in shape)
+        e = np.zeros(shape)
+        e[at] = step
+        diff = (loss(x + e, w) - loss(x - e, w)) / (2 * step)
+        assert abs(diff - dx[at]) <= 1e-6 * (1 + abs(dx[at]))
+        e = np.zeros(shape[-1:])
+        e[at[-1]] = step
+        diff = (loss(x, w + e) - loss(x, w - e)) / (2 * step)
+        assert abs(diff - dw[at[-1]]) <= 1e-6 * (1 + abs(dw[at[-1]]))
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_layouts(dtype):
+    """Windows, every second row, reversed and broadcast rows, transposed storage."""
+    big = inputs((40, 200), dtype, 1)
+    d = cp.asarray(big)
+    views = [(lambda a: a[3:30, 1:100]), (lambda a: a[::2, 5:69]), (lambda a: a[::-1, :64]),
+             (lambda a: a[:, ::3]), (lambda a: a.T), (lambda a: a.reshape(4, 10, 200)[:, ::2, 7:90]),
+             (lambda a: a.reshape(4, 10, 200).transpose(1, 0, 2))]
+    for view in views:
+        x, dx = np.ascontiguousarray(view(big)), view(d)
+        w, r = inputs(x.shape[-1:], dtype, 2), inputs(x.shape, dtype, 3)
+        y, h = cp.rms_norm(dx, cp.asarray(w), cp.asarray(r))
+        h64 = x.astype(np.float64) + r
+        check_norm(y.get(), norm64(h64, w, 1e-6), x.shape[-1], dtype)
+        # the results into windows of other arrays, which keep the rest
+        frame = cp.zeros(tuple(n + 3 for n in x.shape), dtype)
+        into = frame[tuple(slice(1, n + 1) for n in x.shape)]
+        again = cp.rms_norm(dx, cp.asarray(w), cp.asarray(r), out=into)
+        assert again[0] is into
+        assert np.array_equal(into.get(), y.get())
+        assert np.count_nonzero(frame.get()) == np.count_nonzero(y.get())
+        g = cp.rms_norm_grad(dx, dx, cp.asarray(w))
+        g2 = cp.rms_norm_grad(cp.asarray(x), cp.asarray(x), cp.asarray(w))
+        assert np.array_equal(g[0].get(), g2[0].get()) and np.array_equal(g[1].get(), g2[1].get())
+    row = cp.broadcast_to(d[0], (6, 200))
+    got = cp.rms_norm(row).get()
+    assert np.array_equal(got, np.broadcast_to(cp.rms_norm(d[:1]).get(), (6, 200)))
+
+
+@pytest.mark.parametrize('shape', [(50, 512), (4, 40000)])
+def test_outputs_on_inputs(shape):
+    x, w, r = inputs(shape, 'float16', 1), inputs(shape[-1:], 'float16', 2), inputs(shape, 'float16', 3)
+    want, want_h = (a.get() for a in cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r)))
+    wd = cp.asarray(w)
+    for _ in range(2):                # the second time from the record
+        xd, rd = cp.asarray(x), cp.asarray(r)
+        y, h = cp.rms_norm(xd, wd, rd, out=xd, residual_out=rd)
+        assert y is xd and h is rd
+        assert np.array_equal(xd.get(), want) and np.array_equal(rd.get(), want_h)
+    # overlapping by half: as if the inputs had been copied
+    store = cp.zeros((shape[0] + 1, shape[1]), 'float16')
+    store[:-1][...] = cp.asarray(x)
+    y, h = cp.rms_norm(store[:-1], wd, cp.asarray(r), out=store[1:])
+    assert np.array_equal(y.get(), want) and np.array_equal(h.get(), want_h)
+    for k in range(3):
+        args = [cp.asarray(x), cp.asarray(r), cp.asarray(x)]
+        plain = cp.rms_norm_grad(args[0], args[1], wd, residual_grad=args[2])
+        got = cp.rms_norm_grad(args[0], args[1], wd, residual_grad=args[2], out=args[k])
+        assert np.array_equal(got[0].get(), plain[0].get())
+        assert np.array_equal(got[1].get(), plain[1].get())
+
+
+def test_streams_and_repeated_calls():
+    x, w = inputs((2000, 768), 'float16', 1), inputs((768,), 'float16', 2)
+    g = inputs((2000, 768), 'float16', 3)
+    xd, wd, gd = cp.asarray(x), cp.asarray(w), cp.asarray(g)
+    first = [a.get() for a in cp.rms_norm_grad(gd, xd, wd)]
+    streams = [cp.cuda.Stream(non_blocking=True) for _ in range(2)]
+    results = []
+    for k in range(6):
+        with streams[k % 2]:
+            results.append(cp.rms_norm_grad(gd, xd, wd))
+    for s in streams:
+        s.synchronize()
+    for dx, dw in results:
+        assert np.array_equal(dx.get(), first[0]) and np.array_equal(dw.get(), first[1])
+
+
+def test_static_scratch():
+    x, w, g = (cp.asarray(inputs(s, 'float32', k)) for k, s in enumerate([(64, 300), (300,), (64, 300)]))
+    out, wout = cp.empty((64, 300), 'float32'), cp.empty((300,), 'float32')
+    want = [a.get() for a in cp.rms_norm_grad(g, x, w, out=out, weight_out=wout)]
+    out.fill(0), wout.fill(0)
+    with cp.cuda.memory.static_scratch():
+        cp.rms_norm_grad(g, x, w, out=out, weight_out=wout)
+    assert np.array_equal(out.get(), want[0]) and np.array_equal(wout.get(), want[1])
+    with cp.cuda.memory.static_scratch():
+        with pytest.raises(RuntimeError):
+            cp.rms_norm(x, w)
+
+
+def test_empty():
+    for shape in ((0, 5), (5, 0), (0,)):
+        x, w = cp.zeros(shape, 'float16'), cp.ones(shape[-1:], 'float16')
+        y, h = cp.rms_norm(x, w, x)
+        assert y.shape == shape and h.shape == shape
+        q, s = cp.rms_norm_int8(x, w)
+        assert q.shape == shape and s.shape == shape[:-1] and not s.get().any()
+        dx, dw = cp.rms_norm_grad(x, x, w)
+        assert dx.shape == shape and dw.shape == shape[-1:] and not dw.get().any()
+
+
+def test_rows_far_apart():
+    """Rows whose offsets pass 32 bits: a stride of 2**31 elements of float16."""
+    pitch = (1 << 31) + 8
+    buf = cp.empty(pitch + 512, 'float16')
+    rows = cp.ndarray((2, 512), 'float16', buf.data, strides=(pitch * 2, 2))
+    x = inputs((2, 512), 'float16', 1)
+    rows[...] = cp.asarray(x)
+    check_norm(cp.rms_norm(rows, out=rows).get(), norm64(x, None, 1e-6), 512, 'float16')

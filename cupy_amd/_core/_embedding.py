@@ -1,0 +1,597 @@
+"""Lookup of table rows with scaling, and its gradient summed by sorted tokens.
+
+``embedding`` gathers rows; ``embedding_grad`` adds the rows of a gradient that
+belong to the same row of the table.  Where ``ufunc.at`` would add atomically,
+in an order that changes from call to call, the gradient is summed in the order
+of the positions: the pairs (token, position) are sorted (a stable radix sort
+with the positions as its payload), cut into chunks of equal length whatever
+the tokens are, and every chunk sums its runs of equal tokens in registers.
+Runs that cross the border of a chunk leave partial sums that a last kernel
+joins, in order.  The reference scatters such gradients atomically
+(cupy/_core/_routines_indexing.pyx:899-1120 ``_scatter_op``).
+"""
+import operator
+
+import numpy
+
+from cupy_amd._core import _op_calls as _oc
+from cupy_amd._core._op_calls import Ref
+
+_LOOKUP = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<X_T>::type A;
+
+// LANES lanes share a row, each moves ITEMS vectors, all requested before the
+// first is stored; blockIdx.y walks the rest of a wide row.  Bound by memory:
+// nothing is computed but the product with the scale (none at all at 1, so
+// that NaN payloads stay).
+extern "C" __global__ void __launch_bounds__(256)
+cupy_embedding(const X_T* table, const I_T* ids, X_T* out, const long long n, const int width,
+               const long long rows, const long long pt, const long long po, const double scale) {
+  const int lane = threadIdx.x % LANES;
+  const long long step = (long long)gridDim.x * (256 / LANES);
+  for (long long t = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t < n; t += step) {
+    const long long id = ids[t];
+    const bool met = id >= 0 && id < rows;
+    cupy::Vec<X_T, VEC> v[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const long long c = ((long long)(blockIdx.y * ITEMS + k) * LANES + lane) * VEC;
+      if (c >= width) continue;
+      if (met) {
+        v[k] = cupy::load_part<X_T, VEC>(table + id * pt + c, width - c < VEC ? (int)(width - c) : VEC);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[k].v[e] = static_cast<X_T>(0.0f);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const long long c = ((long long)(blockIdx.y * ITEMS + k) * LANES + lane) * VEC;
+      if (c >= width) continue;
+#ifdef SCALE
+      if (met) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          v[k].v[e] = static_cast<X_T>(static_cast<A>(v[k].v[e]) * static_cast<A>(scale));
+      }
+#endif
+      cupy::store_part<X_T, VEC, NT_OUT>(out + t * po + c, v[k], width - c < VEC ? (int)(width - c) : VEC);
+    }
+  }
+}
+''')
+
+# -- the sort ---------------------------------------------------------------------------
+# A tile of ROUNDS * 1024 pairs belongs to a workgroup of 16 waves, a wave to
+# ROUNDS * 64 consecutive ones.  One pass of the sort by a digit: a wave finds
+# for each of its keys how many equal digits come before it in the wave (the
+# lanes of a round that share a digit are found with one ballot per bit of it),
+# the counts per wave and digit are turned into first places, and every pair
+# moves to its place.  Equal digits keep their order, so the sort is stable and
+# its result does not depend on the order in which anything runs.
+# One tile: all passes in one launch, the pairs stay in the LDS between them.
+# More tiles: a launch that counts and one that moves per pass.
+
+_GRAD = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<G_T>::type A;
+typedef unsigned int u32;
+
+constexpr int kThreads = 1024;
+constexpr int kWaves = 16;
+constexpr int kBins = 512;
+constexpr int kTile = ROUNDS * kThreads;
+
+struct Digits {
+  // per wave: how many, then the first place inside the digit (at most kTile)
+  unsigned short count[kWaves][kBins];
+  u32 first[kBins];           // first place of a digit
+  u32 wave_total[kWaves];
+};
+
+// The place of every key among the tile's keys of the same digit within the
+// wave, and count[][] filled in.
+_CUPY_DEV void count_digits(Digits& s, const u32 (&key)[ROUNDS], u32 (&place)[ROUNDS],
+                            int shift, int bits) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < kWaves * kBins; i += kThreads) s.count[i / kBins][i % kBins] = 0;
+  __syncthreads();
+  volatile unsigned short* mine = s.count[wave];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const u32 d = (key[r] >> shift) & ((1u << bits) - 1);
+    unsigned long long same = ~0ull;
+    for (int b = 0; b < bits; ++b) {
+      const unsigned long long set = __ballot((d >> b) & 1);
+      same &= ((d >> b) & 1) ? set : ~set;
+    }
+    const u32 before = __popcll(same & ((1ull << lane) - 1));
+    // (every lane reads the count of its digit before the first of the lanes
+    // that share it raises it: LDS accesses of a wave happen in program order)
+    const u32 had = mine[d];
+    place[r] = had + before;
+    __builtin_amdgcn_wave_barrier();
+    if (before == 0) mine[d] = static_cast<unsigned short>(had + __popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+}
+
+// count[w][d] becomes the number of d's in the waves before w; returns (to the
+// thread that has the number of the digit) how many there are in the tile.
+_CUPY_DEV u32 sum_waves(Digits& s) {
+  u32 total = 0;
+  if (threadIdx.x < kBins) {
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const u32 c = s.count[w][threadIdx.x];
+      s.count[w][threadIdx.x] = static_cast<unsigned short>(total);
+      total += c;
+    }
+  }
+  return total;
+}
+
+// Exclusive sums over the first kBins threads' values, plus `offset`, to first[].
+_CUPY_DEV void first_places(Digits& s, u32 value, u32 offset) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u32 v = value;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const u32 o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) s.wave_total[wave] = v;
+  __syncthreads();
+  u32 base = 0;
+  for (int w = 0; w < wave; ++w) base += s.wave_total[w];
+  if (threadIdx.x < kBins) s.first[threadIdx.x] = base + v - value + offset;
+  __syncthreads();
+}
+
+_CUPY_DEV u32 key_of(const I_T* ids, long long i, u32 rows) {
+  const long long id = ids[i];
+  return id >= 0 && id < (long long)rows ? (u32)id : rows;    // no row: behind all rows
+}
+
+// Zeros to every row of the result, by the workgroups from `first_block` on.
+_CUPY_DEV void clear_rows(O_T* out, u32 rows, int width, long long po, int first_block) {
+  const long long blocks = gridDim.x - first_block;
+  if (blocks <= 0) return;
+  cupy::Vec<O_T, FILL_VEC> zero;
+#pragma unroll
+  for (int e = 0; e < FILL_VEC; ++e) zero.v[e] = static_cast<O_T>(0.0f);
+  const bool dense = po == width;
+  const long long length = dense ? (long long)rows * width : width;
+  const long long lines = dense ? 1 : rows;
+  const long long me = (long long)(blockIdx.x - first_block) * kThreads + threadIdx.x;
+  const long long all = blocks * kThreads;
+  if (dense) {
+    const long long vecs = length / FILL_VEC;
+    for (long long i = me; i < vecs; i += all)
+      cupy::store_vec<O_T, FILL_VEC, NT_OUT>(out + i * FILL_VEC, zero);
+    if (me < length - vecs * FILL_VEC) out[vecs * FILL_VEC + me] = zero.v[0];
+  } else {
+    for (long long r = blockIdx.x - first_block; r < lines; r += blocks)
+      for (int c = threadIdx.x; c < width; c += kThreads) out[r * po + c] = zero.v[0];
+  }
+}
+
+// All tokens in one tile: sorted by workgroup 0 while the others clear the result.
+extern "C" __global__ void __launch_bounds__(kThreads)
+cupy_embedding_sort(const I_T* ids, u32* pairs, O_T* out, const int n, const u32 rows,
+                    const int width, const long long po, const int bits, const int passes) {
+  __shared__ Digits s;
+  __shared__ u32 keys[kTile], places[kTile];
+  if (blockIdx.x > 0) {
+    clear_rows(out, rows, width, po, 1);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = (wave * ROUNDS + r) * 64 + lane;
+    key[r] = i < n ? key_of(ids, i, rows) : 0xffffffffu;
+    pos[r] = i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    count_digits(s, key, place, p * bits, bits);
+    const u32 total = sum_waves(s);
+    first_places(s, total, 0);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const u32 d = (key[r] >> (p * bits)) & ((1u << bits) - 1);
+      const u32 to = s.first[d] + s.count[wave][d] + place[r];
+      keys[to] = key[r];
+      places[to] = pos[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = (wave * ROUNDS + r) * 64 + lane;
+      key[r] = keys[i];
+      pos[r] = places[i];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = (wave * ROUNDS + r) * 64 + lane;
+    if (i < n) {
+      pairs[i] = key[r];
+      pairs[n + i] = pos[r];
+    }
+  }
+}
+
+// Keys and positions of a pass over many tiles: the first pass reads the tokens.
+_CUPY_DEV void load_tile(const I_T* ids, const u32* from, u32 (&key)[ROUNDS], u32 (&pos)[ROUNDS],
+                         long long n, u32 rows, bool first) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const long long i = (long long)blockIdx.x * kTile + (wave * ROUNDS + r) * 64 + lane;
+    key[r] = 0xffffffffu;
+    pos[r] = (u32)i;
+    if (i < n) {
+      key[r] = first ? key_of(ids, i, rows) : from[i];
+      if (!first) pos[r] = from[n + i];
+    }
+  }
+}
+
+// counts[tile][digit]; workgroups behind the tiles clear the result (first pass).
+extern "C" __global__ void __launch_bounds__(kThreads)
+cupy_embedding_count(const I_T* ids, u32* temp, const long long from, const long long at_counts,
+                     O_T* out, const long long n, const u32 rows, const int width,
+                     const long long po, const int shift, const int bits, const int tiles) {
+  __shared__ Digits s;
+  if ((int)blockIdx.x >= tiles) {
+    clear_rows(out, rows, width, po, tiles);
+    return;
+  }
+  u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
+  load_tile(ids, temp + from, key, pos, n, rows, shift == 0);
+  count_digits(s, key, place, shift, bits);
+  const u32 total = sum_waves(s);
+  if (threadIdx.x < kBins) temp[at_counts + (long long)blockIdx.x * kBins + threadIdx.x] = total;
+}
+
+extern "C" __global__ void __launch_bounds__(kThreads)
+cupy_embedding_move(const I_T* ids, u32* temp, const long long from, const long long to_at,
+                    const long long at_counts, const long long n, const u32 rows, const int shift,
+                    const int bits, const int tiles) {
+  __shared__ Digits s;
+  u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
+  load_tile(ids, temp + from, key, pos, n, rows, shift == 0);
+  count_digits(s, key, place, shift, bits);
+  sum_waves(s);
+  // of all tiles, and of those before this one
+  u32 all = 0, before = 0;
+  if (threadIdx.x < kBins) {
+    const u32* c = temp + at_counts + threadIdx.x;
+    for (int t = 0; t < tiles; ++t) {
+      const u32 v = c[(long long)t * kBins];
+      all += v;
+      before += t < (int)blockIdx.x ? v : 0;
+    }
+  }
+  first_places(s, all, before);
+  u32* to = temp + to_at;
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const u32 d = (key[r] >> shift) & ((1u << bits) - 1);
+    const long long at = (long long)s.first[d] + s.count[wave][d] + place[r];
+    // (the filling of the last tile has the largest digit and the last places)
+    if (at < n) {
+      to[at] = key[r];
+      to[n + at] = pos[r];
+    }
+  }
+}
+''')
+
+_SUMS = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<G_T>::type A;
+typedef unsigned int u32;
+
+_CUPY_DEV void put(O_T* out, const A (&sum)[VEC], int have, A scale) {
+  cupy::Vec<O_T, VEC> v;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v.v[e] = static_cast<O_T>(sum[e] * scale);
+  cupy::store_part<O_T, VEC>(out, v, have);
+}
+
+// LANES lanes across the columns; a chunk of `chunk` sorted pairs to each such
+// group.  Rows of the gradient are requested UNROLL at a time.
+// partial[chunk][0]: the sum of a run that began in an earlier chunk;
+// partial[chunk][1]: of one that begins here and goes on behind the chunk.
+extern "C" __global__ void __launch_bounds__(256)
+cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
+                    const long long at_partial, const long long n, const u32 rows,
+                    const int width, const long long pg, const long long po, const int chunk,
+                    const int chunks, const double scale_) {
+  constexpr int UNROLL = 8;
+  const A scale = static_cast<A>(scale_);
+  const long long ch = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const long long c = ((long long)blockIdx.y * LANES + threadIdx.x % LANES) * VEC;
+  if (ch >= chunks || c >= width) return;
+  const int have = width - c < VEC ? (int)(width - c) : VEC;
+  const u32* keys = temp + at_pairs;
+  const u32* pos = keys + n;
+  A* partial = reinterpret_cast<A*>(temp + at_partial);
+  const long long t0 = ch * chunk;
+  const long long t1 = t0 + chunk < n ? t0 + chunk : n;
+  u32 cur = keys[t0];
+  if (cur >= rows) return;
+  bool head = t0 > 0 && keys[t0 - 1] == cur;
+  A sum[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[e] = A(0);
+  A* mine = partial + ch * 2 * width + c;
+  for (long long t = t0; t < t1; t += UNROLL) {
+    u32 key[UNROLL];
+    cupy::Vec<G_T, VEC> v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      key[u] = t + u < t1 ? keys[t + u] : 0xffffffffu;
+      if (key[u] < rows) v[u] = cupy::load_part<G_T, VEC>(g + (long long)pos[t + u] * pg + c, have);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (t + u >= t1) break;
+      if (key[u] != cur) {
+        if (cur < rows) {
+          if (head) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (e < have) mine[e] = sum[e];
+          } else {
+            put(out + (long long)cur * po + c, sum, have, scale);
+          }
+        }
+        head = false;
+        cur = key[u];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] = A(0);
+      }
+      if (cur < rows) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] += static_cast<A>(v[u].v[e]);
+      }
+    }
+  }
+  if (cur >= rows) return;
+  const bool on = t1 < n && keys[t1] == cur;
+  if (!head && !on) {
+    put(out + (long long)cur * po + c, sum, have, scale);
+  } else {
+    A* to = head ? mine : mine + width;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) if (e < have) to[e] = sum[e];
+  }
+}
+
+// The runs that cross chunks, each by the workgroups of the chunk it begins
+// in: 64 columns by 4 slices of the chunks it goes on through.
+extern "C" __global__ void __launch_bounds__(256)
+cupy_embedding_join(const u32* temp, O_T* out, const long long at_pairs,
+                    const long long at_partial, const long long n, const u32 rows,
+                    const int width, const long long po, const int chunk, const int chunks,
+                    const double scale) {
+  __shared__ A lds[4][64];
+  const u32* keys = temp + at_pairs;
+  const A* partial = reinterpret_cast<const A*>(temp + at_partial);
+  const long long ch = blockIdx.x;
+  const long long t0 = ch * chunk, t1 = t0 + chunk;
+  if (t1 >= n) return;
+  const u32 cur = keys[t1];
+  if (cur >= rows || keys[t1 - 1] != cur) return;
+  if (t0 > 0 && keys[t0 - 1] == cur) return;       // it began before this chunk
+  // last chunk that begins with `cur`: doubled steps, then halved ones
+  long long lo = ch + 1, step = 1;
+  while (lo + step < chunks && keys[(lo + step) * chunk] == cur) {
+    lo += step;
+    step <<= 1;
+  }
+  for (; step > 0; step >>= 1)
+    if (lo + step < chunks && keys[(lo + step) * chunk] == cur) lo += step;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int c = blockIdx.y * 64 + tx;
+  A t = A(0);
+  if (c < width) {
+    if (ty == 0) t = partial[(ch * 2 + 1) * width + c];
+    for (long long j = ch + 1 + ty; j <= lo; j += 4) t += partial[j * 2 * width + c];
+  }
+  lds[ty][tx] = t;
+  __syncthreads();
+  if (ty == 0 && c < width)
+    out[(long long)cur * po + c] = static_cast<O_T>(
+        (((lds[0][tx] + lds[1][tx]) + lds[2][tx]) + lds[3][tx]) * static_cast<A>(scale));
+}
+''')
+
+_plans = {}
+_plans_grad = {}
+
+
+def _check_width(width):
+    if width >= 1 << 22:       # (a grid's second dimension)
+        raise ValueError('rows of 2**22 elements and more are not supported')
+
+
+def embedding(table, ids, scale=1.0, *, out=None):
+    """Rows of a table, scaled: ``out[...] = scale * table[ids[...]]``.
+
+    An id outside ``[0, len(table))`` selects no row: its row of the result is
+    zeros (padding may be marked with -1).
+
+    Args:
+        table (cupy.ndarray): float16, float32 or float64 matrix.
+        ids: integers of any shape.
+        scale (float): factor; the product is rounded once.
+        out (cupy.ndarray): receives the result, of shape
+            ``ids.shape + (table.shape[1],)`` and the table's type.
+    """
+    scale = float(scale)
+    arrays = [table, ids] if out is None else [table, ids, out]
+    result, key = _oc.replay(_plans, arrays, (scale, len(arrays)))
+    if result is not _oc._NOTHING:
+        return result
+    _oc.check_float(table, 'table')
+    if table.ndim != 2:
+        raise ValueError('table must have two dimensions, got %d' % table.ndim)
+    given, ids = ids, _oc.index_array(ids, 'ids')
+    if given is not ids:
+        key, arrays[1] = None, ids
+    rows, width = table._shape
+    shape = ids._shape + (width,)
+    _check_width(width)
+    if out is not None:
+        _oc.check_out(out, shape, table.dtype)
+    call = _oc.Call(_plans, key, arrays, 2)
+    i_out = 2 if out is not None else call.allocate(shape, table.dtype)
+    n = ids.size
+    if n == 0 or width == 0:
+        call.key = None
+        call.begin()
+        return call.finish(i_out)
+    call.convert(1, _oc.as_index(call.refs[1]))
+    pt, po = call.rows(0), call.rows(i_out)
+    call.begin()
+    vec = 16 // table.dtype.itemsize
+    vecs = -(-width // vec)
+    lanes = min(256, max(4, _oc.clp2(vecs)))
+    # Few rows: a vector per lane and the row over more workgroups, so that all
+    # of it is requested at once.
+    items = 1 if n * vecs < _oc.compute_units() * 2048 else min(4, -(-vecs // lanes))
+    grid_y = -(-vecs // (lanes * items))
+    per = 256 // lanes
+    grid_x = min(-(-n // per), (1 << 24) - 1)
+    nt_out = _oc.stream_hints(n * width * table.dtype.itemsize, n * width * table.dtype.itemsize)[1]
+    defines = dict(X_T=table.dtype, I_T=call.refs[1].dtype, LANES=lanes, ITEMS=items, VEC=vec,
+                   NT_OUT=nt_out)
+    if scale != 1.0:
+        defines['SCALE'] = 1
+    fn = _LOOKUP.function('cupy_embedding', **defines)
+    call.launch(fn, (grid_x, grid_y, 1), 256, 'PPPqiqqqd', Ref(0), Ref(1), Ref(i_out), n, width,
+                rows, pt, po, scale)
+    return call.finish(i_out)
+
+
+def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
+    """Gradient of :func:`embedding` with respect to its table.
+
+    ``out[v] = scale * (sum of grad[t] over all t with ids[t] == v)``; rows
+    that no id selects are zeros, ids outside ``[0, num_rows)`` have no part.
+    The sums are held in 32 bits (64 for float64), their order is fixed:
+    repeated calls give the same bits.
+
+    Args:
+        grad (cupy.ndarray): gradient of the looked up rows, of shape
+            ``ids.shape + (width,)``; float16, float32 or float64.
+        ids: integers, as in the forward call.
+        num_rows (int): rows of the table.
+        scale (float): as in the forward call.
+        dtype: type of the result; the gradient's (default), or float32 with
+            float16.
+        out (cupy.ndarray): receives the result, ``(num_rows, width)``; not
+            both ``out`` and ``dtype``.
+    """
+    scale = float(scale)
+    arrays = [grad, ids] if out is None else [grad, ids, out]
+    result, key = _oc.replay(_plans_grad, arrays, (scale, len(arrays), num_rows, dtype))
+    if result is not _oc._NOTHING:
+        return result
+    _oc.check_float(grad, 'grad')
+    given, ids = ids, _oc.index_array(ids, 'ids')
+    if given is not ids:
+        key, arrays[1] = None, ids
+    if grad.ndim != ids.ndim + 1 or grad._shape[:-1] != ids._shape:
+        raise ValueError('grad has the shape %r, ids the shape %r: one row per id is expected'
+                         % (grad._shape, ids._shape))
+    num_rows = operator.index(num_rows)
+    if not 0 <= num_rows < (1 << 31) - 1:
+        raise ValueError('num_rows must be at least 0 and below 2**31 - 1')
+    width = grad._shape[-1]
+    n = ids.size
+    _check_width(width)
+    if n >= 1 << 31:
+        raise ValueError('2**31 ids and more are not supported')
+    if out is not None:
+        if dtype is not None:
+            raise TypeError('embedding_grad() takes `out` or `dtype`, but both were provided.')
+        _oc.check_array(out, 'out')
+        dt = out.dtype
+    else:
+        dt = grad.dtype if dtype is None else numpy.dtype(dtype)
+    if dt != grad.dtype and not (grad.dtype.char == 'e' and dt.char == 'f'):
+        raise TypeError('a gradient of type %s is not summed into %s: its own type, or float32 '
+                        'with float16' % (grad.dtype, dt))
+    if out is not None:
+        _oc.check_out(out, (num_rows, width), dt)
+    call = _oc.Call(_plans_grad, key, arrays, 2)
+    i_out = 2 if out is not None else call.allocate((num_rows, width), dt)
+    if num_rows == 0 or width == 0 or n == 0:
+        call.key = None
+        if call.refs[i_out].size:
+            call.refs[i_out].fill(0)
+        call.begin()
+        return call.finish(i_out)
+    call.convert(1, _oc.as_index(call.refs[1]))
+    pg, po = call.rows(0), call.rows(i_out)
+    call.begin()
+    out_vec = 16 // dt.itemsize
+    nt_out = _oc.stream_hints(num_rows * width * dt.itemsize, num_rows * width * dt.itemsize)[1]
+    acc = _oc.acc_dtype(grad.dtype).itemsize
+
+    # chunks: long enough that few runs cross their borders, short enough that
+    # there are some per compute unit
+    chunk = min(128, max(8, _oc.clp2(n // 512)))
+    chunks = -(-n // chunk)
+    # the temporary: sorted pairs (twice for many tiles), counts, partial sums
+    rounds = 1
+    while rounds < 16 and rounds * 1024 < n:
+        rounds *= 2
+    tiles = -(-n // (rounds * 1024))
+    key_bits = num_rows.bit_length()
+    passes = -(-key_bits // 9)
+    bits = -(-key_bits // passes)
+    words = 2 * n if tiles == 1 else 4 * n + tiles * 512
+    words += words & 1
+    i_t = call.temp(words * 4 + chunks * 2 * width * acc)
+    # workgroups that clear the result while it is sorted
+    fill = min(_oc.compute_units(), -(-num_rows * width // (out_vec * 1024)))
+    defines = dict(G_T=grad.dtype, O_T=dt, I_T=call.refs[1].dtype, ROUNDS=rounds,
+                   FILL_VEC=out_vec, NT_OUT=nt_out)
+    at = 0
+    if tiles == 1:
+        fn = _GRAD.function('cupy_embedding_sort', **defines)
+        call.launch(fn, (1 + fill, 1, 1), 1024, 'PPPiIiqii', Ref(1), Ref(i_t), Ref(i_out), n,
+                    num_rows, width, po, bits, passes)
+    else:
+        count = _GRAD.function('cupy_embedding_count', **defines)
+        move = _GRAD.function('cupy_embedding_move', **defines)
+        at = 2 * n
+        for p in range(passes):
+            src, at = at, 2 * n - at
+            call.launch(count, (tiles + (fill if p == 0 else 0), 1, 1), 1024, 'PPqqPqIiqiii',
+                        Ref(1), Ref(i_t), src, 4 * n, Ref(i_out), n, num_rows, width, po,
+                        p * bits, bits, tiles)
+            call.launch(move, (tiles, 1, 1), 1024, 'PPqqqqIiii', Ref(1), Ref(i_t), src, at, 4 * n,
+                        n, num_rows, p * bits, bits, tiles)
+    vec = 16 // grad.dtype.itemsize
+    lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
+    defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec)
+    fn = _SUMS.function('cupy_embedding_sums', **defines)
+    call.launch(fn, (-(-chunks // (256 // lanes)), -(-width // (lanes * vec)), 1), 256,
+                'PPPqqqIiqqiid', Ref(0), Ref(i_t), Ref(i_out), at, words, n, num_rows, width,
+                pg, po, chunk, chunks, scale)
+    if chunks > 1:
+        fn = _SUMS.function('cupy_embedding_join', **defines)
+        call.launch(fn, (chunks, -(-width // 64), 1), 256, 'PPqqqIiqiid', Ref(i_t), Ref(i_out),
+                    at, words, n, num_rows, width, po, chunk, chunks, scale)
+    return call.finish(i_out)

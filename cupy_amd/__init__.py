@@ -102,6 +102,8 @@ from cupy_amd._core._routines_logic import all, any  # noqa
 from cupy_amd._core._scan import cumsum, cumprod, nancumsum, nancumprod  # noqa
 from cupy_amd._core._embedding import embedding, embedding_grad  # noqa
 from cupy_amd._core._rms_norm import rms_norm, rms_norm_int8, rms_norm_grad  # noqa
+from cupy_amd._core._token_log_prob import (  # noqa
+    token_log_prob, token_log_prob_grad, TokenLogProb)
 from cupy_amd._creation import (  # noqa
     empty, empty_like, zeros, zeros_like, ones, ones_like, full, full_like, arange)
 

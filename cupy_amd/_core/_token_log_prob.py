@@ -1,0 +1,708 @@
+"""Log probabilities of given tokens, with entropy and top alternatives, and
+their gradient.
+
+For a row of logits ``x`` and a token ``t``: ``lse = log(sum(exp(x)))``,
+``log_prob = x[t] - lse``, ``entropy = -sum(p * log(p))`` with
+``p = exp(x - lse)``.  All of them, and the ``top`` likeliest tokens, come from
+one pass over the row with a running maximum ``m``, the sum ``s`` of
+``exp(x - m)`` and, for the entropy, the sum ``u`` of ``(x - m) * exp(x - m)``:
+``lse = m + log(s)``, ``entropy = log(s) - u / s``.  The reference composes
+them from reductions (cupyx/scipy/special/_softmax.py, _logsumexp.py).
+"""
+import collections
+
+import numpy
+
+from cupy_amd._core import _op_calls as _oc
+from cupy_amd._core._op_calls import Ref
+
+TokenLogProb = collections.namedtuple(
+    'TokenLogProb', ['log_prob', 'lse', 'entropy', 'top_log_prob', 'top_token'])
+TokenLogProb.__doc__ = """What :func:`token_log_prob` returns (None where not asked for)."""
+
+MAX_TOP = 32
+
+_COMMON = r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<X_T>::type A;
+typedef unsigned int u32;
+
+#define LOG2E 1.4426950408889634
+#define LN2 0.6931471805599453
+
+_CUPY_DEV float exp2_(float t) { return __builtin_amdgcn_exp2f(t); }
+_CUPY_DEV double exp2_(double t) { return exp2(t); }
+_CUPY_DEV float max_(float a, float b) { return __builtin_fmaxf(a, b); }
+_CUPY_DEV double max_(double a, double b) { return __builtin_fmax(a, b); }
+template <typename T> struct lowest;
+template <> struct lowest<float16> { static _CUPY_DEV A value() { return A(-65504.0f); } };
+template <> struct lowest<float> { static _CUPY_DEV A value() { return A(-3.4028234663852886e38f); } };
+template <> struct lowest<double> { static _CUPY_DEV A value() { return A(-1.7976931348623157e308); } };
+
+// A row is seen as vectors of 16 bytes that start on 16-byte borders whatever
+// the row starts on: the first and the last may hang over its ends.
+struct RowVecs {
+  const X_T* x;
+  int phase;        // elements of the first vector that lie before the row
+  int width;
+  _CUPY_DEV RowVecs(const X_T* row, int w) : x(row), width(w) {
+    phase = (int)((reinterpret_cast<unsigned long long>(row) & 15) / sizeof(X_T));
+  }
+  _CUPY_DEV long long count() const { return ((long long)phase + width + VEC - 1) / VEC; }
+  _CUPY_DEV long long column(long long j) const { return j * VEC - phase; }
+  // elements outside the row are -inf: they add nothing and are never the best
+  _CUPY_DEV cupy::Vec<X_T, VEC> load(long long j) const {
+    const long long c = column(j);
+    if (c >= 0 && c + VEC <= width) return cupy::load_vec<X_T, VEC, NT_IN>(x + c);
+    cupy::Vec<X_T, VEC> v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      v.v[e] = c + e >= 0 && c + e < width ? x[c + e] : static_cast<X_T>(-__builtin_inff());
+    return v;
+  }
+};
+
+// Running statistics.  The maximum starts at the type's lowest value, not at
+// -inf, so that x - m is never inf - inf: masked rows need no case of their own.
+// float16: 2^(x log2e - m log2e) takes one fused multiply-add per element; the
+// rounded m log2e is what is added back at the end, so its rounding cancels.
+// float32: m log2e may overflow, and x - m is exact where it matters.
+struct Run {
+  A m, s, u;
+  _CUPY_DEV static bool half() { return sizeof(X_T) == 2; }
+  _CUPY_DEV A base() const { return half() ? m * A(LOG2E) : m; }
+  _CUPY_DEV static A power(A x, A base) {
+    return half() ? cupy::fma_(x, A(LOG2E), -base) : (x - base) * A(LOG2E);
+  }
+  // ... the same of another maximum, kept finite (0 * -inf)
+  _CUPY_DEV A below(A to) const {
+    const A d = half() ? m * A(LOG2E) - to * A(LOG2E) : (m - to) * A(LOG2E);
+    return max_(d, A(-30000));
+  }
+  _CUPY_DEV void lift(A to) {
+    const A t = below(to), f = exp2_(t);
+    u = f * cupy::fma_(s, t, u);
+    s *= f;
+    m = to;
+  }
+  _CUPY_DEV double log2_sum() const { return log2((double)s); }
+  _CUPY_DEV double lse() const {
+    if (s == A(0)) return -__builtin_inf();          // every element is -inf
+    if (half()) return ((double)(m * A(LOG2E)) + log2_sum()) / (double)A(LOG2E);
+    return (double)m + log2_sum() * LN2;
+  }
+  _CUPY_DEV double entropy() const {
+    if (s == A(0)) return 0.0;
+    return (log2_sum() - (double)u / (double)s) * LN2;
+  }
+};
+struct JoinRun {
+  _CUPY_DEV Run operator()(Run a, Run b) const {
+    const A top = max_(a.m, b.m);
+    a.lift(top);
+    b.lift(top);
+    a.s += b.s;
+    a.u += b.u;
+    return a;
+  }
+};
+
+#if TOP > 0
+// A value and its column; of equal values the lower column comes first.
+struct Key {
+  A v;
+  u32 i;
+};
+constexpr u32 kNone = 0xffffffffu;
+_CUPY_DEV bool better(const Key& a, const Key& b) {
+  return (a.v > b.v) | ((a.v == b.v) & (a.i < b.i));
+}
+_CUPY_DEV Key no_key() {
+  Key k;
+  k.v = -__builtin_inff();
+  k.i = kNone;
+  return k;
+}
+struct BestKey {
+  _CUPY_DEV Key operator()(const Key& a, const Key& b) const {
+    const bool t = better(b, a);
+    Key k;
+    k.v = t ? b.v : a.v;
+    k.i = t ? b.i : a.i;
+    return k;
+  }
+};
+
+constexpr int kMost = 1024;     // keys that are ranked against each other
+
+struct TopState {
+  Key sample[64];
+  Key key[kMost];
+  Key last;
+  u32 n;
+};
+
+// The TOP-th best of the 64 sample keys: at least TOP keys are as good.
+_CUPY_DEV Key bar(const TopState& t) {
+  const int lane = threadIdx.x & 63;
+  const Key me = t.sample[lane];
+  int rank = 0;
+  for (int o = 0; o < 64; ++o) {
+    const Key k = t.sample[o];
+    rank += better(k, me) | ((k.i == me.i) & (k.v == me.v) & (o < lane));
+  }
+  const int src = __ffsll(__ballot(rank == TOP - 1)) - 1;
+  return cupy::shfl_idx(me, src);
+}
+
+_CUPY_DEV void offer(TopState& t, const Key& k, const Key& least) {
+  if (better(least, k) | !(k.v == k.v)) return;
+  const u32 at = atomicAdd(&t.n, 1u);
+  if (at < kMost) t.key[at] = k;
+}
+#endif
+'''
+
+_SOURCE = _oc.Source(_COMMON + r'''
+#if TOP > 0
+// Writes the n <= kMost keys collected in t by rank, the best TOP of them.
+template <typename Put>
+_CUPY_DEV void put_ranked(const TopState& t, u32 n, Put put) {
+  for (u32 q = threadIdx.x; q < n; q += blockDim.x) {
+    const Key me = t.key[q];
+    int rank = 0;
+    for (u32 o = 0; o < n; ++o) rank += better(t.key[o], me);
+    if (rank < TOP) put(rank, me);
+  }
+  // (fewer elements than TOP: the rest of the places hold nothing)
+  for (u32 q = n + threadIdx.x; q < TOP; q += blockDim.x) put(q, no_key());
+}
+#endif
+
+struct Outputs {
+  A* log_prob;
+  A* lse;
+  A* entropy;
+  A* top;
+  long long* index;
+};
+
+// A row's results from its joined statistics, by one thread.
+_CUPY_DEV void put_row(const Outputs& o, const Run& run, const X_T* x, const I_T* tokens,
+                       long long row, int width) {
+  const double lse = run.lse();
+  o.lse[row] = static_cast<A>(lse);
+  const long long token = tokens[row];
+  double lp = 0.0;
+  if (token >= 0 && token < width) {
+    const double at = static_cast<double>(static_cast<A>(x[token]));
+    lp = run.s == A(0) ? at : at - lse;        // (a row of -inf: -inf, not NaN)
+  }
+  o.log_prob[row] = static_cast<A>(lp);
+#ifdef ENTROPY
+  o.entropy[row] = static_cast<A>(run.entropy());
+#endif
+}
+#if TOP > 0
+_CUPY_DEV void put_top(const Outputs& o, const Run& run, long long row, int rank, const Key& k) {
+  const double lse = run.lse();
+  const bool nan = !(run.s == run.s);          // no order in a row with NaN or +inf
+  o.top[row * TOP + rank] =
+      nan ? static_cast<A>(run.s) : static_cast<A>(run.s == A(0) ? (double)k.v : (double)k.v - lse);
+  o.index[row * TOP + rank] = nan ? -1 : (long long)k.i;
+}
+#endif
+
+// A workgroup per part of a row (PARTS == 1: the whole row, with its results).
+// Bound by memory: a vector costs a compare of its maximum, and per element a
+// multiply-add, an exponential (a quarter of the rate) and one or two
+// additions; the rescaling by a new maximum is taken only when a vector has one.
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy, A* top,
+                    long long* index, A* runs, const long long rows, const int width,
+                    const long long pitch, const int parts, const long long at_keys) {
+  __shared__ Run lds[BLOCK / 64];
+#if TOP > 0
+  __shared__ TopState ts;
+#endif
+  Outputs out;
+  out.log_prob = log_prob;
+  out.lse = lse;
+  out.entropy = entropy;
+  out.top = top;
+  out.index = index;
+  for (long long w = blockIdx.x; w < rows * parts; w += gridDim.x) {
+    const long long row = parts == 1 ? w : w / parts;
+    const int part = parts == 1 ? 0 : (int)(w - row * parts);
+    const X_T* x = logits + row * pitch;
+    const RowVecs vecs(x, width);
+    const long long n = vecs.count();
+    const long long share = (n + parts - 1) / parts;
+    const long long j0 = part * share + threadIdx.x;
+    const long long j1 = (part + 1) * share < n ? (part + 1) * share : n;
+    Run run;
+    run.m = lowest<X_T>::value();
+    run.s = run.u = A(0);
+    A base = run.base();
+#if TOP > 0
+    A best = -__builtin_inff();
+    long long best_at = j0;
+#endif
+    for (long long j = j0; j < j1; j += (long long)BLOCK * UNROLL) {
+      cupy::Vec<X_T, VEC> v[UNROLL];
+#pragma unroll
+      for (int k = 0; k < UNROLL; ++k)
+        if (j + k * BLOCK < j1) v[k] = vecs.load(j + k * BLOCK);
+#pragma unroll
+      for (int k = 0; k < UNROLL; ++k) {
+        if (j + k * BLOCK >= j1) break;
+        A e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = static_cast<A>(v[k].v[i]);
+        A vm = e[0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) vm = max_(vm, e[i]);
+#if TOP > 0
+        if (vm > best) {
+          best = vm;
+          best_at = j + k * BLOCK;
+        }
+#endif
+        if (vm > run.m) {
+          run.lift(vm);
+          base = run.base();
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const A t = Run::power(e[i], base), p = exp2_(t);
+          run.s += p;
+#ifdef ENTROPY
+          run.u = cupy::fma_(max_(t, A(-30000)), p, run.u);
+#endif
+        }
+      }
+    }
+    run = cupy::row_allreduce<BLOCK, BLOCK>(run, JoinRun(), lds);
+    if (threadIdx.x == 0) {
+      if (parts == 1) {
+        put_row(out, run, x, tokens, row, width);
+      } else {
+        A* to = runs + w * 3;
+        to[0] = run.m;
+        to[1] = run.s;
+        to[2] = run.u;
+      }
+    }
+#if TOP > 0
+    // The best key of every thread, then of 64 groups of threads.
+    Key mine = no_key();
+    if (j0 < j1) {
+      const cupy::Vec<X_T, VEC> v = vecs.load(best_at);
+      const long long c = vecs.column(best_at);
+#pragma unroll
+      for (int i = VEC - 1; i >= 0; --i)
+        if (c + i >= 0 && c + i < width && static_cast<A>(v.v[i]) == best) {
+          mine.v = best;
+          mine.i = (u32)(c + i);
+        }
+    }
+    const Key group = cupy::group_allreduce<BLOCK / 64>(mine, BestKey());
+    if (threadIdx.x % (BLOCK / 64) == 0) ts.sample[threadIdx.x / (BLOCK / 64)] = group;
+    if (threadIdx.x == 0) ts.n = 0;
+    __syncthreads();
+    const Key least = bar(ts);
+    // whoever may hold one of the best looks through its vectors again
+    if (!better(least, mine)) {
+      for (long long j = j0; j < j1; j += BLOCK) {
+        const cupy::Vec<X_T, VEC> v = vecs.load(j);
+        const long long c = vecs.column(j);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (c + i < 0 || c + i >= width) continue;
+          Key k;
+          k.v = static_cast<A>(v.v[i]);
+          k.i = (u32)(c + i);
+          offer(ts, k, least);
+        }
+      }
+    }
+    __syncthreads();
+    const u32 found = ts.n;
+    A* key_values = runs + at_keys + w * TOP;
+    u32* key_columns = reinterpret_cast<u32*>(runs + at_keys + rows * parts * TOP) + w * TOP;
+    auto put = [&](int rank, const Key& k) {
+      if (parts == 1) {
+        put_top(out, run, row, rank, k);
+      } else {
+        key_values[rank] = k.v;
+        key_columns[rank] = k.i;
+      }
+    };
+    if (found <= kMost) {
+      put_ranked(ts, found, put);
+    } else {
+      // More than can be ranked (the best lie in the vectors of a few threads):
+      // one pass over the row per place, each for the best behind the last.
+      if (threadIdx.x == 0) {
+        ts.last.v = __builtin_inff();
+        ts.last.i = 0;
+      }
+      bool first = true;
+      for (int rank = 0; rank < TOP; ++rank) {
+        __syncthreads();
+        const Key last = ts.last;
+        Key b = no_key();
+        for (long long j = j0; j < j1; j += BLOCK) {
+          const cupy::Vec<X_T, VEC> v = vecs.load(j);
+          const long long c = vecs.column(j);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            if (c + i < 0 || c + i >= width) continue;
+            Key k;
+            k.v = static_cast<A>(v.v[i]);
+            k.i = (u32)(c + i);
+            if ((first | better(last, k)) & better(k, b)) b = k;
+          }
+        }
+        first = false;
+        b = cupy::group_allreduce<64>(b, BestKey());
+        if ((threadIdx.x & 63) == 0) ts.key[threadIdx.x >> 6] = b;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          for (int q = 1; q < BLOCK / 64; ++q) b = BestKey()(b, ts.key[q]);
+          ts.last = b;
+          put(rank, b);
+        }
+      }
+    }
+#endif
+    __syncthreads();
+  }
+}
+
+// The parts of a row joined: a workgroup per row, at most 64 parts.
+extern "C" __global__ void __launch_bounds__(256)
+cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy,
+                         A* top, long long* index, const A* runs, const long long rows,
+                         const int width, const long long pitch, const int parts,
+                         const long long at_keys) {
+#if TOP > 0
+  __shared__ TopState ts;
+  if (threadIdx.x == 0) ts.n = 0;
+#endif
+  Outputs out;
+  out.log_prob = log_prob;
+  out.lse = lse;
+  out.entropy = entropy;
+  out.top = top;
+  out.index = index;
+  const long long row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  Run run;
+  run.m = lowest<X_T>::value();
+  run.s = run.u = A(0);
+  if (lane < parts) {
+    const A* from = runs + (row * parts + lane) * 3;
+    run.m = from[0];
+    run.s = from[1];
+    run.u = from[2];
+  }
+  run = cupy::group_allreduce<64>(run, JoinRun());     // (by every wave for itself)
+  if (threadIdx.x == 0) put_row(out, run, logits + row * pitch, tokens, row, width);
+#if TOP > 0
+  const A* key_values = runs + at_keys + row * parts * TOP;
+  const u32* key_columns =
+      reinterpret_cast<const u32*>(runs + at_keys + rows * parts * TOP) + row * parts * TOP;
+  // Every part's keys are in order: the first few of each are the sample.
+  const int each = 64 / parts < TOP ? 64 / parts : TOP;
+  if (threadIdx.x < 64) {
+    Key k = no_key();
+    if (lane < parts * each) {
+      const int at = (lane / each) * TOP + lane % each;
+      k.v = key_values[at];
+      k.i = key_columns[at];
+    }
+    ts.sample[lane] = k;
+  }
+  __syncthreads();
+  const Key least = bar(ts);
+  for (int q = threadIdx.x; q < parts * TOP; q += 256) {
+    Key k;
+    k.v = key_values[q];
+    k.i = key_columns[q];
+    if (k.i != kNone) offer(ts, k, least);
+  }
+  __syncthreads();
+  put_ranked(ts, ts.n < kMost ? ts.n : kMost,
+             [&](int rank, const Key& k) { put_top(out, run, row, rank, k); });
+#endif
+}
+''')
+
+_GRAD = _oc.Source(_COMMON + r'''
+// d x_j = g (delta_jt - p_j) - gH p_j (log p_j + H).  Bound by memory: read
+// once, written once, whatever the row starts on (RowVecs); the target's column
+// is found by comparing vector numbers.
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_token_log_prob_grad(const A* g, const X_T* logits, const I_T* tokens, const A* lse,
+                         const A* entropy, const A* entropy_grad, X_T* out,
+                         const long long rows, const int width, const long long pitch,
+                         const long long po, const int blocks) {
+  for (long long w = blockIdx.x; w < rows * blocks; w += gridDim.x) {
+    const long long row = w / blocks;
+    const int block = (int)(w - row * blocks);
+    const RowVecs vecs(logits + row * pitch, width);
+    const long long n = vecs.count();
+    X_T* to = out + row * po;
+    const A norm = lse[row];
+    const long long token = tokens[row];
+    const bool met = token >= 0 && token < width;
+    const A gain = met ? g[row] : A(0);
+#ifdef ENTROPY
+    const A gh = entropy_grad[row], h = entropy[row];
+#endif
+    const long long base = (long long)block * BLOCK * UNROLL + threadIdx.x;
+    cupy::Vec<X_T, VEC> v[UNROLL];
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k)
+      if (base + k * BLOCK < n) v[k] = vecs.load(base + k * BLOCK);
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const long long j = base + k * BLOCK;
+      if (j >= n) break;
+      const long long c = vecs.column(j);
+      const long long hit = met ? token - c : -1;
+      cupy::Vec<X_T, VEC> d;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A x = static_cast<A>(v[k].v[e]);
+        const A lp = x - norm, p = exp2_(lp * A(LOG2E));
+#ifdef ENTROPY
+        // (p = 0 where log p = -inf: kept finite, so that the product is 0)
+        A r = -p * cupy::fma_(gh, max_(lp, A(-1e30)) + h, gain);
+#else
+        A r = -p * gain;
+#endif
+        if (hit == e) r += gain;
+        // a row with nothing left has no distribution to change
+        d.v[e] = static_cast<X_T>(norm == -__builtin_inff() ? A(0) : r);
+      }
+      if (c >= 0 && c + VEC <= width) {
+        cupy::store_vec<X_T, VEC, NT_OUT>(to + c, d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) if (c + e >= 0 && c + e < width) to[c + e] = d.v[e];
+      }
+    }
+  }
+}
+''')
+
+_plans = {}
+_plans_grad = {}
+
+
+def _check_logits(logits, tokens):
+    _oc.check_float(logits, 'logits')
+    if logits.ndim == 0:
+        raise ValueError('logits must have at least one dimension')
+    if tokens._shape != logits._shape[:-1]:
+        raise ValueError('tokens has the shape %r, logits the shape %r: one token per row is '
+                         'expected' % (tokens._shape, logits._shape))
+    width = logits._shape[-1]
+    if width >= 1 << 31:
+        raise ValueError('rows of 2**31 elements and more are not supported')
+    if width == 0 and tokens.size:
+        raise ValueError('zero-size rows of logits have no distribution')
+    return width
+
+
+def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
+    """Log probability of one token per row of logits.
+
+    Args:
+        logits (cupy.ndarray): float16, float32 or float64, ``(..., n)``;
+            elements of -inf are ruled out.
+        tokens: integers of shape ``logits.shape[:-1]``.  A token outside
+            ``[0, n)`` marks a row without a target: its log probability is 0.
+        entropy (bool): also the entropy of every row's distribution.
+        top (int): also the ``top`` likeliest tokens of every row (at most 32
+            and ``n``) and their log probabilities, likeliest first; of equally
+            likely ones the lower token comes first.
+        out (TokenLogProb): arrays that receive the results.
+
+    Sums are held in 32 bits (64 for float64) and joined in 64.  A row whose
+    elements are all -inf has log probabilities of -inf and the entropy 0; a
+    row with a NaN or +inf has NaN everywhere and -1 for its likeliest tokens.
+
+    Returns:
+        TokenLogProb: ``log_prob``, ``lse`` (the logarithm of the sum of
+        exponentials, which the gradient takes), ``entropy``, ``top_log_prob``
+        and ``top_token``; float32 (float64 for float64) and int64.
+    """
+    entropy = bool(entropy)
+    arrays = [logits, tokens]
+    if out is not None:
+        arrays.extend([a for a in out if a is not None])
+    result, key = _oc.replay(_plans, arrays, (entropy, top, out is None))
+    if result is not _oc._NOTHING:
+        return _named(result, entropy, top)
+    given, tokens = tokens, _oc.index_array(tokens, 'tokens')
+    if given is not tokens:
+        key, arrays[1] = None, tokens
+    width = _check_logits(logits, tokens)
+    if isinstance(top, bool) or not isinstance(top, (int, numpy.integer)):
+        raise TypeError('top must be an integer')
+    top = int(top)
+    if not 0 <= top <= min(MAX_TOP, width):
+        raise ValueError('top must be between 0 and %d, got %d' % (min(MAX_TOP, width), top))
+    acc = _oc.acc_dtype(logits.dtype)
+    lead = logits._shape[:-1]
+    specs = [(lead, acc, 'log_prob'), (lead, acc, 'lse')]
+    if entropy:
+        specs.append((lead, acc, 'entropy'))
+    if top:
+        specs.append((lead + (top,), acc, 'top_log_prob'))
+        specs.append((lead + (top,), numpy.dtype(numpy.int64), 'top_token'))
+    if out is not None:
+        if not isinstance(out, TokenLogProb):
+            raise TypeError('out must be a TokenLogProb')
+        asked = {name for _, _, name in specs}
+        for name, a in zip(out._fields, out):
+            if (a is None) == (name in asked):
+                raise ValueError('out.%s is %s' % (
+                    name, 'missing' if a is None else 'given, but was not asked for'))
+        for shape, dt, name in specs:
+            _oc.check_out(getattr(out, name), shape, dt, 'out.' + name)
+    call = _oc.Call(_plans, key, arrays, 2)
+    if out is None:
+        at = [call.allocate(shape, dt) for shape, dt, _ in specs]
+    else:
+        at = list(range(2, 2 + len(specs)))
+    ret = tuple(at)
+    rows = tokens.size
+    if rows == 0:
+        call.key = None
+        call.begin()
+        return _named(call.finish(ret), entropy, top)
+    call.convert(1, _oc.as_index(call.refs[1]))
+    pitch = call.rows(0)
+    for i in at:
+        call.dense(i)
+    call.begin()
+    vec = 16 // logits.dtype.itemsize
+    vecs = -(-width // vec) + 1
+    units = _oc.compute_units()
+    # A workgroup per row, its size by the row's length; rows too few to fill
+    # the device are cut into parts, of at least a vector per thread.
+    block = 256 if vecs <= 4096 else 1024
+    parts = 1
+    if rows < 2 * units and vecs > 512:
+        block = 256
+        parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
+    unroll = 4
+    nt_in = _oc.stream_hints(logits.nbytes, 0)[0] and not top
+    defines = dict(X_T=logits.dtype, I_T=call.refs[1].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
+                   TOP=top, NT_IN=nt_in, NT_OUT=False)
+    if entropy:
+        defines['ENTROPY'] = 1
+    slots = [Ref(i) for i in at[:2]]
+    slots.append(Ref(at[2]) if entropy else 0)
+    slots += [Ref(at[-2]), Ref(at[-1])] if top else [0, 0]
+    at_keys = rows * parts * 3
+    if parts > 1:
+        i_t = call.temp((at_keys + rows * parts * top * 2) * acc.itemsize)
+        slots.append(Ref(i_t))
+    else:
+        slots.append(0)
+    fn = _SOURCE.function('cupy_token_log_prob', **defines)
+    grid = min(rows * parts, 0xffffffff // block)
+    values = slots + [rows, width, pitch, parts, at_keys]
+    call.launch(fn, (grid, 1, 1), block, 'PPPPPPPPqiqiq', Ref(0), Ref(1), *values)
+    if parts > 1:
+        fn = _SOURCE.function('cupy_token_log_prob_join', **defines)
+        call.launch(fn, (rows, 1, 1), 256, 'PPPPPPPPqiqiq', Ref(0), Ref(1), *values)
+    return _named(call.finish(ret), entropy, top)
+
+
+def _named(results, entropy, top):
+    results = iter(results)
+    return TokenLogProb(next(results), next(results), next(results) if entropy else None,
+                        *((next(results), next(results)) if top else (None, None)))
+
+
+def token_log_prob_grad(grad, logits, tokens, lse, *, entropy=None, entropy_grad=None, out=None):
+    """Gradient of :func:`token_log_prob` with respect to the logits.
+
+    ``out[j] = grad * ((j == token) - p[j])``, and with ``entropy_grad`` also
+    ``- entropy_grad * p[j] * (log(p[j]) + entropy)``, ``p = exp(logits - lse)``.
+    A row whose token is out of range has no part in the first term; a row
+    whose elements are all -inf has the gradient 0.
+
+    Args:
+        grad (cupy.ndarray): gradient of ``log_prob``, one per row.
+        logits, tokens: as in the forward call.
+        lse (cupy.ndarray): ``lse`` of the forward call.
+        entropy, entropy_grad (cupy.ndarray): ``entropy`` of the forward call
+            and its gradient (both or neither).
+        out (cupy.ndarray): receives the gradient, of the shape and type of
+            ``logits``; may be ``logits`` itself.
+    """
+    arrays = [grad, logits, tokens, lse]
+    if entropy is not None:
+        arrays.append(entropy)
+    if entropy_grad is not None:
+        arrays.append(entropy_grad)
+    if out is not None:
+        arrays.append(out)
+    with_entropy = entropy_grad is not None
+    result, key = _oc.replay(
+        _plans_grad, arrays, (entropy is None, entropy_grad is None, out is None))
+    if result is not _oc._NOTHING:
+        return result
+    if (entropy is None) != (entropy_grad is None):
+        raise ValueError('entropy and entropy_grad are given together or not at all')
+    given, tokens = tokens, _oc.index_array(tokens, 'tokens')
+    if given is not tokens:
+        key, arrays[2] = None, tokens
+    width = _check_logits(logits, tokens)
+    acc = _oc.acc_dtype(logits.dtype)
+    per_row = [(0, 'grad'), (3, 'lse')]
+    if with_entropy:
+        per_row += [(4, 'entropy'), (5, 'entropy_grad')]
+    for i, name in per_row:
+        _oc.check_float(arrays[i], name)
+        if arrays[i]._shape != tokens._shape:
+            raise ValueError('%s has the wrong shape: %r, expected %r'
+                             % (name, arrays[i]._shape, tokens._shape))
+    if out is not None:
+        _oc.check_out(out, logits._shape, logits.dtype)
+    n_in = 6 if with_entropy else 4
+    call = _oc.Call(_plans_grad, key, arrays, n_in, [(1, n_in)])
+    i_out = n_in if out is not None else call.allocate(logits._shape, logits.dtype)
+    if logits.size == 0:
+        call.key = None
+        call.begin()
+        return call.finish(i_out)
+    for i, _ in per_row:
+        call.convert(i, call.refs[i].astype(acc, copy=False))
+        call.dense(i)
+    call.convert(2, _oc.as_index(call.refs[2]))
+    pitch, po = call.rows(1), call.rows(i_out)
+    call.begin()
+    rows = tokens.size
+    vec = 16 // logits.dtype.itemsize
+    vecs = -(-width // vec) + 1
+    block = 256
+    unroll = 4 if vecs > 1024 else 2 if vecs > 256 else 1
+    blocks = -(-vecs // (block * unroll))
+    nt_in, nt_out = _oc.stream_hints(logits.nbytes, logits.nbytes)
+    defines = dict(X_T=logits.dtype, I_T=call.refs[2].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
+                   TOP=0, NT_IN=nt_in, NT_OUT=nt_out)
+    if with_entropy:
+        defines['ENTROPY'] = 1
+    fn = _GRAD.function('cupy_token_log_prob_grad', **defines)
+    call.launch(fn, (min(rows * blocks, 0xffffffff // block), 1, 1), block, 'PPPPPPPqiqqi',
+                Ref(0), Ref(1), Ref(2), Ref(3), Ref(4) if with_entropy else 0,
+                Ref(5) if with_entropy else 0, Ref(i_out), rows, width, pitch, po, blocks)
+    return call.finish(i_out)

@@ -101,6 +101,7 @@ from cupy_amd._core._routines_statistics import (  # noqa
 from cupy_amd._core._routines_logic import all, any  # noqa
 from cupy_amd._core._scan import cumsum, cumprod, nancumsum, nancumprod  # noqa
 from cupy_amd._core._embedding import embedding, embedding_grad  # noqa
+from cupy_amd._core._global_norm import global_norm, clip_by_global_norm  # noqa
 from cupy_amd._core._rms_norm import rms_norm, rms_norm_int8, rms_norm_grad  # noqa
 from cupy_amd._core._token_log_prob import (  # noqa
     token_log_prob, token_log_prob_grad, TokenLogProb)

@@ -1,0 +1,363 @@
+"""Norm of many arrays taken together, and scaling them down to a bound on it.
+
+``global_norm`` is the square root of the sum of the squares of all elements of
+all arrays; ``clip_by_global_norm`` multiplies every array by
+``min(1, max_norm / (norm + eps))``.  The arrays are described by tables in the
+argument block (up to 100 to a launch), so that a model's hundreds of gradients
+take a few launches: the squares are summed per piece of 32 KiB, a single
+workgroup joins the pieces' sums in order and derives the factor, and the
+scaling reads it from device memory: nothing waits for the host.
+"""
+import functools
+import struct
+
+import numpy
+
+from cupy_amd import _rt
+from cupy_amd._core import _op_calls as _oc
+from cupy_amd._core._kernel import _check_peer_access
+from cupy_amd._core._ufuncs import elementwise_copy
+from cupy_amd._core.core import ndarray, _byte_extent
+from cupy_amd.cuda import device as _device
+from cupy_amd.cuda import memory as _memory
+
+_MAX = 100                  # arrays to a launch: 3200 bytes of its 4 KiB of arguments
+_BLOCK = 256
+_UNROLL = 8                 # vectors of 16 bytes per thread
+_ENTRY = numpy.dtype([('src', 'u8'), ('dst', 'u8'), ('n', 'u8'), ('first', 'u4'), ('pad', 'u4')])
+_TYPES = [numpy.dtype(c) for c in _oc.FLOATS]
+_SIZES = numpy.array([t.itemsize for t in _TYPES])
+# what the extension module says of an array: address, elements, position of its
+# type in _TYPES, 1 if stored in C order plus 2 if in Fortran order, device
+_DESCRIPTION = numpy.dtype([('ptr', 'u8'), ('n', 'u8'), ('type', 'u4'), ('dense', 'u4'),
+                            ('device', 'i8')])
+
+_SOURCE = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<X_T>::type A;
+
+struct Entry {
+  const X_T* src;
+  X_T* dst;
+  unsigned long long n;
+  unsigned int first;       // the array's first workgroup
+  unsigned int pad;
+};
+struct Table { Entry e[MAX_ENTRIES]; };
+
+// The array a workgroup works on: the last one that begins at or before it.
+_CUPY_DEV int entry_of(const Table& t, int n, unsigned int block) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.e[mid].first <= block) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Vectors on 16-byte borders of the source, whatever the array starts on.
+struct Piece {
+  long long c[UNROLL];
+  cupy::Vec<X_T, VEC> v[UNROLL];
+  long long n;
+  _CUPY_DEV void load(const Entry& e, unsigned int block) {
+    const int phase = (int)((reinterpret_cast<unsigned long long>(e.src) & 15) / sizeof(X_T));
+    n = (long long)e.n;
+    const long long base = ((long long)block * UNROLL * BLOCK + threadIdx.x) * VEC - phase;
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      c[k] = base + (long long)k * BLOCK * VEC;
+      if (c[k] >= 0 && c[k] + VEC <= n) {
+        v[k] = cupy::load_vec<X_T, VEC, NT_IN>(e.src + c[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          v[k].v[i] = c[k] + i >= 0 && c[k] + i < n ? e.src[c[k] + i] : static_cast<X_T>(0.0f);
+      }
+    }
+  }
+};
+
+struct Add {
+  template <typename T> _CUPY_DEV T operator()(T a, T b) const { return a + b; }
+};
+
+// float16: 64 squares, at most 2^32 each, are added in 32 bits, the rest in 64.
+// float32: the squares are taken in 64 bits, where none over- or underflows.
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_square_sums(const Table t, const int entries, double* sums) {
+  __shared__ double lds[BLOCK / 64];
+  const int k = entry_of(t, entries, blockIdx.x);
+  const Entry e = t.e[k];
+  Piece p;
+  p.load(e, blockIdx.x - e.first);
+  double total;
+  if (sizeof(X_T) == 2) {
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float x = static_cast<float>(p.v[u].v[i]);
+        s = __builtin_fmaf(x, x, s);
+      }
+    total = s;
+  } else {
+    total = 0.0;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const double x = static_cast<double>(static_cast<A>(p.v[u].v[i]));
+        total = __builtin_fma(x, x, total);
+      }
+  }
+  total = cupy::row_allreduce<BLOCK, BLOCK>(total, Add(), lds);
+  if (threadIdx.x == 0) sums[blockIdx.x] = total;
+}
+
+extern "C" __global__ void __launch_bounds__(BLOCK)
+cupy_scale_arrays(const Table t, const int entries, const int blocks, const double* factor_) {
+  // last pieces first: they are what the sums have left in the cache
+  const unsigned int block = blocks - 1 - blockIdx.x;
+  const Entry e = t.e[entry_of(t, entries, block)];
+  const A factor = static_cast<A>(*factor_);
+  if (factor == A(1) && e.src == e.dst) return;       // what is there is the result
+  Piece p;
+  p.load(e, block - e.first);
+#pragma unroll
+  for (int k = 0; k < UNROLL; ++k) {
+    cupy::Vec<X_T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = static_cast<X_T>(static_cast<A>(p.v[k].v[i]) * factor);
+    if (p.c[k] >= 0 && p.c[k] + VEC <= p.n) {
+      cupy::store_vec<X_T, VEC, NT_OUT>(e.dst + p.c[k], r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (p.c[k] + i >= 0 && p.c[k] + i < p.n) e.dst[p.c[k] + i] = r.v[i];
+    }
+  }
+}
+''')
+
+_FINISH = _oc.Source(r'''
+#include <cupy/rows.cuh>
+struct Add {
+  template <typename T> _CUPY_DEV T operator()(T a, T b) const { return a + b; }
+};
+// One workgroup: every thread a run of the sums, the threads by a tree.
+extern "C" __global__ void __launch_bounds__(1024)
+cupy_norm_of_sums(const double* sums, const long long n, N_T* norm, double* factor,
+                  const double max_norm, const double eps) {
+  __shared__ double lds[16];
+  double t = 0.0;
+  for (long long i = threadIdx.x; i < n; i += 1024) t += sums[i];
+  t = cupy::row_allreduce<1024, 1024>(t, Add(), lds);
+  if (threadIdx.x == 0) {
+    const double r = __builtin_sqrt(t);
+    *norm = static_cast<N_T>(r);
+    const double q = max_norm / (r + eps);
+    *factor = q >= 1.0 ? 1.0 : q;       // (a NaN stays one)
+  }
+}
+''')
+
+_TYPES = [numpy.dtype(c) for c in _oc.FLOATS]
+
+
+def _describe(arrays, name):
+    """Addresses, sizes, types and layouts of a list of arrays, checked."""
+    for a in arrays:
+        if not isinstance(a, ndarray):
+            raise TypeError('%s must hold cupy.ndarrays, got %s' % (name, type(a).__name__))
+    d = numpy.frombuffer(_rt.hot.describe(arrays, _TYPES), _DESCRIPTION)
+    if len(d):
+        if d['type'].max() >= len(_TYPES):
+            for a in arrays:
+                _oc.check_float(a, name)
+        dev = _device.get_device_id()
+        if (d['device'] != dev).any():
+            for a in arrays:
+                _check_peer_access(a, dev)
+    return d
+
+
+def _ranges(arrays, d):
+    """First and one-past-last address that each array touches (0 and 0 where it
+    has no elements: such arrays overlap nothing)."""
+    start = d['ptr'].astype(numpy.int64)
+    end = start + d['n'].astype(numpy.int64) * _SIZES[d['type']]
+    for i in numpy.flatnonzero(d['dense'] == 0):
+        lo, hi = _byte_extent(arrays[i]._shape, arrays[i]._strides, arrays[i].dtype.itemsize)
+        start[i], end[i] = start[i] + lo, start[i] + hi
+    start[d['n'] == 0] = end[d['n'] == 0] = 0
+    return start, end
+
+
+def _check_apart(start, end):
+    """The arrays to write may not share memory with each other."""
+    order = numpy.argsort(start, kind='stable')
+    if (start[order][1:] < numpy.maximum.accumulate(end[order])[:-1]).any():
+        raise ValueError('two of the arrays to write overlap in memory')
+
+
+def _hit_by(src, dst):
+    """Positions of the inputs that share memory with an output other than
+    their own (which may be the very same memory)."""
+    order = numpy.argsort(dst[0], kind='stable')
+    first = numpy.searchsorted(dst[1][order], src[0], 'right')
+    last = numpy.searchsorted(dst[0][order], src[1], 'left')
+    own = (src[0] == dst[0]) & (src[1] == dst[1])
+    return numpy.flatnonzero(last - first > own)
+
+
+def _tables(src, dst):
+    """[(dtype, [(table, arrays in it, workgroups)], bytes)] per type."""
+    found = []
+    for code, dtype in enumerate(_TYPES):
+        at = numpy.flatnonzero((src['type'] == code) & (src['n'] > 0))
+        if not len(at):
+            continue
+        item = dtype.itemsize
+        ptr, n = src['ptr'][at], src['n'][at]
+        phase = (ptr.astype(numpy.int64) & 15) // item
+        per = 16 // item * _BLOCK * _UNROLL
+        blocks = (phase + n.astype(numpy.int64) + (per - 1)) // per
+        table = numpy.zeros(-(-len(at) // _MAX) * _MAX, _ENTRY)
+        table['src'][:len(at)] = ptr
+        table['dst'][:len(at)] = dst['ptr'][at]
+        table['n'][:len(at)] = n
+        launches = []
+        for lo in range(0, len(at), _MAX):
+            these = blocks[lo:lo + _MAX]
+            ends = numpy.cumsum(these)
+            if int(ends[-1]) > 0xffffffff // _BLOCK:
+                raise ValueError('more than 2**39 bytes of arrays in one launch')
+            table['first'][lo:lo + len(these)] = ends - these
+            launches.append((table[lo:lo + _MAX].tobytes(), len(these), int(ends[-1])))
+        found.append((dtype, launches, int(n.sum()) * item))
+    return found
+
+
+def _launch(fn, blocks, block, *parts):
+    fn.launch_packed((blocks, 1, 1), (block, 1, 1), b''.join(parts), 0)
+
+
+def _defines(dtype, nbytes):
+    return dict(X_T=dtype, MAX_ENTRIES=_MAX, BLOCK=_BLOCK, UNROLL=_UNROLL,
+                VEC=16 // dtype.itemsize, NT_IN=False,
+                NT_OUT=_oc.stream_hints(nbytes, nbytes)[1])
+
+
+def _run(arrays, targets, norm_out, max_norm, eps):
+    src = _describe(arrays, 'arrays')
+    dst = src if targets is None else _describe(targets, 'out')
+    dtype = _TYPES[2] if (src['type'] == 2).any() else _TYPES[1]
+    if norm_out is None:
+        norm_out = ndarray((), dtype)
+    else:
+        _oc.check_out(norm_out, (), dtype, 'norm_out')
+    reads, writes, aside = arrays, arrays, ()
+    if max_norm is None:
+        if (src['dense'] == 0).any():
+            reads = writes = [a if d else a.copy('C') for a, d in zip(arrays, src['dense'])]
+            src = dst = _describe(reads, 'arrays')
+    else:
+        finals = arrays if targets is None else targets
+        ranges = _ranges(finals, dst)
+        _check_apart(*ranges)
+        at = norm_out.data.ptr
+        if ((ranges[0] < at + dtype.itemsize) & (at < ranges[1])).any():
+            raise ValueError('norm_out overlaps an array to write')
+        hit = ()
+        if targets is not None:
+            hit = _hit_by(_ranges(arrays, src), ranges)
+        # an array and its result are walked in the order they are stored in:
+        # where these differ, or are no order at all, the result is made aside
+        aside = numpy.flatnonzero((src['dense'] & dst['dense']) == 0)
+        if len(hit) or len(aside):
+            reads, writes = list(arrays), list(finals)
+            for i in hit:
+                reads[i] = arrays[i].copy('K')
+            for i in aside:
+                reads[i] = arrays[i].copy('C')
+                writes[i] = ndarray(arrays[i]._shape, arrays[i].dtype)
+            src, dst = _describe(reads, 'arrays'), _describe(writes, 'out')
+    tables = _tables(src, dst)
+    total = sum(blocks for _, launches, _ in tables for _, _, blocks in launches)
+    temp = _memory.alloc((total + 1) * 8)     # the factor, then the sums
+    word = functools.partial(struct.pack, '<Q')
+    at = temp.ptr + 8
+    for t, launches, nbytes in tables:
+        fn = _SOURCE.function('cupy_square_sums', **_defines(t, nbytes))
+        for table, n, blocks in launches:
+            _launch(fn, blocks, _BLOCK, table, word(n), word(at))
+            at += blocks * 8
+    fn = _FINISH.function('cupy_norm_of_sums', N_T=dtype)
+    _launch(fn, 1, 1024, struct.pack('<QqQQdd', temp.ptr + 8, total, norm_out.data.ptr, temp.ptr,
+                                     0.0 if max_norm is None else max_norm, eps))
+    if max_norm is not None:
+        for t, launches, nbytes in reversed(tables):
+            fn = _SOURCE.function('cupy_scale_arrays', **_defines(t, nbytes))
+            for table, n, blocks in reversed(launches):
+                _launch(fn, blocks, _BLOCK, table, struct.pack('<iiQ', n, blocks, temp.ptr))
+        for i in aside:
+            elementwise_copy(writes[i], finals[i])
+    return norm_out
+
+
+def global_norm(arrays, *, norm_out=None):
+    """Square root of the sum of the squares of all elements of ``arrays``.
+
+    Args:
+        arrays: sequence of float16, float32 and float64 arrays of any shapes;
+            of no arrays the norm is 0.
+        norm_out (cupy.ndarray): receives the result, of shape ``()``.
+
+    Returns:
+        cupy.ndarray: of shape ``()``; float32, or float64 if any array is.
+        Nothing waits for it: it is on the device.
+    """
+    return _run(_as_list(arrays, 'arrays'), None, norm_out, None, 0.0)
+
+
+def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
+    """Scales arrays down so that their :func:`global_norm` is ``max_norm`` at most.
+
+    Every array is multiplied by ``min(1, max_norm / (norm + eps))`` and rounded
+    once.  Where the norm is infinite the factor is 0, where it is NaN the
+    factor is NaN.
+
+    Args:
+        arrays: sequence of float16, float32 and float64 arrays; scaled in
+            place without ``out``.
+        max_norm (float): bound on the norm.
+        eps (float): added to the norm in the quotient.
+        out: sequence of arrays that receive the results, of the same shapes
+            and types; each may be the array it belongs to.
+        norm_out (cupy.ndarray): receives the norm, of shape ``()``.
+
+    Returns:
+        cupy.ndarray: the norm before scaling, as :func:`global_norm` returns it.
+    """
+    max_norm, eps = float(max_norm), float(eps)
+    if not (max_norm >= 0 and eps >= 0):
+        raise ValueError('max_norm and eps must not be negative, got %r and %r' % (max_norm, eps))
+    arrays = _as_list(arrays, 'arrays')
+    if out is not None:
+        out = _as_list(out, 'out')
+        if len(out) != len(arrays):
+            raise ValueError('out holds %d arrays, expected %d' % (len(out), len(arrays)))
+        for i, (a, b) in enumerate(zip(arrays, out)):
+            if isinstance(a, ndarray) and isinstance(b, ndarray) and (
+                    a._shape != b._shape or a.dtype != b.dtype):
+                raise ValueError('out[%d] has the shape %r and type %s, expected %r %s'
+                                 % (i, b._shape, b.dtype, a._shape, a.dtype))
+    return _run(arrays, out, norm_out, max_norm, eps)
+
+
+def _as_list(arrays, name):
+    if isinstance(arrays, ndarray):
+        raise TypeError('%s is a sequence of arrays, not one array' % name)
+    return list(arrays)

@@ -1,0 +1,162 @@
+"""global_norm and clip_by_global_norm against NumPy in float64.
+
+float16: 64 squares are added in 32 bits (64 * 2^-24, half of it in the root),
+the rest in 64; the result is rounded to its type, the scaled elements once."""
+import numpy as np
+import pytest
+
+import cupy_amd as cp
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ['float16', 'float32', 'float64']
+
+
+def half_step(dtype):
+    return np.finfo(dtype).eps / 2
+
+
+def off(dtypes):
+    return 34 * 2.0 ** -24 if 'float16' in dtypes else 2.0 ** -40 if 'float64' not in dtypes else 2.0 ** -48
+
+
+def make(shapes, dtype, seed=0, spread=1.0):
+    rng = np.random.default_rng(seed)
+    types = dtype if isinstance(dtype, list) else [dtype] * len(shapes)
+    return [(rng.standard_normal(s) * spread).astype(t) for s, t in zip(shapes, types)]
+
+
+def norm64(arrays):
+    return float(np.sqrt(sum((a.astype(np.float64) ** 2).sum() for a in arrays)))
+
+
+SHAPES = [(), (1,), (7, 3), (0,), (4096, 9), (16384,), (16385,), (3, 5, 7), (100, 1001), (2, 0, 3)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('copies', [1, 15, 31])
+def test_norm_and_clipping(dtype, copies):
+    arrays = make(SHAPES * copies, dtype, copies)
+    dev = [cp.asarray(a) for a in arrays]
+    want = norm64(arrays)
+    got = cp.global_norm(dev)
+    kind = 'float64' if dtype == 'float64' else 'float32'
+    assert got.dtype == kind and got.shape == ()
+    assert abs(float(got.get()) - want) <= (half_step(kind) + off([dtype])) * want
+    for share in (0.25, 0.999, 1.5):
+        outs = [cp.empty_like(a) for a in dev]
+        norm = cp.clip_by_global_norm(dev, want * share, out=outs)
+        assert np.array_equal(norm.get(), got.get())
+        factor = min(1.0, want * share / (want + 1e-6))
+        for a, o, d in zip(arrays, outs, dev):
+            exact = a.astype(np.float64) * factor
+            bound = (half_step(dtype) + off([dtype]) + 2 * half_step(kind)) * np.abs(exact)
+            assert np.all(np.abs(o.get() - exact) <= bound + float(np.finfo(dtype).smallest_subnormal) / 2)
+            assert np.array_equal(d.get(), a)
+    inside = [a.copy() for a in dev]
+    cp.clip_by_global_norm(inside, want * 0.25)
+    again = [cp.empty_like(a) for a in dev]
+    cp.clip_by_global_norm(dev, want * 0.25, out=again)
+    for a, b in zip(inside, again):
+        assert np.array_equal(a.get(), b.get())
+    cp.clip_by_global_norm(inside, want * 2)          # nothing to do
+    for a, b in zip(inside, again):
+        assert np.array_equal(a.get(), b.get())
+
+
+def test_mixed_types_and_layouts():
+    shapes = [(50, 60), (33,), (20, 30), (7, 8, 9), (64, 64)]
+    arrays = make(shapes, ['float16', 'float32', 'float32', 'float64', 'float16'], 3)
+    base = [cp.asarray(a) for a in arrays]
+    dev = [base[0].T, base[1][::2], base[2][:, 1::3], base[3].transpose(2, 0, 1), base[4][5:40]]
+    host = [arrays[0].T, arrays[1][::2], arrays[2][:, 1::3], arrays[3].transpose(2, 0, 1), arrays[4][5:40]]
+    want = norm64(host)
+    got = cp.global_norm(dev)
+    assert got.dtype == 'float64'
+    assert abs(float(got.get()) - want) <= off(['float16']) * want
+    factor = 3.0 / (want + 1e-6)
+    outs = [cp.empty(a.shape, a.dtype) for a in dev]
+    cp.clip_by_global_norm(dev, 3.0, out=outs)
+    cp.clip_by_global_norm(dev, 3.0)
+    for a, o, d in zip(host, outs, dev):
+        exact = a.astype(np.float64) * factor
+        bound = (half_step(a.dtype) + off(['float16']) + 2 * half_step('float32')) * np.abs(exact) + 2.0 ** -25
+        assert np.all(np.abs(o.get() - exact) <= bound)
+        # (in place: the arrays are walked in another order where they are copied
+        # first, which regroups the 64 squares added in 32 bits: the same bound,
+        # not the same bits)
+        assert np.all(np.abs(d.get() - exact) <= bound)
+    # what lies between the elements of the views is left as it was
+    assert np.array_equal(base[1].get()[1::2], arrays[1][1::2])
+    assert np.array_equal(base[2].get()[:, ::3], arrays[2][:, ::3])
+
+
+def test_large_small_and_missing_values():
+    big = [cp.full(1000, 3e30, 'float32'), cp.full(10, -3e30, 'float32')]
+    assert abs(float(cp.global_norm(big).get()) / (3e30 * np.sqrt(1010.0)) - 1) < 1e-6
+    small = [cp.full(1000, 3e-30, 'float32')]
+    assert abs(float(cp.global_norm(small).get()) / (3e-30 * np.sqrt(1000.0)) - 1) < 1e-6
+    top = [cp.full(100000, 65504, 'float16')]
+    assert abs(float(cp.global_norm(top).get()) / (65504 * np.sqrt(1e5)) - 1) < 1e-5
+    x = [cp.ones(5, 'float32'), cp.asarray(np.array([1, np.inf, 2], 'float32'))]
+    n = cp.clip_by_global_norm(x, 1.0)
+    assert np.isinf(n.get()) and not x[0].get().any() and np.isnan(x[1].get()[1])
+    x = [cp.ones(5, 'float32'), cp.asarray(np.array([1, np.nan, 2], 'float32'))]
+    n = cp.clip_by_global_norm(x, 1.0)
+    assert np.isnan(n.get()) and np.all(np.isnan(x[0].get()))
+    zero = [cp.zeros(5, 'float32')]
+    assert cp.clip_by_global_norm(zero, 1.0).get() == 0 and not zero[0].get().any()
+    assert cp.global_norm([]).get() == 0 and cp.global_norm([cp.zeros((0, 3))]).get() == 0
+    x = [cp.full(4, 2.0, 'float32')]
+    cp.clip_by_global_norm(x, 0.0)
+    assert not x[0].get().any()
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_arrays_that_start_anywhere(dtype):
+    flat = np.random.default_rng(1).standard_normal(200000).astype(dtype)
+    src, dst = cp.asarray(flat), cp.zeros(200000, dtype)
+    cuts = [(0, 1), (1, 3), (5, 40), (40, 16451), (16461, 60000), (60001, 60001), (60003, 199999)]
+    xs, ys = [src[a:b] for a, b in cuts], [dst[a:b] for a, b in cuts]
+    want = norm64([flat[a:b] for a, b in cuts])
+    n = cp.empty((), 'float32')
+    assert cp.clip_by_global_norm(xs, 1.0, out=ys, norm_out=n) is n
+    assert abs(float(n.get()) - want) <= (2 ** -24 + off([dtype])) * want
+    got = dst.get().astype(np.float64)
+    held = np.zeros(200000, bool)
+    for a, b in cuts:
+        held[a:b] = True
+    assert not got[~held].any()
+    exact = flat[held].astype(np.float64) / (want + 1e-6)
+    bound = (half_step(dtype) + off([dtype]) + 2.0 ** -23) * np.abs(exact) + 2.0 ** -25
+    assert np.all(np.abs(got[held] - exact) <= bound)
+
+
+def test_results_that_overlap_inputs():
+    flat = np.random.default_rng(1).standard_normal(40000).astype('float32')
+    want = [flat[:30000] / (norm64([flat[:30000], flat[30000:]]) + 1e-6),
+            flat[30000:] / (norm64([flat[:30000], flat[30000:]]) + 1e-6)]
+    d = cp.asarray(flat)
+    # each result where the other array is
+    cp.clip_by_global_norm([d[:30000], d[30000:]], 1.0, out=[d[10000:], d[:10000]])
+    assert np.allclose(d.get()[10000:], want[0], rtol=1e-6) and np.allclose(d.get()[:10000], want[1], rtol=1e-6)
+    d = cp.asarray(flat)
+    cp.clip_by_global_norm([d[:30000], d[30000:]], 1.0, out=[d[:30000], cp.empty(10000, 'float32')])
+    assert np.allclose(d.get()[:30000], want[0], rtol=1e-6)
+
+
+def test_streams():
+    arrays = [cp.asarray(a) for a in make([(1000, 300), (17,)] * 5, 'float32', 1)]
+    want = cp.global_norm(arrays).get()
+    streams = [cp.cuda.Stream(non_blocking=True) for _ in range(2)]
+    results = []
+    for k in range(6):
+        with streams[k % 2]:
+            outs = [cp.empty_like(a) for a in arrays]
+            results.append((cp.clip_by_global_norm(arrays, 1.0, out=outs), outs))
+    for s in streams:
+        s.synchronize()
+    first = [o.get() for o in results[0][1]]
+    for n, outs in results:
+        assert np.array_equal(n.get(), want)
+        assert all(np.array_equal(o.get(), f) for o, f in zip(outs, first))

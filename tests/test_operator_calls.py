@@ -1,0 +1,326 @@
+"""Host side of the hand-written operators, without a GPU: what they refuse, how
+arrays are seen as rows, overlap checks, records of calls."""
+import struct
+
+import numpy as np
+import pytest
+
+import cupy_amd as cp
+from cupy_amd import _dryrun, _rt
+from cupy_amd._core import _global_norm, _op_calls
+
+dry = pytest.mark.skipif(not _dryrun.enabled(), reason='looks at launches that are only recorded')
+
+
+def arr(shape, dtype='float32'):
+    return cp.empty(shape, dtype)
+
+
+# -- refusals -------------------------------------------------------------------------
+
+def test_rms_norm_refuses():
+    x, w = arr((4, 8)), arr((8,))
+    for bad in (np.zeros((4, 8), 'f'), [1.0], 3.0, None):
+        with pytest.raises(TypeError):
+            cp.rms_norm(bad, w)
+    for kind in ('int32', 'complex64', 'bool'):
+        with pytest.raises(TypeError):
+            cp.rms_norm(arr((4, 8), kind))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, np.zeros(8, 'f'))
+    with pytest.raises(ValueError):
+        cp.rms_norm(arr(()))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, arr((7,)))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, arr((4, 8)))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, arr((8,), 'float64'))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, arr((8,), 'float16'))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, w, arr((8,)))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, w, arr((4, 8), 'float16'))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, w, out=arr((8, 4)))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, w, out=arr((4, 8), 'float16'))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, w, residual_out=arr((4, 8)))
+    with pytest.raises(TypeError):
+        cp.rms_norm_int8(x, w, out=arr((4, 8)))
+    with pytest.raises(ValueError):
+        cp.rms_norm_int8(x, w, scale_out=arr((4, 1)))
+    with pytest.raises(TypeError):
+        cp.rms_norm(x, w, eps=None)
+    both = arr((4, 8))
+    with pytest.raises(ValueError):
+        cp.rms_norm(x, w, arr((4, 8)), out=both, residual_out=both)
+
+
+def test_rms_norm_grad_refuses():
+    x, w = arr((4, 8)), arr((8,))
+    with pytest.raises(ValueError):
+        cp.rms_norm_grad(arr((8, 4)), x, w)
+    with pytest.raises(ValueError):
+        cp.rms_norm_grad(arr((4, 8), 'float16'), x, w)
+    with pytest.raises(ValueError):
+        cp.rms_norm_grad(x, x, weight_out=w)
+    with pytest.raises(TypeError):
+        cp.rms_norm_grad(x, x, w, weight_out=arr((8,), 'float16'))
+    with pytest.raises(ValueError):
+        cp.rms_norm_grad(x, x, w, residual_grad=arr((4, 7)))
+    with pytest.raises(TypeError):
+        cp.rms_norm_grad(np.zeros((4, 8), 'f'), x)
+
+
+def test_embedding_refuses():
+    table, ids = arr((10, 4)), arr((3,), 'int64')
+    with pytest.raises(TypeError):
+        cp.embedding(np.zeros((10, 4), 'f'), ids)
+    with pytest.raises(TypeError):
+        cp.embedding(arr((10, 4), 'int32'), ids)
+    with pytest.raises(ValueError):
+        cp.embedding(arr((10,)), ids)
+    for bad in (arr((3,), 'float32'), arr((3,), 'bool'), [0.5], np.array([True])):
+        with pytest.raises(IndexError):
+            cp.embedding(table, bad)
+    with pytest.raises(ValueError):
+        cp.embedding(table, ids, out=arr((3, 5)))
+    with pytest.raises(TypeError):
+        cp.embedding(table, ids, out=arr((3, 4), 'float16'))
+    with pytest.raises((TypeError, ValueError)):
+        cp.embedding(table, ids, 'x')
+    grad = arr((3, 4))
+    with pytest.raises(ValueError):
+        cp.embedding_grad(arr((4, 4)), ids, 10)
+    with pytest.raises(ValueError):
+        cp.embedding_grad(arr((3,)), ids, 10)
+    with pytest.raises(ValueError):
+        cp.embedding_grad(grad, ids, -1)
+    with pytest.raises(ValueError):
+        cp.embedding_grad(grad, ids, 1 << 31)
+    with pytest.raises(TypeError):
+        cp.embedding_grad(grad, ids, 10.0)
+    with pytest.raises(TypeError):
+        cp.embedding_grad(grad, ids, 10, dtype='float16')
+    with pytest.raises(TypeError):
+        cp.embedding_grad(grad, ids, 10, dtype='float32', out=arr((10, 4)))
+    with pytest.raises(ValueError):
+        cp.embedding_grad(grad, ids, 10, out=arr((11, 4)))
+
+
+def test_token_log_prob_refuses():
+    x, t = arr((4, 50)), arr((4,), 'int64')
+    with pytest.raises(TypeError):
+        cp.token_log_prob(np.zeros((4, 50), 'f'), t)
+    with pytest.raises(TypeError):
+        cp.token_log_prob(arr((4, 50), 'int32'), t)
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, arr((5,), 'int64'))
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, arr((4, 1), 'int64'))
+    with pytest.raises(IndexError):
+        cp.token_log_prob(x, arr((4,)))
+    with pytest.raises(ValueError):
+        cp.token_log_prob(arr((4, 0)), t)
+    for top in (-1, 33, 51):
+        with pytest.raises(ValueError):
+            cp.token_log_prob(x, t, top=top)
+    with pytest.raises(ValueError):
+        cp.token_log_prob(arr((4, 5)), t, top=6)
+    for top in (1.0, '1', None):
+        with pytest.raises(TypeError):
+            cp.token_log_prob(x, t, top=top)
+    out = cp.TokenLogProb(arr(4), arr(4), None, None, None)
+    with pytest.raises(TypeError):
+        cp.token_log_prob(x, t, out=arr((4,)))
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, t, entropy=True, out=out)
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, t, out=out._replace(entropy=arr(4)))
+    with pytest.raises(TypeError):
+        cp.token_log_prob(x, t, out=out._replace(lse=arr(4, 'float64')))
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, t, out=out._replace(lse=out.log_prob))
+    with pytest.raises(ValueError):
+        cp.token_log_prob_grad(arr(4), x, t, arr(4), entropy=arr(4))
+    with pytest.raises(ValueError):
+        cp.token_log_prob_grad(arr(4), x, t, arr(4), entropy_grad=arr(4))
+    with pytest.raises(ValueError):
+        cp.token_log_prob_grad(arr(5), x, t, arr(4))
+    with pytest.raises(TypeError):
+        cp.token_log_prob_grad(1.0, x, t, arr(4))
+    with pytest.raises(TypeError):
+        cp.token_log_prob_grad(arr(4), x, t, arr(4), out=arr((4, 50), 'float16'))
+
+
+def test_global_norm_refuses():
+    x = arr((4, 50))
+    with pytest.raises(TypeError):
+        cp.global_norm(x)
+    with pytest.raises(TypeError):
+        cp.global_norm([x, np.zeros(3, 'f')])
+    with pytest.raises(TypeError):
+        cp.global_norm([x, arr(3, 'int32')])
+    with pytest.raises(TypeError):
+        cp.global_norm([x], norm_out=arr((), 'float64'))
+    with pytest.raises(ValueError):
+        cp.global_norm([x], norm_out=arr((1,)))
+    for bad in (-1.0, float('nan')):
+        with pytest.raises(ValueError):
+            cp.clip_by_global_norm([x], bad)
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x], 1.0, out=[])
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x], 1.0, out=[arr((50, 4))])
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x], 1.0, out=[arr((4, 50), 'float16')])
+    # written twice: by name, and by views that share elements
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x, x], 1.0)
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x[:3], x[2:]], 1.0)
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([x, arr((4, 50))], 1.0, out=[x, x])
+    flat = arr(10)
+    with pytest.raises(ValueError):
+        cp.clip_by_global_norm([flat], 1.0, norm_out=flat[3:4].reshape(()))
+    cp.global_norm([x, x])       # read twice is no harm
+
+
+# -- rows, overlap, descriptions ----------------------------------------------------------
+
+def test_row_form():
+    a = arr((6, 10, 40))
+    assert _op_calls.row_form(a) == (60, 40)
+    assert _op_calls.row_form(a[:, :, 3:20]) == (60, 40)
+    assert _op_calls.row_form(a[::2]) is None
+    assert _op_calls.row_form(a[:, ::2]) == (30, 80)
+    assert _op_calls.row_form(a[:, 3]) == (6, 400)
+    assert _op_calls.row_form(a[2, 3]) == (1, 40)
+    assert _op_calls.row_form(a[..., ::2]) is None
+    assert _op_calls.row_form(a[..., :1]) == (60, 40)
+    assert _op_calls.row_form(a[::-1]) is None
+    assert _op_calls.row_form(a[0, ::-1]) == (10, -40)
+    assert _op_calls.row_form(a.transpose(1, 0, 2)) is None
+    assert _op_calls.row_form(cp.broadcast_to(a[0, 0], (5, 40))) == (5, 0)
+    assert not _op_calls.writable_rows(cp.broadcast_to(a[0, 0], (5, 40)))
+    assert _op_calls.writable_rows(a[0, ::-1])
+
+
+def test_overlap_of_listed_pairs():
+    a = arr((10, 8))
+    views = [a, a[:5], a[5:], arr((3,)), a[::2], a[0:0]]
+
+    def hit(i, j, same=False):
+        return _rt.hot.overlap(views, _op_calls._pack_spans(views, [(i, j, same)]))
+    assert hit(0, 1) and hit(1, 0) and hit(0, 0) and hit(1, 4)
+    assert not hit(1, 2) and not hit(0, 3) and not hit(0, 5) and not hit(5, 5)
+    assert not hit(0, 0, True) and not hit(0, 1, True) and hit(2, 4, True)
+    rev = a[::-1]
+    views.append(rev)
+    assert hit(6, 1) and hit(6, 2) and not hit(6, 3)
+    with pytest.raises(ValueError):
+        _rt.hot.overlap(views, b'1234')
+    with pytest.raises(ValueError):
+        _rt.hot.overlap([], _op_calls._pack_spans(views, [(0, 1, False)]))
+    bad = bytearray(_op_calls._pack_spans(views, [(0, 1, False)]))
+    bad[-8:] = struct.pack('<II', 99, 1)
+    with pytest.raises(ValueError):
+        _rt.hot.overlap(views, bytes(bad))
+    with pytest.raises(AttributeError):
+        _rt.hot.overlap([1], _op_calls._pack_spans([a], []))
+
+
+def test_descriptions():
+    a = arr((6, 4), 'float16')
+    arrays = [a, a.T, a[:, ::2], arr((), 'float64'), arr((0, 3)), arr(3, 'int32')]
+    d = np.frombuffer(_rt.hot.describe(arrays, _global_norm._TYPES), _global_norm._DESCRIPTION)
+    assert list(d['type']) == [0, 0, 0, 2, 1, 3]
+    assert list(d['n']) == [24, 24, 12, 1, 0, 3]
+    assert list(d['dense']) == [1, 2, 0, 3, 3, 3]
+    assert [int(p) for p in d['ptr']] == [x.data.ptr for x in arrays]
+    with pytest.raises(AttributeError):
+        _rt.hot.describe([None], _global_norm._TYPES)
+    with pytest.raises(TypeError):
+        _rt.hot.describe(arrays, 3)
+
+
+@pytest.mark.parametrize('item,dtype', [(2, 'float16'), (4, 'float32'), (8, 'float64')])
+def test_tables_cover_every_array(item, dtype):
+    """Replays the kernels' search: every element of every array is met once, by
+    a workgroup of the array it belongs to."""
+    rng = np.random.default_rng(1)
+    flat = arr(1 << 20, dtype)
+    cuts = np.sort(rng.integers(0, 1 << 20, 500))
+    arrays = [flat[a:b] for a, b in zip(cuts[:-1], cuts[1:])]
+    d = _global_norm._describe(arrays, 'arrays')
+    (found, launches, nbytes), = _global_norm._tables(d, d)
+    assert found == np.dtype(dtype) and nbytes == (cuts[-1] - cuts[0]) * item
+    per = 16 // item * 256 * 8
+    seen = 0
+    for table, n, blocks in launches:
+        entries = np.frombuffer(table, _global_norm._ENTRY)
+        assert len(entries) == 100 and n <= 100 and len(table) == 3200
+        firsts = entries['first'][:n].astype(int)
+        for k in range(n):
+            e = entries[k]
+            phase = (int(e['src']) & 15) // item
+            count = (firsts[k + 1] if k + 1 < n else blocks) - firsts[k]
+            assert (count - 1) * per < phase + int(e['n']) <= count * per
+            seen += int(e['n'])
+    assert seen == cuts[-1] - cuts[0]
+
+
+# -- records --------------------------------------------------------------------------
+
+def calls():
+    x, w, r = arr((40, 96), 'float16'), arr((96,), 'float16'), arr((40, 96), 'float16')
+    y, h, q, s = arr((40, 96), 'float16'), arr((40, 96), 'float16'), arr((40, 96), 'int8'), arr(40)
+    dw = arr(96, 'float16')
+    ids = arr((40,), 'int32')
+    table = arr((300, 96), 'float16')
+    stats = [arr(40) for _ in range(5)]
+    result = cp.TokenLogProb(arr(40), arr(40), arr(40), arr((40, 3)), arr((40, 3), 'int64'))
+    return [
+        lambda: cp.rms_norm(x, w, r, out=y, residual_out=h),
+        lambda: cp.rms_norm_int8(x, w, r, out=q, scale_out=s, residual_out=h),
+        lambda: cp.rms_norm_grad(y, x, w, residual_grad=r, out=h, weight_out=dw),
+        lambda: cp.embedding(table, ids, 2.0, out=y),
+        lambda: cp.embedding_grad(y, ids, 300, 2.0, out=table),
+        lambda: cp.token_log_prob(table[:40], ids, entropy=True, top=3, out=result),
+        lambda: cp.token_log_prob_grad(stats[0], x, ids, stats[1], entropy=stats[2],
+                                       entropy_grad=stats[3], out=y),
+        lambda: cp.rms_norm(x, w, r, out=x, residual_out=r),
+        lambda: cp.clip_by_global_norm([x, w], 1.0, out=[y, dw]),
+    ]
+
+
+@dry
+@pytest.mark.parametrize('which', range(9))
+def test_a_replayed_call_launches_the_same(which):
+    call = calls()[which]
+    seen = []
+    for _ in range(3):
+        _dryrun.launches.clear()
+        call()
+        seen.append([(l[0], l[1], l[2], l[3], len(l[4])) for l in _dryrun.launches])
+    assert seen[0] and seen[0] == seen[1] == seen[2]
+
+
+@dry
+def test_records_are_found_by_layout_not_by_address():
+    a, b = arr((4, 8)), arr((4, 8))
+    keys = set()
+    for x in (a, b):
+        result, key = _op_calls.replay({}, [x], (1,))
+        assert result is _op_calls._NOTHING and key is not None
+        keys.add(key)
+    assert len(keys) == 1
+    assert _op_calls.replay({}, [np.zeros(3)], ())[1] is None
+    # another layout, type or option: another key
+    keys = {_op_calls.replay({}, [x], e)[1] for x, e in
+            ((a, (1,)), (a, (2,)), (a[:, ::2], (1,)), (arr((4, 8), 'float16'), (1,)))}
+    assert len(keys) == 4

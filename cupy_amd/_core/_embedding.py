@@ -63,15 +63,15 @@ cupy_embedding(const X_T* table, const I_T* ids, X_T* out, const long long n, co
 ''')
 
 # -- the sort ---------------------------------------------------------------------------
-# A tile of ROUNDS * 1024 pairs belongs to a workgroup of 16 waves, a wave to
-# ROUNDS * 64 consecutive ones.  One pass of the sort by a digit: a wave finds
-# for each of its keys how many equal digits come before it in the wave (the
-# lanes of a round that share a digit are found with one ballot per bit of it),
-# the counts per wave and digit are turned into first places, and every pair
-# moves to its place.  Equal digits keep their order, so the sort is stable and
-# its result does not depend on the order in which anything runs.
-# One tile: all passes in one launch, the pairs stay in the LDS between them.
-# More tiles: a launch that counts and one that moves per pass.
+# Up to _RANKED pairs whose token and position fit one word are put in order by
+# counting, for each, the pairs before it.  More of them are sorted digit by
+# digit, in two launches per digit: workgroups of 1024 threads count the digits
+# of their tiles, then every pair moves to its place: behind the smaller digits
+# of all tiles, the equal ones of earlier tiles, and the equal ones before it in
+# its own.  Equal digits keep their order, so the sort is stable and its result
+# does not depend on the order in which anything runs.
+# The result is cleared by further workgroups of the same launches, an equal
+# share of its rows in each: the sort keeps few units busy and hides behind them.
 
 _GRAD = _oc.Source(r'''
 #include <cupy/rows.cuh>
@@ -90,6 +90,8 @@ struct Digits {
   u32 wave_total[kWaves];
 };
 
+_CUPY_DEV u32 digit_of(u32 key, int shift, int bits) { return (key >> shift) & ((1u << bits) - 1); }
+
 // The place of every key among the tile's keys of the same digit within the
 // wave, and count[][] filled in.
 _CUPY_DEV void count_digits(Digits& s, const u32 (&key)[ROUNDS], u32 (&place)[ROUNDS],
@@ -100,7 +102,7 @@ _CUPY_DEV void count_digits(Digits& s, const u32 (&key)[ROUNDS], u32 (&place)[RO
   volatile unsigned short* mine = s.count[wave];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const u32 d = (key[r] >> shift) & ((1u << bits) - 1);
+    const u32 d = digit_of(key[r], shift, bits);
     unsigned long long same = ~0ull;
     for (int b = 0; b < bits; ++b) {
       const unsigned long long set = __ballot((d >> b) & 1);
@@ -118,19 +120,18 @@ _CUPY_DEV void count_digits(Digits& s, const u32 (&key)[ROUNDS], u32 (&place)[RO
   __syncthreads();
 }
 
-// count[w][d] becomes the number of d's in the waves before w; returns (to the
-// thread that has the number of the digit) how many there are in the tile.
-_CUPY_DEV u32 sum_waves(Digits& s) {
-  u32 total = 0;
+// count[w][d] becomes the number of d's in the waves before w.
+_CUPY_DEV void sum_waves(Digits& s) {
   if (threadIdx.x < kBins) {
+    u32 c[kWaves], total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) c[w] = s.count[w][threadIdx.x];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const u32 c = s.count[w][threadIdx.x];
       s.count[w][threadIdx.x] = static_cast<unsigned short>(total);
-      total += c;
+      total += c[w];
     }
   }
-  return total;
 }
 
 // Exclusive sums over the first kBins threads' values, plus `offset`, to first[].
@@ -150,79 +151,93 @@ _CUPY_DEV void first_places(Digits& s, u32 value, u32 offset) {
   __syncthreads();
 }
 
-_CUPY_DEV u32 key_of(const I_T* ids, long long i, u32 rows) {
-  const long long id = ids[i];
+_CUPY_DEV u32 key_of(long long id, u32 rows) {
   return id >= 0 && id < (long long)rows ? (u32)id : rows;    // no row: behind all rows
 }
 
-// Zeros to every row of the result, by the workgroups from `first_block` on.
-_CUPY_DEV void clear_rows(O_T* out, u32 rows, int width, long long po, int first_block) {
-  const long long blocks = gridDim.x - first_block;
-  if (blocks <= 0) return;
+// Zeros to the rows [r0, r1) of the result, by the workgroups from `first_block`
+// on, of which one to a unit, and four of its waves, store fastest (537 MB: 84 us;
+// all sixteen waves 94, of two workgroups 111, of four 126).
+_CUPY_DEV void clear_rows(O_T* out, u32 r0, u32 r1, int width, long long po, int first_block) {
+  constexpr int kStoring = 256;
+  if (threadIdx.x >= kStoring) return;
+  const long long blocks = gridDim.x - first_block, block = blockIdx.x - first_block;
   cupy::Vec<O_T, FILL_VEC> zero;
 #pragma unroll
   for (int e = 0; e < FILL_VEC; ++e) zero.v[e] = static_cast<O_T>(0.0f);
-  const bool dense = po == width;
-  const long long length = dense ? (long long)rows * width : width;
-  const long long lines = dense ? 1 : rows;
-  const long long me = (long long)(blockIdx.x - first_block) * kThreads + threadIdx.x;
-  const long long all = blocks * kThreads;
-  if (dense) {
-    const long long vecs = length / FILL_VEC;
-    for (long long i = me; i < vecs; i += all)
+  if (po == width) {
+    // stored one after the other: one piece
+    out += (long long)r0 * width;
+    const long long length = (long long)(r1 - r0) * width, vecs = length / FILL_VEC;
+    const long long me = block * kStoring + threadIdx.x;
+    for (long long i = me; i < vecs; i += blocks * kStoring)
       cupy::store_vec<O_T, FILL_VEC, NT_OUT>(out + i * FILL_VEC, zero);
     if (me < length - vecs * FILL_VEC) out[vecs * FILL_VEC + me] = zero.v[0];
   } else {
-    for (long long r = blockIdx.x - first_block; r < lines; r += blocks)
-      for (int c = threadIdx.x; c < width; c += kThreads) out[r * po + c] = zero.v[0];
+    for (long long r = r0 + block; r < r1; r += blocks)
+      for (int c = threadIdx.x; c < width; c += kStoring) out[r * po + c] = zero.v[0];
   }
 }
 
-// All tokens in one tile: sorted by workgroup 0 while the others clear the result.
+// Few tokens: the place of a pair is the number of pairs before it, counted by
+// comparing it with all of them: the work grows with the square, but is spread
+// over the whole device and takes one short step instead of a chain of them.
+// A pair is one word, its token above its position.  16 * EACH pairs by 64
+// slices of all pairs to a workgroup.
 extern "C" __global__ void __launch_bounds__(kThreads)
-cupy_embedding_sort(const I_T* ids, u32* pairs, O_T* out, const int n, const u32 rows,
-                    const int width, const long long po, const int bits, const int passes) {
-  __shared__ Digits s;
-  __shared__ u32 keys[kTile], places[kTile];
-  if (blockIdx.x > 0) {
-    clear_rows(out, rows, width, po, 1);
+cupy_embedding_rank(const I_T* ids, u32* pairs, O_T* out, const int n, const u32 rows,
+                    const int width, const long long po, const int position_bits,
+                    const int blocks) {
+  constexpr int kLoads = EACH * 4;                   // 4096 * EACH pairs at most
+  __shared__ u32 all[kLoads * kThreads];
+  __shared__ u32 count[kWaves][16 * EACH];
+  if ((int)blockIdx.x >= blocks) {
+    clear_rows(out, 0, rows, width, po, blocks);
     return;
   }
+  long long id[kLoads];
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) {
+    const int i = k * kThreads + (int)threadIdx.x;
+    id[k] = ids[i < n ? i : n - 1];
+  }
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) {
+    const int i = k * kThreads + (int)threadIdx.x;
+    all[i] = i < n ? key_of(id[k], rows) << position_bits | i : 0xffffffffu;
+  }
+  __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
+  const int slice = (n + 255) / 256;                 // in 16-byte words
+  const uint4* from = reinterpret_cast<const uint4*>(all) + (wave * 4 + (lane >> 4)) * slice;
+  u32 me[EACH], before[EACH];
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int i = (wave * ROUNDS + r) * 64 + lane;
-    key[r] = i < n ? key_of(ids, i, rows) : 0xffffffffu;
-    pos[r] = i;
+  for (int e = 0; e < EACH; ++e) {
+    const int mine = (blockIdx.x * EACH + e) * 16 + (lane & 15);
+    me[e] = mine < n ? all[mine] : 0u;
+    before[e] = 0;
   }
-  for (int p = 0; p < passes; ++p) {
-    count_digits(s, key, place, p * bits, bits);
-    const u32 total = sum_waves(s);
-    first_places(s, total, 0);
+#pragma unroll 2
+  for (int i = 0; i < slice; ++i) {
+    const uint4 k = from[i];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const u32 d = (key[r] >> (p * bits)) & ((1u << bits) - 1);
-      const u32 to = s.first[d] + s.count[wave][d] + place[r];
-      keys[to] = key[r];
-      places[to] = pos[r];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const int i = (wave * ROUNDS + r) * 64 + lane;
-      key[r] = keys[i];
-      pos[r] = places[i];
-    }
-    __syncthreads();
+    for (int e = 0; e < EACH; ++e)
+      before[e] += (k.x < me[e]) + (k.y < me[e]) + (k.z < me[e]) + (k.w < me[e]);
   }
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int i = (wave * ROUNDS + r) * 64 + lane;
-    if (i < n) {
-      pairs[i] = key[r];
-      pairs[n + i] = pos[r];
-    }
+  for (int e = 0; e < EACH; ++e) {
+    before[e] += __shfl_xor(before[e], 16, 64);
+    before[e] += __shfl_xor(before[e], 32, 64);
+    if (lane < 16) count[wave][e * 16 + lane] = before[e];
+  }
+  __syncthreads();
+  const int mine = blockIdx.x * EACH * 16 + (int)threadIdx.x;
+  if (threadIdx.x < 16 * EACH && mine < n) {
+    u32 at = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) at += count[w][threadIdx.x];
+    pairs[at] = all[mine] >> position_bits;
+    pairs[n + at] = mine;
   }
 }
 
@@ -236,54 +251,65 @@ _CUPY_DEV void load_tile(const I_T* ids, const u32* from, u32 (&key)[ROUNDS], u3
     key[r] = 0xffffffffu;
     pos[r] = (u32)i;
     if (i < n) {
-      key[r] = first ? key_of(ids, i, rows) : from[i];
+      key[r] = first ? key_of(ids[i], rows) : from[i];
       if (!first) pos[r] = from[n + i];
     }
   }
 }
 
-// counts[tile][digit]; workgroups behind the tiles clear the result (first pass).
+// counts[tile][digit]; the workgroups behind the tiles clear rows of the result.
 extern "C" __global__ void __launch_bounds__(kThreads)
 cupy_embedding_count(const I_T* ids, u32* temp, const long long from, const long long at_counts,
                      O_T* out, const long long n, const u32 rows, const int width,
-                     const long long po, const int shift, const int bits, const int tiles) {
-  __shared__ Digits s;
+                     const long long po, const int shift, const int bits, const int tiles,
+                     const u32 clear0, const u32 clear1) {
+  __shared__ u32 count[kBins];
   if ((int)blockIdx.x >= tiles) {
-    clear_rows(out, rows, width, po, tiles);
+    clear_rows(out, clear0, clear1, width, po, tiles);
     return;
   }
-  u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
+  if (threadIdx.x < kBins) count[threadIdx.x] = 0;
+  u32 key[ROUNDS], pos[ROUNDS];
   load_tile(ids, temp + from, key, pos, n, rows, shift == 0);
-  count_digits(s, key, place, shift, bits);
-  const u32 total = sum_waves(s);
-  if (threadIdx.x < kBins) temp[at_counts + (long long)blockIdx.x * kBins + threadIdx.x] = total;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) atomicAdd(&count[digit_of(key[r], shift, bits)], 1u);
+  __syncthreads();
+  if (threadIdx.x < kBins)
+    temp[at_counts + (long long)blockIdx.x * kBins + threadIdx.x] = count[threadIdx.x];
 }
 
 extern "C" __global__ void __launch_bounds__(kThreads)
 cupy_embedding_move(const I_T* ids, u32* temp, const long long from, const long long to_at,
-                    const long long at_counts, const long long n, const u32 rows, const int shift,
-                    const int bits, const int tiles) {
+                    const long long at_counts, O_T* out, const long long n, const u32 rows,
+                    const int width, const long long po, const int shift, const int bits,
+                    const int tiles, const u32 clear0, const u32 clear1) {
   __shared__ Digits s;
+  if ((int)blockIdx.x >= tiles) {
+    clear_rows(out, clear0, clear1, width, po, tiles);
+    return;
+  }
   u32 key[ROUNDS], pos[ROUNDS], place[ROUNDS];
   load_tile(ids, temp + from, key, pos, n, rows, shift == 0);
-  count_digits(s, key, place, shift, bits);
-  sum_waves(s);
-  // of all tiles, and of those before this one
+  // how many of a digit there are, and how many in the tiles before this one
   u32 all = 0, before = 0;
   if (threadIdx.x < kBins) {
     const u32* c = temp + at_counts + threadIdx.x;
+#pragma unroll 8
     for (int t = 0; t < tiles; ++t) {
       const u32 v = c[(long long)t * kBins];
       all += v;
       before += t < (int)blockIdx.x ? v : 0;
     }
   }
+  count_digits(s, key, place, shift, bits);
+  sum_waves(s);
   first_places(s, all, before);
   u32* to = temp + to_at;
   const int wave = threadIdx.x >> 6;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const u32 d = (key[r] >> shift) & ((1u << bits) - 1);
+    const u32 d = digit_of(key[r], shift, bits);
     const long long at = (long long)s.first[d] + s.count[wave][d] + place[r];
     // (the filling of the last tile has the largest digit and the last places)
     if (at < n) {
@@ -327,19 +353,37 @@ cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
   const long long t0 = ch * chunk;
   const long long t1 = t0 + chunk < n ? t0 + chunk : n;
   u32 cur = keys[t0];
+  const u32 before = keys[t0 > 0 ? t0 - 1 : 0], behind = keys[t1 < n ? t1 : n - 1];
+  bool head = t0 > 0 && before == cur;
+  u32 key_ahead[UNROLL], at_ahead[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    key_ahead[u] = keys[t0 + u < t1 ? t0 + u : t1 - 1];
+    at_ahead[u] = pos[t0 + u < t1 ? t0 + u : t1 - 1];
+  }
   if (cur >= rows) return;
-  bool head = t0 > 0 && keys[t0 - 1] == cur;
   A sum[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sum[e] = A(0);
   A* mine = partial + ch * 2 * width + c;
   for (long long t = t0; t < t1; t += UNROLL) {
-    u32 key[UNROLL];
+    u32 key[UNROLL], at[UNROLL];
     cupy::Vec<G_T, VEC> v[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      key[u] = t + u < t1 ? keys[t + u] : 0xffffffffu;
-      if (key[u] < rows) v[u] = cupy::load_part<G_T, VEC>(g + (long long)pos[t + u] * pg + c, have);
+      key[u] = key_ahead[u];
+      at[u] = at_ahead[u];
+    }
+    // (positions are in range whatever their token: nothing to wait for)
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      v[u] = WHOLE ? cupy::load_vec<G_T, VEC>(g + (long long)at[u] * pg + c)
+                   : cupy::load_part<G_T, VEC>(g + (long long)at[u] * pg + c, have);
+    const long long ahead = t + UNROLL < t1 ? t + UNROLL : t;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      key_ahead[u] = keys[ahead + u < t1 ? ahead + u : t1 - 1];
+      at_ahead[u] = pos[ahead + u < t1 ? ahead + u : t1 - 1];
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -365,7 +409,7 @@ cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
     }
   }
   if (cur >= rows) return;
-  const bool on = t1 < n && keys[t1] == cur;
+  const bool on = t1 < n && behind == cur;
   if (!head && !on) {
     put(out + (long long)cur * po + c, sum, have, scale);
   } else {
@@ -376,43 +420,71 @@ cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
 }
 
 // The runs that cross chunks, each by the workgroups of the chunk it begins
-// in: 64 columns by 4 slices of the chunks it goes on through.
+// in: 64 lanes of JVEC columns by 4 slices of the chunks it goes on through.
 extern "C" __global__ void __launch_bounds__(256)
 cupy_embedding_join(const u32* temp, O_T* out, const long long at_pairs,
                     const long long at_partial, const long long n, const u32 rows,
                     const int width, const long long po, const int chunk, const int chunks,
                     const double scale) {
-  __shared__ A lds[4][64];
+  constexpr int JVEC = 16 / sizeof(A);
+  __shared__ cupy::Vec<A, JVEC> lds[4][64];
   const u32* keys = temp + at_pairs;
   const A* partial = reinterpret_cast<const A*>(temp + at_partial);
   const long long ch = blockIdx.x;
   const long long t0 = ch * chunk, t1 = t0 + chunk;
   if (t1 >= n) return;
-  const u32 cur = keys[t1];
-  if (cur >= rows || keys[t1 - 1] != cur) return;
-  if (t0 > 0 && keys[t0 - 1] == cur) return;       // it began before this chunk
-  // last chunk that begins with `cur`: doubled steps, then halved ones
-  long long lo = ch + 1, step = 1;
-  while (lo + step < chunks && keys[(lo + step) * chunk] == cur) {
-    lo += step;
-    step <<= 1;
+  const u32 cur = keys[t1], last = keys[t1 - 1], before = keys[t0 > 0 ? t0 - 1 : 0];
+  const u32 next = ch + 2 < chunks ? keys[t1 + chunk] : rows;
+  if (cur >= rows || last != cur) return;
+  if (t0 > 0 && before == cur) return;             // it began before this chunk
+  // last chunk that begins with `cur`, 256 looked at together
+  long long lo = ch + 1;
+  if (next == cur) {
+    int found;
+    do {
+      const long long q = lo + 1 + threadIdx.x;
+      found = __syncthreads_count(q < chunks && keys[q * chunk] == cur);
+      lo += found;
+    } while (found == 256);
   }
-  for (; step > 0; step >>= 1)
-    if (lo + step < chunks && keys[(lo + step) * chunk] == cur) lo += step;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int c = blockIdx.y * 64 + tx;
-  A t = A(0);
-  if (c < width) {
-    if (ty == 0) t = partial[(ch * 2 + 1) * width + c];
-    for (long long j = ch + 1 + ty; j <= lo; j += 4) t += partial[j * 2 * width + c];
+  const int c = (blockIdx.y * 64 + tx) * JVEC;
+  const int have = width - c;
+  A t[JVEC];
+#pragma unroll
+  for (int e = 0; e < JVEC; ++e) t[e] = A(0);
+  if (have > 0) {
+    // (the first one is the sum of the run's beginning, at the end of its chunk)
+    for (long long j = ch + ty; j <= lo; j += 16) {
+      cupy::Vec<A, JVEC> p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long q = j + 4 * k <= lo ? j + 4 * k : lo;
+        p[k] = cupy::load_part<A, JVEC>(partial + (q * 2 + (q == ch)) * width + c, have);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j + 4 * k <= lo)
+#pragma unroll
+          for (int e = 0; e < JVEC; ++e) t[e] += p[k].v[e];
+    }
   }
-  lds[ty][tx] = t;
+#pragma unroll
+  for (int e = 0; e < JVEC; ++e) lds[ty][tx].v[e] = t[e];
   __syncthreads();
-  if (ty == 0 && c < width)
-    out[(long long)cur * po + c] = static_cast<O_T>(
-        (((lds[0][tx] + lds[1][tx]) + lds[2][tx]) + lds[3][tx]) * static_cast<A>(scale));
+  if (ty == 0 && have > 0) {
+    cupy::Vec<O_T, JVEC> r;
+#pragma unroll
+    for (int e = 0; e < JVEC; ++e)
+      r.v[e] = static_cast<O_T>((((lds[0][tx].v[e] + lds[1][tx].v[e]) + lds[2][tx].v[e]) +
+                                 lds[3][tx].v[e]) * static_cast<A>(scale));
+    cupy::store_part<O_T, JVEC>(out + (long long)cur * po + c, r, have);
+  }
 }
 ''')
+
+# most pairs that are put in order by comparing all of them
+_RANKED = 8192
 
 _plans = {}
 _plans_grad = {}
@@ -552,46 +624,52 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     # there are some per compute unit
     chunk = min(128, max(8, _oc.clp2(n // 512)))
     chunks = -(-n // chunk)
-    # the temporary: sorted pairs (twice for many tiles), counts, partial sums
-    rounds = 1
-    while rounds < 16 and rounds * 1024 < n:
+    position_bits = max(1, (n - 1).bit_length())
+    rank = n <= _RANKED and num_rows.bit_length() + position_bits <= 32
+    each = _oc.clp2(-(-n // 4096)) if rank else 1     # (it holds 4096 * each pairs)
+    # tiles of as many rounds as leave 64 of them at most, up to 16
+    rounds = 2
+    while rounds < 16 and rounds * 1024 * 64 < n:
         rounds *= 2
     tiles = -(-n // (rounds * 1024))
     key_bits = num_rows.bit_length()
     passes = -(-key_bits // 9)
     bits = -(-key_bits // passes)
-    words = 2 * n if tiles == 1 else 4 * n + tiles * 512
+    # the temporary: sorted pairs (two copies and counts if sorted by digits), partial sums
+    words = 2 * n if rank else 4 * n + tiles * 512
     words += words & 1
     i_t = call.temp(words * 4 + chunks * 2 * width * acc)
-    # workgroups that clear the result while it is sorted
-    fill = min(_oc.compute_units(), -(-num_rows * width // (out_vec * 1024)))
     defines = dict(G_T=grad.dtype, O_T=dt, I_T=call.refs[1].dtype, ROUNDS=rounds,
-                   FILL_VEC=out_vec, NT_OUT=nt_out)
+                   FILL_VEC=out_vec, EACH=each, NT_OUT=nt_out)
     at = 0
-    if tiles == 1:
-        fn = _GRAD.function('cupy_embedding_sort', **defines)
-        call.launch(fn, (1 + fill, 1, 1), 1024, 'PPPiIiqii', Ref(1), Ref(i_t), Ref(i_out), n,
-                    num_rows, width, po, bits, passes)
+    fill = min(_oc.compute_units(), -(-num_rows * width // (out_vec * 256)))
+    if rank:
+        blocks = -(-n // (16 * each))
+        fn = _GRAD.function('cupy_embedding_rank', **defines)
+        call.launch(fn, (blocks + fill, 1, 1), 1024, 'PPPiIiqii', Ref(1), Ref(i_t), Ref(i_out), n,
+                    num_rows, width, po, position_bits, blocks)
     else:
         count = _GRAD.function('cupy_embedding_count', **defines)
         move = _GRAD.function('cupy_embedding_move', **defines)
         at = 2 * n
+        cuts = [num_rows * k // (2 * passes) for k in range(2 * passes + 1)]
         for p in range(passes):
             src, at = at, 2 * n - at
-            call.launch(count, (tiles + (fill if p == 0 else 0), 1, 1), 1024, 'PPqqPqIiqiii',
-                        Ref(1), Ref(i_t), src, 4 * n, Ref(i_out), n, num_rows, width, po,
-                        p * bits, bits, tiles)
-            call.launch(move, (tiles, 1, 1), 1024, 'PPqqqqIiii', Ref(1), Ref(i_t), src, at, 4 * n,
-                        n, num_rows, p * bits, bits, tiles)
+            call.launch(count, (tiles + fill, 1, 1), 1024, 'PPqqPqIiqiiiII', Ref(1), Ref(i_t), src,
+                        4 * n, Ref(i_out), n, num_rows, width, po, p * bits, bits, tiles,
+                        cuts[2 * p], cuts[2 * p + 1])
+            call.launch(move, (tiles + fill, 1, 1), 1024, 'PPqqqPqIiqiiiII', Ref(1), Ref(i_t), src,
+                        at, 4 * n, Ref(i_out), n, num_rows, width, po, p * bits, bits, tiles,
+                        cuts[2 * p + 1], cuts[2 * p + 2])
     vec = 16 // grad.dtype.itemsize
     lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
-    defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec)
+    defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec, WHOLE=width % vec == 0)
     fn = _SUMS.function('cupy_embedding_sums', **defines)
     call.launch(fn, (-(-chunks // (256 // lanes)), -(-width // (lanes * vec)), 1), 256,
                 'PPPqqqIiqqiid', Ref(0), Ref(i_t), Ref(i_out), at, words, n, num_rows, width,
                 pg, po, chunk, chunks, scale)
     if chunks > 1:
         fn = _SUMS.function('cupy_embedding_join', **defines)
-        call.launch(fn, (chunks, -(-width // 64), 1), 256, 'PPqqqIiqiid', Ref(i_t), Ref(i_out),
+        call.launch(fn, (chunks, -(-width // (64 * (16 // acc))), 1), 256, 'PPqqqIiqiid', Ref(i_t), Ref(i_out),
                     at, words, n, num_rows, width, po, chunk, chunks, scale)
     return call.finish(i_out)

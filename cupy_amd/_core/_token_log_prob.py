@@ -39,26 +39,32 @@ template <> struct lowest<float16> { static _CUPY_DEV A value() { return A(-6550
 template <> struct lowest<float> { static _CUPY_DEV A value() { return A(-3.4028234663852886e38f); } };
 template <> struct lowest<double> { static _CUPY_DEV A value() { return A(-1.7976931348623157e308); } };
 
-// A row is seen as vectors of 16 bytes that start on 16-byte borders whatever
-// the row starts on: the first and the last may hang over its ends.
+// A row is seen as vectors of 16 bytes that start on 16-byte borders, whatever
+// the row starts on, and as the single elements before the first and behind
+// the last of them (fewer than a vector each).
 struct RowVecs {
   const X_T* x;
-  int phase;        // elements of the first vector that lie before the row
   int width;
+  int head;         // elements before the first vector
+  int n;            // vectors
+  int tail;         // elements behind the last
   _CUPY_DEV RowVecs(const X_T* row, int w) : x(row), width(w) {
-    phase = (int)((reinterpret_cast<unsigned long long>(row) & 15) / sizeof(X_T));
+    const int phase = (int)((reinterpret_cast<unsigned long long>(row) & 15) / sizeof(X_T));
+    head = phase ? VEC - phase : 0;
+    if (head > w) head = w;
+    n = (w - head) / VEC;
+    tail = w - head - n * VEC;
   }
-  _CUPY_DEV long long count() const { return ((long long)phase + width + VEC - 1) / VEC; }
-  _CUPY_DEV long long column(long long j) const { return j * VEC - phase; }
-  // elements outside the row are -inf: they add nothing and are never the best
-  _CUPY_DEV cupy::Vec<X_T, VEC> load(long long j) const {
-    const long long c = column(j);
-    if (c >= 0 && c + VEC <= width) return cupy::load_vec<X_T, VEC, NT_IN>(x + c);
-    cupy::Vec<X_T, VEC> v;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      v.v[e] = c + e >= 0 && c + e < width ? x[c + e] : static_cast<X_T>(-__builtin_inff());
-    return v;
+  _CUPY_DEV int column(int j) const { return head + j * VEC; }
+  _CUPY_DEV cupy::Vec<X_T, VEC> load(int j) const {
+    return cupy::load_vec<X_T, VEC, NT_IN>(x + head + (long long)j * VEC);
+  }
+  // Column of the single element that thread t takes, or -1: threads 0 and up
+  // the head's, threads 32 and up the tail's.
+  _CUPY_DEV int single(int t) const {
+    if (t < head) return t;
+    if (t >= 32 && t - 32 < tail) return width - tail + t - 32;
+    return -1;
   }
 };
 
@@ -85,6 +91,14 @@ struct Run {
     s *= f;
     m = to;
   }
+  // one more element (-inf: nothing; its argument is kept finite for 0 * -inf)
+  _CUPY_DEV void add(A x, A base) {
+    const A t = power(x, base), p = exp2_(t);
+    s += p;
+#ifdef ENTROPY
+    u = cupy::fma_(max_(t, A(-30000)), p, u);
+#endif
+  }
   _CUPY_DEV double log2_sum() const { return log2((double)s); }
   _CUPY_DEV double lse() const {
     if (s == A(0)) return -__builtin_inf();          // every element is -inf
@@ -106,6 +120,24 @@ struct JoinRun {
     return a;
   }
 };
+
+// The largest element of a vector, NaNs left out.
+_CUPY_DEV A largest(const cupy::Vec<X_T, VEC>& v) {
+  if (sizeof(X_T) == 2) {
+    // two halves at a time
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+    half2 p[VEC / 2];
+    __builtin_memcpy(p, &v, sizeof(p));
+    half2 m = p[0];
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) m = __builtin_elementwise_max(m, p[i]);
+    return max_(static_cast<A>(m.x), static_cast<A>(m.y));
+  }
+  A m = static_cast<A>(v.v[0]);
+#pragma unroll
+  for (int i = 1; i < VEC; ++i) m = max_(m, static_cast<A>(v.v[i]));
+  return m;
+}
 
 #if TOP > 0
 // A value and its column; of equal values the lower column comes first.
@@ -132,6 +164,13 @@ struct BestKey {
     return k;
   }
 };
+
+_CUPY_DEV Key key_at(const cupy::Vec<X_T, VEC>& v, int j, int i, const RowVecs& vecs) {
+  Key k;
+  k.v = static_cast<A>(v.v[i]);
+  k.i = (u32)(vecs.column(j) + i);
+  return k;
+}
 
 constexpr int kMost = 1024;     // keys that are ranked against each other
 
@@ -236,36 +275,36 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     const int part = parts == 1 ? 0 : (int)(w - row * parts);
     const X_T* x = logits + row * pitch;
     const RowVecs vecs(x, width);
-    const long long n = vecs.count();
-    const long long share = (n + parts - 1) / parts;
-    const long long j0 = part * share + threadIdx.x;
-    const long long j1 = (part + 1) * share < n ? (part + 1) * share : n;
+    const int share = (vecs.n + parts - 1) / parts;
+    const int j0 = part * share;
+    const int j1 = j0 + share < vecs.n ? j0 + share : vecs.n;
+    const int single = part == 0 ? vecs.single(threadIdx.x) : -1;
     Run run;
     run.m = lowest<X_T>::value();
     run.s = run.u = A(0);
-    A base = run.base();
+    const X_T alone = x[single >= 0 ? single : 0];
 #if TOP > 0
     A best = -__builtin_inff();
-    long long best_at = j0;
+    int best_at = j0 + threadIdx.x;
 #endif
-    for (long long j = j0; j < j1; j += (long long)BLOCK * UNROLL) {
+    A base = run.base();
+    // All vectors of a trip are requested before the first is used; the last
+    // trip's requests beyond the end go to the last vector and are not used.
+    for (int j = j0; j < j1; j += BLOCK * UNROLL) {
       cupy::Vec<X_T, VEC> v[UNROLL];
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k)
-        if (j + k * BLOCK < j1) v[k] = vecs.load(j + k * BLOCK);
+      for (int k = 0; k < UNROLL; ++k) {
+        const int at = j + k * BLOCK + (int)threadIdx.x;
+        v[k] = vecs.load(at < j1 ? at : j1 - 1);
+      }
 #pragma unroll
       for (int k = 0; k < UNROLL; ++k) {
-        if (j + k * BLOCK >= j1) break;
-        A e[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = static_cast<A>(v[k].v[i]);
-        A vm = e[0];
-#pragma unroll
-        for (int i = 1; i < VEC; ++i) vm = max_(vm, e[i]);
+        if (j + k * BLOCK + (int)threadIdx.x >= j1) break;
+        const A vm = largest(v[k]);
 #if TOP > 0
         if (vm > best) {
           best = vm;
-          best_at = j + k * BLOCK;
+          best_at = j + k * BLOCK + threadIdx.x;
         }
 #endif
         if (vm > run.m) {
@@ -273,14 +312,13 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
           base = run.base();
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const A t = Run::power(e[i], base), p = exp2_(t);
-          run.s += p;
-#ifdef ENTROPY
-          run.u = cupy::fma_(max_(t, A(-30000)), p, run.u);
-#endif
-        }
+        for (int i = 0; i < VEC; ++i) run.add(static_cast<A>(v[k].v[i]), base);
       }
+    }
+    if (single >= 0) {
+      const A e = static_cast<A>(alone);
+      if (e > run.m) run.lift(e);
+      run.add(e, run.base());
     }
     run = cupy::row_allreduce<BLOCK, BLOCK>(run, JoinRun(), lds);
     if (threadIdx.x == 0) {
@@ -296,15 +334,17 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
 #if TOP > 0
     // The best key of every thread, then of 64 groups of threads.
     Key mine = no_key();
-    if (j0 < j1) {
+    if (best_at < j1) {
       const cupy::Vec<X_T, VEC> v = vecs.load(best_at);
-      const long long c = vecs.column(best_at);
 #pragma unroll
       for (int i = VEC - 1; i >= 0; --i)
-        if (c + i >= 0 && c + i < width && static_cast<A>(v.v[i]) == best) {
-          mine.v = best;
-          mine.i = (u32)(c + i);
-        }
+        if (static_cast<A>(v.v[i]) == best) mine = key_at(v, best_at, i, vecs);
+    }
+    Key other = no_key();
+    if (single >= 0) {
+      other.v = static_cast<A>(alone);
+      other.i = (u32)single;
+      if (better(other, mine)) mine = other;
     }
     const Key group = cupy::group_allreduce<BLOCK / 64>(mine, BestKey());
     if (threadIdx.x % (BLOCK / 64) == 0) ts.sample[threadIdx.x / (BLOCK / 64)] = group;
@@ -313,17 +353,11 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     const Key least = bar(ts);
     // whoever may hold one of the best looks through its vectors again
     if (!better(least, mine)) {
-      for (long long j = j0; j < j1; j += BLOCK) {
+      if (single >= 0) offer(ts, other, least);
+      for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
         const cupy::Vec<X_T, VEC> v = vecs.load(j);
-        const long long c = vecs.column(j);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          if (c + i < 0 || c + i >= width) continue;
-          Key k;
-          k.v = static_cast<A>(v.v[i]);
-          k.i = (u32)(c + i);
-          offer(ts, k, least);
-        }
+        for (int i = 0; i < VEC; ++i) offer(ts, key_at(v, j, i, vecs), least);
       }
     }
     __syncthreads();
@@ -352,15 +386,12 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
         __syncthreads();
         const Key last = ts.last;
         Key b = no_key();
-        for (long long j = j0; j < j1; j += BLOCK) {
+        if (single >= 0 && (first | better(last, other))) b = BestKey()(b, other);
+        for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
           const cupy::Vec<X_T, VEC> v = vecs.load(j);
-          const long long c = vecs.column(j);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            if (c + i < 0 || c + i >= width) continue;
-            Key k;
-            k.v = static_cast<A>(v.v[i]);
-            k.i = (u32)(c + i);
+            const Key k = key_at(v, j, i, vecs);
             if ((first | better(last, k)) & better(k, b)) b = k;
           }
         }
@@ -440,9 +471,20 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
 ''')
 
 _GRAD = _oc.Source(_COMMON + r'''
-// d x_j = g (delta_jt - p_j) - gH p_j (log p_j + H).  Bound by memory: read
-// once, written once, whatever the row starts on (RowVecs); the target's column
-// is found by comparing vector numbers.
+// d x_j = g (delta_jt - p_j) - gH p_j (log p_j + H).
+_CUPY_DEV X_T gradient(X_T logit, A norm, A gain, A gh, A h, bool hit, bool empty) {
+  const A lp = static_cast<A>(logit) - norm, p = exp2_(lp * A(LOG2E));
+#ifdef ENTROPY
+  // (p = 0 where log p = -inf: kept finite, so that the product is 0)
+  A r = -p * cupy::fma_(gh, max_(lp, A(-1e30)) + h, gain);
+#else
+  A r = -p * gain;
+#endif
+  if (hit) r += gain;
+  return static_cast<X_T>(empty ? A(0) : r);
+}
+
+// Bound by memory: read once, written once.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_token_log_prob_grad(const A* g, const X_T* logits, const I_T* tokens, const A* lse,
                          const A* entropy, const A* entropy_grad, X_T* out,
@@ -451,48 +493,43 @@ cupy_token_log_prob_grad(const A* g, const X_T* logits, const I_T* tokens, const
   for (long long w = blockIdx.x; w < rows * blocks; w += gridDim.x) {
     const long long row = w / blocks;
     const int block = (int)(w - row * blocks);
-    const RowVecs vecs(logits + row * pitch, width);
-    const long long n = vecs.count();
+    const X_T* x = logits + row * pitch;
+    const RowVecs vecs(x, width);
     X_T* to = out + row * po;
     const A norm = lse[row];
     const long long token = tokens[row];
     const bool met = token >= 0 && token < width;
+    const int target = met ? (int)token : -1;
     const A gain = met ? g[row] : A(0);
+    A gh = A(0), h = A(0);
 #ifdef ENTROPY
-    const A gh = entropy_grad[row], h = entropy[row];
+    gh = entropy_grad[row];
+    h = entropy[row];
 #endif
-    const long long base = (long long)block * BLOCK * UNROLL + threadIdx.x;
+    // a row with nothing left has no distribution to change
+    const bool empty = norm == -__builtin_inff();
+    const int base = block * BLOCK * UNROLL + threadIdx.x;
     cupy::Vec<X_T, VEC> v[UNROLL];
+    if (vecs.n > 0) {
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k)
-      if (base + k * BLOCK < n) v[k] = vecs.load(base + k * BLOCK);
+      for (int k = 0; k < UNROLL; ++k) {
+        const int j = base + k * BLOCK;
+        v[k] = vecs.load(j < vecs.n ? j : vecs.n - 1);
+      }
+    }
+    const int single = block == 0 ? vecs.single(threadIdx.x) : -1;
+    if (single >= 0)
+      to[single] = gradient(x[single], norm, gain, gh, h, single == target, empty);
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const long long j = base + k * BLOCK;
-      if (j >= n) break;
-      const long long c = vecs.column(j);
-      const long long hit = met ? token - c : -1;
+      const int j = base + k * BLOCK;
+      if (j >= vecs.n) break;
+      const int hit = target - vecs.column(j);
       cupy::Vec<X_T, VEC> d;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const A x = static_cast<A>(v[k].v[e]);
-        const A lp = x - norm, p = exp2_(lp * A(LOG2E));
-#ifdef ENTROPY
-        // (p = 0 where log p = -inf: kept finite, so that the product is 0)
-        A r = -p * cupy::fma_(gh, max_(lp, A(-1e30)) + h, gain);
-#else
-        A r = -p * gain;
-#endif
-        if (hit == e) r += gain;
-        // a row with nothing left has no distribution to change
-        d.v[e] = static_cast<X_T>(norm == -__builtin_inff() ? A(0) : r);
-      }
-      if (c >= 0 && c + VEC <= width) {
-        cupy::store_vec<X_T, VEC, NT_OUT>(to + c, d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) if (c + e >= 0 && c + e < width) to[c + e] = d.v[e];
-      }
+      for (int e = 0; e < VEC; ++e)
+        d.v[e] = gradient(v[k].v[e], norm, gain, gh, h, hit == e && met, empty);
+      cupy::store_vec<X_T, VEC, NT_OUT>(to + vecs.column(j), d);
     }
   }
 }
@@ -591,16 +628,7 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         call.dense(i)
     call.begin()
     vec = 16 // logits.dtype.itemsize
-    vecs = -(-width // vec) + 1
-    units = _oc.compute_units()
-    # A workgroup per row, its size by the row's length; rows too few to fill
-    # the device are cut into parts, of at least a vector per thread.
-    block = 256 if vecs <= 4096 else 1024
-    parts = 1
-    if rows < 2 * units and vecs > 512:
-        block = 256
-        parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
-    unroll = 4
+    block, unroll, parts = _geometry(rows, max(1, width // vec), top)
     nt_in = _oc.stream_hints(logits.nbytes, 0)[0] and not top
     defines = dict(X_T=logits.dtype, I_T=call.refs[1].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
                    TOP=top, NT_IN=nt_in, NT_OUT=False)
@@ -623,6 +651,19 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         fn = _SOURCE.function('cupy_token_log_prob_join', **defines)
         call.launch(fn, (rows, 1, 1), 256, 'PPPPPPPPqiqiq', Ref(0), Ref(1), *values)
     return _named(call.finish(ret), entropy, top)
+
+
+def _geometry(rows, vecs, top):
+    """(threads of a workgroup, vectors a thread requests at a time, parts of a row)"""
+    units = _oc.compute_units()
+    # A workgroup per row: of 256 threads, so that a unit holds eight whose
+    # reductions do not wait for each other (8192 rows of 50257 float16 with
+    # entropy: 178 us with 256, 187 with 512, 225 with 1024).  Rows too few to
+    # fill the device are cut into parts, of at least two vectors per thread.
+    block, parts = 256, 1
+    if rows < 2 * units and vecs > 512:
+        parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
+    return block, 4, parts
 
 
 def _named(results, entropy, top):
@@ -692,7 +733,7 @@ def token_log_prob_grad(grad, logits, tokens, lse, *, entropy=None, entropy_grad
     call.begin()
     rows = tokens.size
     vec = 16 // logits.dtype.itemsize
-    vecs = -(-width // vec) + 1
+    vecs = max(1, width // vec)
     block = 256
     unroll = 4 if vecs > 1024 else 2 if vecs > 256 else 1
     blocks = -(-vecs // (block * unroll))

@@ -160,7 +160,7 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
         yv.v[e] = fin(h[e]);
 #endif
       }
-      cupy::store_part<Y_T, VEC, NT_OUT>(y + row * py + c, yv, width - c);
+      cupy::store_part<Y_T, VEC, NT_Y>(y + row * py + c, yv, width - c);
     }
 #ifdef INT8
     if (lane == 0) scale[row] = static_cast<float>(fin.scale);
@@ -464,28 +464,31 @@ cupy_rms_norm_columns(const X_T* g, const X_T* x, A* temp, const long long rows,
   temp[skip + (long long)blockIdx.y * width + c] = t;
 }
 
-// dw = the sum of the partial rows: 16 columns by 64 slices of the partial
-// rows to a workgroup; a slice is summed in order, the slices by a tree.
+// dw = the sum of the partial rows: 32 columns (a cache line of float32) by 32
+// slices of the partial rows to a workgroup; a slice is summed in order, the
+// slices by a tree.
 extern "C" __global__ void __launch_bounds__(1024)
 cupy_rms_norm_join(const A* temp, W_T* dw, const long long skip, const int n, const int width) {
+  constexpr int kAhead = 8;
+  __shared__ A lds[32][33];
   const A* partial = temp + skip;
-  __shared__ A lds[64][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + tx;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
   A t = A(0);
   if (c < width) {
-    int p = ty;
-    for (; p + 192 < n; p += 256) {
-      const A a = partial[(long long)p * width + c], b = partial[(long long)(p + 64) * width + c];
-      const A d = partial[(long long)(p + 128) * width + c], e = partial[(long long)(p + 192) * width + c];
-      t += a; t += b; t += d; t += e;
+    for (int p = ty; p < n; p += 32 * kAhead) {
+      A v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        v[k] = partial[(long long)(p + 32 * k < n ? p + 32 * k : p) * width + c];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) if (p + 32 * k < n) t += v[k];
     }
-    for (; p < n; p += 64) t += partial[(long long)p * width + c];
   }
   lds[ty][tx] = t;
   __syncthreads();
 #pragma unroll
-  for (int half = 32; half > 0; half >>= 1) {
+  for (int half = 16; half > 0; half >>= 1) {
     if (ty < half) lds[ty][tx] += lds[ty + half][tx];
     __syncthreads();
   }
@@ -497,35 +500,22 @@ _plans = {}
 _plans_int8 = {}
 _plans_grad = {}
 
-# threads of a workgroup a CU may hold
-_THREADS_PER_CU = 2048
-
-
-def _geometry(width, itemsize, rows, most_items):
+def _geometry(width, itemsize, most_items):
     """(lanes per row, threads of a workgroup, vectors per lane, elements per
-    vector) of rows held in registers; 0 vectors: too long for them."""
+    vector) of rows held in registers; 0 vectors: too long for them.
+
+    One vector per lane, as many lanes as that takes: all of a row is requested
+    at once and the units hold many rows (16384 x 4096 float16 with residual:
+    89 us with 512 lanes, 92 with 256 and two vectors; 9001 x 2047 float32: 50.5
+    with 512, 52.8 with 256; 4096 x 8192 to int8: 66 with 1024, 75 with 512, 84
+    with 256).  Rows of up to 64 vectors share a workgroup of 256 threads."""
     vec = 16 // itemsize
     n = (width + vec - 1) // vec
-    if n <= 64:
-        lanes = max(4, _oc.clp2(n))
-        return lanes, 256, 1, vec
-    if n <= 256:
-        lanes = 256 if rows < 1024 else 64
-        return lanes, 256, -(-n // lanes), vec
-    # few rows: the whole row at once, as many lanes as it has vectors
-    items = 1 if rows < 512 else 2
-    lanes = 256
-    while lanes < 1024 and lanes * items < n:
-        lanes *= 2
+    lanes = min(1024, max(4, _oc.clp2(n)))
     items = -(-n // lanes)
     if items > most_items:
         return 1024, 1024, 0, vec
-    return lanes, lanes, items, vec
-
-
-def _grid(rows, lanes, block):
-    per = block // lanes
-    return max(1, min(-(-rows // per), _oc.compute_units() * (_THREADS_PER_CU // block)))
+    return lanes, 256 if lanes <= 64 else lanes, items, vec
 
 
 def _check(x, weight, residual, what):
@@ -626,19 +616,25 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
     if int8:
         call.dense(i_s)
     call.begin()
-    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, rows, 4)
+    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, 4)
     nt_in, nt_out = _oc.stream_hints(
         x.nbytes + (residual.nbytes if residual is not None else 0),
         x.size * y_dtype.itemsize + (residual.nbytes if residual is not None else 0))
     defines = dict(X_T=x.dtype, R_T=x.dtype if residual is None else residual.dtype,
                    W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
-                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out)
+                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out,
+                   # (8 bits fit the cache where the rest does not)
+                   NT_Y=nt_out and not int8)
     for name, on in (('INT8', int8), ('WEIGHT', weight is not None),
                      ('RESIDUAL', residual is not None)):
         if on:
             defines[name] = 1
     fn = _SOURCE.function('cupy_rms_norm', **defines)
-    call.launch(fn, (_grid(rows, lanes, block), 1, 1), block, 'PPPPPPqiqqqqd',
+    # a workgroup per row (or 256 / lanes of them): stores run fastest without a
+    # loop around them.  Those of 1024 threads, of which a unit holds two, loop.
+    grid = -(-rows // (block // lanes))
+    grid = min(grid, 2 * _oc.compute_units() if block == 1024 else 0xffffffff // block)
+    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
                 Ref(0), Ref(i_r) if i_r is not None else 0, Ref(i_w) if i_w is not None else 0,
                 Ref(i_y), Ref(i_s) if int8 else 0, Ref(i_h) if i_h is not None else 0,
                 rows, width, px, pr, py, ps, eps)
@@ -756,8 +752,7 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
         i_dw, at = at, at + 1
     width = x._shape[-1]
     rows = x.size // width if width else 0
-    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, rows,
-                                         2 if x.dtype.char == 'd' else 4)
+    lanes, block, items, vec = _geometry(width, x.dtype.itemsize, 2 if x.dtype.char == 'd' else 4)
     # rows in registers: written by the threads that have read them.  (Rows
     # that are walked are read again for dw.)
     places = [(i, i_d) for i in (0, 1, i_r) if i is not None and i_d is not None
@@ -789,7 +784,10 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
         if on:
             defines[name] = 1
     acc = _oc.acc_dtype(x.dtype).itemsize
-    grid = _grid(rows, lanes, block)
+    # Workgroups that loop over rows, each with its sums for dw in registers: of
+    # 1536 threads to a unit (16384 x 4096 float16: 102 us; 107 with 2048, 111 to
+    # 114 with 1024), of which each adds a partial row to what is joined.
+    grid = max(1, min(-(-rows // (block // lanes)), _oc.compute_units() * max(1, 1536 // block)))
     fn = _GRAD_SOURCE.function('cupy_rms_norm_grad', **defines)
     # the temporary: the rows' r (walked rows only), then the partial sums of dw
     n_partial, skip, run = grid, 0, 0
@@ -811,6 +809,6 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
             call.launch(fn, (blocks, n_partial, 1), 256, 'PPPqiqqqq',
                         Ref(0), Ref(1), Ref(i_t), rows, width, pg, px, run, skip)
         fn = _GRAD_SOURCE.function('cupy_rms_norm_join', **defines)
-        call.launch(fn, (-(-width // 16), 1, 1), 1024, 'PPqii',
+        call.launch(fn, (-(-width // 32), 1, 1), 1024, 'PPqii',
                     Ref(i_t), Ref(i_dw), skip, n_partial, width)
     return call.finish(ret)

@@ -45,35 +45,60 @@ struct Entry {
 };
 struct Table { Entry e[MAX_ENTRIES]; };
 
-// The array a workgroup works on: the last one that begins at or before it.
+// The array a workgroup works on: the last one that begins at or before it,
+// found by every wave in one step, a lane per array (a search by halves is a
+// chain of seven loads).
 _CUPY_DEV int entry_of(const Table& t, int n, unsigned int block) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (t.e[mid].first <= block) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 63;
+  int found = 0;
+#pragma unroll
+  for (int base = 0; base < MAX_ENTRIES; base += 64) {
+    const int at = base + lane < MAX_ENTRIES ? base + lane : MAX_ENTRIES - 1;
+    found += __popcll(__ballot(base + lane < n && t.e[at].first <= block));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(found - 1);
 }
 
-// Vectors on 16-byte borders of the source, whatever the array starts on.
+// Vectors on 16-byte borders of the source, whatever the array starts on.  A
+// piece that lies inside its array is loaded without a question between the
+// requests.
 struct Piece {
-  long long c[UNROLL];
-  cupy::Vec<X_T, VEC> v[UNROLL];
+  long long c0;      // the thread's first element
   long long n;
+  bool inside;
+  cupy::Vec<X_T, VEC> v[UNROLL];
+  _CUPY_DEV long long column(int k) const { return c0 + (long long)k * BLOCK * VEC; }
   _CUPY_DEV void load(const Entry& e, unsigned int block) {
     const int phase = (int)((reinterpret_cast<unsigned long long>(e.src) & 15) / sizeof(X_T));
     n = (long long)e.n;
-    const long long base = ((long long)block * UNROLL * BLOCK + threadIdx.x) * VEC - phase;
+    const long long first = (long long)block * UNROLL * BLOCK * VEC - phase;
+    inside = first >= 0 && first + UNROLL * BLOCK * VEC <= n;
+    c0 = first + threadIdx.x * VEC;
+    if (inside) {
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-      c[k] = base + (long long)k * BLOCK * VEC;
-      if (c[k] >= 0 && c[k] + VEC <= n) {
-        v[k] = cupy::load_vec<X_T, VEC, NT_IN>(e.src + c[k]);
-      } else {
+      for (int k = 0; k < UNROLL; ++k) v[k] = cupy::load_vec<X_T, VEC, NT_IN>(e.src + column(k));
+    } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          v[k].v[i] = c[k] + i >= 0 && c[k] + i < n ? e.src[c[k] + i] : static_cast<X_T>(0.0f);
+      for (int k = 0; k < UNROLL; ++k) {
+        const long long c = column(k);
+        if (c >= 0 && c + VEC <= n) {
+          v[k] = cupy::load_vec<X_T, VEC, NT_IN>(e.src + c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            v[k].v[i] = c + i >= 0 && c + i < n ? e.src[c + i] : static_cast<X_T>(0.0f);
+        }
       }
+    }
+  }
+  _CUPY_DEV void store(X_T* to, int k, const cupy::Vec<X_T, VEC>& r) const {
+    const long long c = column(k);
+    if (inside || (c >= 0 && c + VEC <= n)) {
+      cupy::store_vec<X_T, VEC, NT_OUT>(to + c, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i >= 0 && c + i < n) to[c + i] = r.v[i];
     }
   }
 };
@@ -130,13 +155,7 @@ cupy_scale_arrays(const Table t, const int entries, const int blocks, const doub
     cupy::Vec<X_T, VEC> r;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) r.v[i] = static_cast<X_T>(static_cast<A>(p.v[k].v[i]) * factor);
-    if (p.c[k] >= 0 && p.c[k] + VEC <= p.n) {
-      cupy::store_vec<X_T, VEC, NT_OUT>(e.dst + p.c[k], r);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (p.c[k] + i >= 0 && p.c[k] + i < p.n) e.dst[p.c[k] + i] = r.v[i];
-    }
+    p.store(e.dst, k, r);
   }
 }
 ''')
@@ -152,7 +171,13 @@ cupy_norm_of_sums(const double* sums, const long long n, N_T* norm, double* fact
                   const double max_norm, const double eps) {
   __shared__ double lds[16];
   double t = 0.0;
-  for (long long i = threadIdx.x; i < n; i += 1024) t += sums[i];
+  for (long long i = threadIdx.x; i < n; i += 8 * 1024) {
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = sums[i + 1024 * k < n ? i + 1024 * k : i];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (i + 1024 * k < n) t += v[k];
+  }
   t = cupy::row_allreduce<1024, 1024>(t, Add(), lds);
   if (threadIdx.x == 0) {
     const double r = __builtin_sqrt(t);

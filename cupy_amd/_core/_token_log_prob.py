@@ -110,16 +110,17 @@ struct Run {
     return (log2_sum() - (double)u / (double)s) * LN2;
   }
 };
-struct JoinRun {
-  _CUPY_DEV Run operator()(Run a, Run b) const {
-    const A top = max_(a.m, b.m);
-    a.lift(top);
-    b.lift(top);
-    a.s += b.s;
-    a.u += b.u;
-    return a;
-  }
-};
+struct Greater { _CUPY_DEV A operator()(A a, A b) const { return max_(a, b); } };
+struct Add { _CUPY_DEV A operator()(A a, A b) const { return a + b; } };
+// Joined over groups of kGroup lanes: the maximum first, so that every lane
+// rescales its sums once.
+template <int kGroup>
+_CUPY_DEV Run join_lanes(Run r) {
+  r.lift(cupy::group_allreduce<kGroup>(r.m, Greater()));
+  r.s = cupy::group_allreduce<kGroup>(r.s, Add());
+  r.u = cupy::group_allreduce<kGroup>(r.u, Add());
+  return r;
+}
 
 // The largest element of a vector, NaNs left out.
 _CUPY_DEV A largest(const cupy::Vec<X_T, VEC>& v) {
@@ -140,42 +141,61 @@ _CUPY_DEV A largest(const cupy::Vec<X_T, VEC>& v) {
 }
 
 #if TOP > 0
-// A value and its column; of equal values the lower column comes first.
+// A value and its column in one order: larger values first, of equal values the
+// lower column.  float16 and float32: one word, the value's bits turned so that
+// they order as integers (-0 as 0) above the complement of the column.  A key
+// that stands for nothing comes behind every element, also behind -inf.
+#if SMALL_KEYS
+typedef unsigned long long Key;
+_CUPY_DEV Key key_of(A v, u32 column) {
+  const u32 b = __builtin_bit_cast(u32, v + 0.0f);
+  const u32 turned = b ^ ((u32)((int)b >> 31) | 0x80000000u);
+  return (Key)turned << 32 | (u32)~column;
+}
+_CUPY_DEV Key no_key(u32 number) { return number; }
+_CUPY_DEV bool is_none(Key k) { return (k >> 32) == 0; }
+_CUPY_DEV bool better(Key a, Key b) { return a > b; }
+_CUPY_DEV A value_of(Key k) {
+  const u32 t = (u32)(k >> 32);
+  return __builtin_bit_cast(A, t & 0x80000000u ? t ^ 0x80000000u : ~t);
+}
+_CUPY_DEV u32 column_of(Key k) { return ~(u32)k; }
+#else
 struct Key {
   A v;
   u32 i;
+  u32 pad;
 };
-constexpr u32 kNone = 0xffffffffu;
+_CUPY_DEV Key key_of(A v, u32 column) {
+  Key k;
+  k.v = v;
+  k.i = column;
+  k.pad = 0;
+  return k;
+}
+_CUPY_DEV Key no_key(u32 number) { return key_of(-__builtin_inf(), 0xffffffffu - number); }
+_CUPY_DEV bool is_none(const Key& k) { return k.i >= 0x80000000u; }
 _CUPY_DEV bool better(const Key& a, const Key& b) {
   return (a.v > b.v) | ((a.v == b.v) & (a.i < b.i));
 }
-_CUPY_DEV Key no_key() {
-  Key k;
-  k.v = -__builtin_inff();
-  k.i = kNone;
-  return k;
-}
+_CUPY_DEV A value_of(const Key& k) { return k.v; }
+_CUPY_DEV u32 column_of(const Key& k) { return k.i; }
+#endif
+
 struct BestKey {
   _CUPY_DEV Key operator()(const Key& a, const Key& b) const {
-    const bool t = better(b, a);
-    Key k;
-    k.v = t ? b.v : a.v;
-    k.i = t ? b.i : a.i;
-    return k;
+    return cupy::select_value(better(b, a), b, a);
   }
 };
 
 _CUPY_DEV Key key_at(const cupy::Vec<X_T, VEC>& v, int j, int i, const RowVecs& vecs) {
-  Key k;
-  k.v = static_cast<A>(v.v[i]);
-  k.i = (u32)(vecs.column(j) + i);
-  return k;
+  return key_of(static_cast<A>(v.v[i]), (u32)(vecs.column(j) + i));
 }
 
 constexpr int kMost = 1024;     // keys that are ranked against each other
 
 struct TopState {
-  Key sample[64];
+  Key sample[64];               // (no two alike)
   Key key[kMost];
   Key last;
   u32 n;
@@ -183,19 +203,16 @@ struct TopState {
 
 // The TOP-th best of the 64 sample keys: at least TOP keys are as good.
 _CUPY_DEV Key bar(const TopState& t) {
-  const int lane = threadIdx.x & 63;
-  const Key me = t.sample[lane];
+  const Key me = t.sample[threadIdx.x & 63];
   int rank = 0;
-  for (int o = 0; o < 64; ++o) {
-    const Key k = t.sample[o];
-    rank += better(k, me) | ((k.i == me.i) & (k.v == me.v) & (o < lane));
-  }
-  const int src = __ffsll(__ballot(rank == TOP - 1)) - 1;
-  return cupy::shfl_idx(me, src);
+#pragma unroll 8
+  for (int o = 0; o < 64; ++o) rank += better(t.sample[o], me);
+  return cupy::shfl_idx(me, __ffsll(__ballot(rank == TOP - 1)) - 1);
 }
 
-_CUPY_DEV void offer(TopState& t, const Key& k, const Key& least) {
-  if (better(least, k) | !(k.v == k.v)) return;
+// Keeps an element that is as good as `least` (a NaN is none: its row has no order).
+_CUPY_DEV void offer(TopState& t, A value, const Key& k, const Key& least) {
+  if (better(least, k) | !(value == value)) return;
   const u32 at = atomicAdd(&t.n, 1u);
   if (at < kMost) t.key[at] = k;
 }
@@ -210,11 +227,12 @@ _CUPY_DEV void put_ranked(const TopState& t, u32 n, Put put) {
   for (u32 q = threadIdx.x; q < n; q += blockDim.x) {
     const Key me = t.key[q];
     int rank = 0;
+#pragma unroll 4
     for (u32 o = 0; o < n; ++o) rank += better(t.key[o], me);
     if (rank < TOP) put(rank, me);
   }
   // (fewer elements than TOP: the rest of the places hold nothing)
-  for (u32 q = n + threadIdx.x; q < TOP; q += blockDim.x) put(q, no_key());
+  for (u32 q = n + threadIdx.x; q < TOP; q += blockDim.x) put(q, no_key(0));
 }
 #endif
 
@@ -226,29 +244,32 @@ struct Outputs {
   long long* index;
 };
 
+// The logit of the row's token, 0 if it has none.
+_CUPY_DEV A logit_of(const X_T* x, long long token, int width) {
+  return token >= 0 && token < width ? static_cast<A>(x[token]) : A(0);
+}
+
 // A row's results from its joined statistics, by one thread.
-_CUPY_DEV void put_row(const Outputs& o, const Run& run, const X_T* x, const I_T* tokens,
-                       long long row, int width) {
+_CUPY_DEV void put_row(const Outputs& o, const Run& run, A logit, long long token, long long row,
+                       int width) {
   const double lse = run.lse();
   o.lse[row] = static_cast<A>(lse);
-  const long long token = tokens[row];
   double lp = 0.0;
-  if (token >= 0 && token < width) {
-    const double at = static_cast<double>(static_cast<A>(x[token]));
-    lp = run.s == A(0) ? at : at - lse;        // (a row of -inf: -inf, not NaN)
-  }
+  if (token >= 0 && token < width)
+    lp = run.s == A(0) ? (double)logit : (double)logit - lse;   // (a row of -inf: -inf, not NaN)
   o.log_prob[row] = static_cast<A>(lp);
 #ifdef ENTROPY
   o.entropy[row] = static_cast<A>(run.entropy());
 #endif
 }
 #if TOP > 0
-_CUPY_DEV void put_top(const Outputs& o, const Run& run, long long row, int rank, const Key& k) {
-  const double lse = run.lse();
+_CUPY_DEV void put_top(const Outputs& o, const Run& run, double lse, long long row, int rank,
+                       const Key& k) {
   const bool nan = !(run.s == run.s);          // no order in a row with NaN or +inf
+  const A v = value_of(k);
   o.top[row * TOP + rank] =
-      nan ? static_cast<A>(run.s) : static_cast<A>(run.s == A(0) ? (double)k.v : (double)k.v - lse);
-  o.index[row * TOP + rank] = nan ? -1 : (long long)k.i;
+      nan ? static_cast<A>(run.s) : static_cast<A>(run.s == A(0) ? (double)v : (double)v - lse);
+  o.index[row * TOP + rank] = nan ? -1 : (long long)column_of(k);
 }
 #endif
 
@@ -260,7 +281,8 @@ extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy, A* top,
                     long long* index, A* runs, const long long rows, const int width,
                     const long long pitch, const int parts, const long long at_keys) {
-  __shared__ Run lds[BLOCK / 64];
+  constexpr int kWaves = BLOCK / 64;
+  __shared__ Run lds[kWaves];
 #if TOP > 0
   __shared__ TopState ts;
 #endif
@@ -283,15 +305,17 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     run.m = lowest<X_T>::value();
     run.s = run.u = A(0);
     const X_T alone = x[single >= 0 ? single : 0];
+    const long long token = parts == 1 ? (long long)tokens[row] : 0;
 #if TOP > 0
     A best = -__builtin_inff();
     int best_at = j0 + threadIdx.x;
+    const bool once = j1 - j0 <= BLOCK * UNROLL;   // one trip: its vectors stay in registers
 #endif
     A base = run.base();
+    cupy::Vec<X_T, VEC> v[UNROLL];
     // All vectors of a trip are requested before the first is used; the last
     // trip's requests beyond the end go to the last vector and are not used.
     for (int j = j0; j < j1; j += BLOCK * UNROLL) {
-      cupy::Vec<X_T, VEC> v[UNROLL];
 #pragma unroll
       for (int k = 0; k < UNROLL; ++k) {
         const int at = j + k * BLOCK + (int)threadIdx.x;
@@ -320,10 +344,42 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
       if (e > run.m) run.lift(e);
       run.add(e, run.base());
     }
-    run = cupy::row_allreduce<BLOCK, BLOCK>(run, JoinRun(), lds);
+    const A logit = parts == 1 && threadIdx.x == 0 ? logit_of(x, token, width) : A(0);
+    run = join_lanes<64>(run);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = run;
+#if TOP > 0
+    // The best key of every thread, then of 64 groups of threads.
+    Key mine = no_key(0);
+    if (once) {
+#pragma unroll
+      for (int k = UNROLL - 1; k >= 0; --k)
+#pragma unroll
+        for (int i = VEC - 1; i >= 0; --i) {
+          const int j = j0 + k * BLOCK + threadIdx.x;
+          if (j == best_at && j < j1 && static_cast<A>(v[k].v[i]) == best)
+            mine = key_at(v[k], j, i, vecs);
+        }
+    } else if (best_at < j1) {
+      const cupy::Vec<X_T, VEC> w = vecs.load(best_at);
+#pragma unroll
+      for (int i = VEC - 1; i >= 0; --i)
+        if (static_cast<A>(w.v[i]) == best) mine = key_at(w, best_at, i, vecs);
+    }
+    Key other = no_key(0);
+    if (single >= 0 && alone == alone) {
+      other = key_of(static_cast<A>(alone), (u32)single);
+      mine = BestKey()(mine, other);
+    }
+    const Key group = cupy::group_allreduce<kWaves>(mine, BestKey());
+    if (threadIdx.x % kWaves == 0)
+      ts.sample[threadIdx.x / kWaves] = is_none(group) ? no_key(threadIdx.x / kWaves) : group;
+    if (threadIdx.x == 0) ts.n = 0;
+#endif
+    __syncthreads();
+    run = join_lanes<kWaves>(lds[threadIdx.x & (kWaves - 1)]);
     if (threadIdx.x == 0) {
       if (parts == 1) {
-        put_row(out, run, x, tokens, row, width);
+        put_row(out, run, logit, token, row, width);
       } else {
         A* to = runs + w * 3;
         to[0] = run.m;
@@ -332,44 +388,37 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
       }
     }
 #if TOP > 0
-    // The best key of every thread, then of 64 groups of threads.
-    Key mine = no_key();
-    if (best_at < j1) {
-      const cupy::Vec<X_T, VEC> v = vecs.load(best_at);
-#pragma unroll
-      for (int i = VEC - 1; i >= 0; --i)
-        if (static_cast<A>(v.v[i]) == best) mine = key_at(v, best_at, i, vecs);
-    }
-    Key other = no_key();
-    if (single >= 0) {
-      other.v = static_cast<A>(alone);
-      other.i = (u32)single;
-      if (better(other, mine)) mine = other;
-    }
-    const Key group = cupy::group_allreduce<BLOCK / 64>(mine, BestKey());
-    if (threadIdx.x % (BLOCK / 64) == 0) ts.sample[threadIdx.x / (BLOCK / 64)] = group;
-    if (threadIdx.x == 0) ts.n = 0;
-    __syncthreads();
     const Key least = bar(ts);
     // whoever may hold one of the best looks through its vectors again
     if (!better(least, mine)) {
-      if (single >= 0) offer(ts, other, least);
-      for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
-        const cupy::Vec<X_T, VEC> v = vecs.load(j);
+      if (single >= 0) offer(ts, static_cast<A>(alone), other, least);
+      if (once) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) offer(ts, key_at(v, j, i, vecs), least);
+        for (int k = 0; k < UNROLL; ++k) {
+          const int j = j0 + k * BLOCK + threadIdx.x;
+          if (j >= j1) break;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            offer(ts, static_cast<A>(v[k].v[i]), key_at(v[k], j, i, vecs), least);
+        }
+      } else {
+        for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
+          const cupy::Vec<X_T, VEC> w = vecs.load(j);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            offer(ts, static_cast<A>(w.v[i]), key_at(w, j, i, vecs), least);
+        }
       }
     }
     __syncthreads();
     const u32 found = ts.n;
-    A* key_values = runs + at_keys + w * TOP;
-    u32* key_columns = reinterpret_cast<u32*>(runs + at_keys + rows * parts * TOP) + w * TOP;
+    Key* keys = reinterpret_cast<Key*>(runs + at_keys) + w * TOP;
+    const double lse_ = run.lse();
     auto put = [&](int rank, const Key& k) {
       if (parts == 1) {
-        put_top(out, run, row, rank, k);
+        put_top(out, run, lse_, row, rank, k);
       } else {
-        key_values[rank] = k.v;
-        key_columns[rank] = k.i;
+        keys[rank] = k;
       }
     };
     if (found <= kMost) {
@@ -377,22 +426,19 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     } else {
       // More than can be ranked (the best lie in the vectors of a few threads):
       // one pass over the row per place, each for the best behind the last.
-      if (threadIdx.x == 0) {
-        ts.last.v = __builtin_inff();
-        ts.last.i = 0;
-      }
       bool first = true;
       for (int rank = 0; rank < TOP; ++rank) {
         __syncthreads();
         const Key last = ts.last;
-        Key b = no_key();
-        if (single >= 0 && (first | better(last, other))) b = BestKey()(b, other);
+        Key b = no_key(0);
+        if (!is_none(other) && (first || better(last, other))) b = other;
         for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
-          const cupy::Vec<X_T, VEC> v = vecs.load(j);
+          const cupy::Vec<X_T, VEC> w = vecs.load(j);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            const Key k = key_at(v, j, i, vecs);
-            if ((first | better(last, k)) & better(k, b)) b = k;
+            const A value = static_cast<A>(w.v[i]);
+            const Key k = key_at(w, j, i, vecs);
+            if (value == value && (first || better(last, k)) && better(k, b)) b = k;
           }
         }
         first = false;
@@ -400,7 +446,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
         if ((threadIdx.x & 63) == 0) ts.key[threadIdx.x >> 6] = b;
         __syncthreads();
         if (threadIdx.x == 0) {
-          for (int q = 1; q < BLOCK / 64; ++q) b = BestKey()(b, ts.key[q]);
+          for (int q = 1; q < kWaves; ++q) b = BestKey()(b, ts.key[q]);
           ts.last = b;
           put(rank, b);
         }
@@ -411,16 +457,13 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
   }
 }
 
-// The parts of a row joined: a workgroup per row, at most 64 parts.
+// The parts of a row joined: a workgroup per row, at most 64 parts.  A chain of
+// waits: all that does not depend on a result is requested at the start.
 extern "C" __global__ void __launch_bounds__(256)
 cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy,
                          A* top, long long* index, const A* runs, const long long rows,
                          const int width, const long long pitch, const int parts,
                          const long long at_keys) {
-#if TOP > 0
-  __shared__ TopState ts;
-  if (threadIdx.x == 0) ts.n = 0;
-#endif
   Outputs out;
   out.log_prob = log_prob;
   out.lse = lse;
@@ -429,43 +472,51 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
   out.index = index;
   const long long row = blockIdx.x;
   const int lane = threadIdx.x & 63;
+  const long long token = tokens[row];
+  const A* from = runs + (row * parts + (lane < parts ? lane : 0)) * 3;
   Run run;
-  run.m = lowest<X_T>::value();
-  run.s = run.u = A(0);
-  if (lane < parts) {
-    const A* from = runs + (row * parts + lane) * 3;
-    run.m = from[0];
-    run.s = from[1];
-    run.u = from[2];
-  }
-  run = cupy::group_allreduce<64>(run, JoinRun());     // (by every wave for itself)
-  if (threadIdx.x == 0) put_row(out, run, logits + row * pitch, tokens, row, width);
+  run.m = from[0];
+  run.s = from[1];
+  run.u = from[2];
 #if TOP > 0
-  const A* key_values = runs + at_keys + row * parts * TOP;
-  const u32* key_columns =
-      reinterpret_cast<const u32*>(runs + at_keys + rows * parts * TOP) + row * parts * TOP;
+  __shared__ TopState ts;
+  const Key* keys = reinterpret_cast<const Key*>(runs + at_keys) + row * parts * TOP;
+  constexpr int kEach = (64 * TOP + 255) / 256;
+  Key mine[kEach];
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    const int at = q * 256 + threadIdx.x;
+    mine[q] = at < parts * TOP ? keys[at] : no_key(0);
+  }
   // Every part's keys are in order: the first few of each are the sample.
-  const int each = 64 / parts < TOP ? 64 / parts : TOP;
   if (threadIdx.x < 64) {
-    Key k = no_key();
+    const int each = 64 / parts < TOP ? 64 / parts : TOP;
+    Key k = no_key(lane);
     if (lane < parts * each) {
-      const int at = (lane / each) * TOP + lane % each;
-      k.v = key_values[at];
-      k.i = key_columns[at];
+      k = keys[(lane / each) * TOP + lane % each];
+      if (is_none(k)) k = no_key(lane);
     }
     ts.sample[lane] = k;
   }
+  if (threadIdx.x == 0) ts.n = 0;
+#endif
+  const A logit = threadIdx.x == 0 ? logit_of(logits + row * pitch, token, width) : A(0);
+  if (lane >= parts) {
+    run.m = lowest<X_T>::value();
+    run.s = run.u = A(0);
+  }
+  run = join_lanes<64>(run);     // (by every wave for itself)
+  if (threadIdx.x == 0) put_row(out, run, logit, token, row, width);
+#if TOP > 0
   __syncthreads();
   const Key least = bar(ts);
-  for (int q = threadIdx.x; q < parts * TOP; q += 256) {
-    Key k;
-    k.v = key_values[q];
-    k.i = key_columns[q];
-    if (k.i != kNone) offer(ts, k, least);
-  }
+#pragma unroll
+  for (int q = 0; q < kEach; ++q)
+    if (!is_none(mine[q])) offer(ts, value_of(mine[q]), mine[q], least);
   __syncthreads();
+  const double lse_ = run.lse();
   put_ranked(ts, ts.n < kMost ? ts.n : kMost,
-             [&](int rank, const Key& k) { put_top(out, run, row, rank, k); });
+             [&](int rank, const Key& k) { put_top(out, run, lse_, row, rank, k); });
 #endif
 }
 ''')
@@ -631,13 +682,13 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
     block, unroll, parts = _geometry(rows, max(1, width // vec), top)
     nt_in = _oc.stream_hints(logits.nbytes, 0)[0] and not top
     defines = dict(X_T=logits.dtype, I_T=call.refs[1].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
-                   TOP=top, NT_IN=nt_in, NT_OUT=False)
+                   TOP=top, SMALL_KEYS=int(acc == numpy.float32), NT_IN=nt_in, NT_OUT=False)
     if entropy:
         defines['ENTROPY'] = 1
     slots = [Ref(i) for i in at[:2]]
     slots.append(Ref(at[2]) if entropy else 0)
     slots += [Ref(at[-2]), Ref(at[-1])] if top else [0, 0]
-    at_keys = rows * parts * 3
+    at_keys = -(-rows * parts * 3 // 4) * 4          # (keys of 8 or 16 bytes)
     if parts > 1:
         i_t = call.temp((at_keys + rows * parts * top * 2) * acc.itemsize)
         slots.append(Ref(i_t))

@@ -83,73 +83,58 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
               const long long py, const long long ps, const double eps) {
   constexpr int kRows = BLOCK / LANES;
   __shared__ Stat lds[2][BLOCK / 64];
-  const int lane = threadIdx.x % LANES;
+  const cupy::RowShare<ITEMS, LANES, VEC, TINY> mine(threadIdx.x % LANES, width);
   cupy::Vec<W_T, VEC> wv[ITEMS];
 #ifdef WEIGHT
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const int c = (lane + k * LANES) * VEC;
-    if (c < width) wv[k] = cupy::load_part<W_T, VEC>(w + c, width - c);
-  }
+  mine.load(wv, w);
 #endif
   int flip = 0;
   for (long long base = (long long)blockIdx.x * kRows; base < rows;
        base += (long long)gridDim.x * kRows) {
-    const long long row = base + threadIdx.x / LANES;
-    const bool valid = kRows == 1 || row < rows;
+    const long long at = base + threadIdx.x / LANES;
+    const bool valid = kRows == 1 || at < rows;
+    const long long row = valid ? at : rows - 1;
     cupy::Vec<X_T, VEC> xv[ITEMS];
     cupy::Vec<R_T, VEC> rv[ITEMS];
-    if (valid) {
-#pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        const int c = (lane + k * LANES) * VEC;
-        if (c < width) {
-          xv[k] = cupy::load_part<X_T, VEC, NT_IN>(x + row * px + c, width - c);
+    mine.template load<NT_IN>(xv, x + row * px);
 #ifdef RESIDUAL
-          rv[k] = cupy::load_part<R_T, VEC, NT_IN>(res + row * pr + c, width - c);
+    mine.template load<NT_IN>(rv, res + row * pr);
 #endif
-        }
-      }
-    }
     Stat s;
     s.square = A(0);
     s.top = 0;
-    if (valid) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        if ((lane + k * LANES) * VEC >= width) continue;
-        A h[VEC];
-        sums_of<VEC>(xv[k], rv[k], h);
+    for (int k = 0; k < ITEMS; ++k) {
+      A h[VEC];
+      sums_of<VEC>(xv[k], rv[k], h);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          s.square = cupy::fma_(h[e], h[e], s.square);
+      for (int e = 0; e < VEC; ++e) {
+        if (!mine.owns(k, e)) h[e] = A(0);
+        s.square = cupy::fma_(h[e], h[e], s.square);
 #ifdef INT8
 #ifdef WEIGHT
-          // (a partial vector's tail is zeros)
-          const Bits b = cupy::abs_bits(h[e] * static_cast<A>(wv[k].v[e]));
+        // (what is not owned counts as 0 whatever the weight is)
+        const Bits b = cupy::abs_bits(mine.owns(k, e) ? h[e] * static_cast<A>(wv[k].v[e]) : A(0));
 #else
-          const Bits b = cupy::abs_bits(h[e]);
+        const Bits b = cupy::abs_bits(h[e]);
 #endif
-          s.top = b > s.top ? b : s.top;
+        s.top = b > s.top ? b : s.top;
 #endif
-        }
       }
     }
     s = cupy::row_allreduce<LANES, BLOCK>(s, JoinStat(), lds[flip]);
     flip ^= 1;
-    if (!valid) continue;
     const Finish fin(s, width, static_cast<A>(eps));
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const int c = (lane + k * LANES) * VEC;
-      if (c >= width) continue;
+      if (!valid || !mine.any(k)) continue;
       A h[VEC];
       sums_of<VEC>(xv[k], rv[k], h);
 #ifdef RESIDUAL
       cupy::Vec<R_T, VEC> hv;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) hv.v[e] = static_cast<R_T>(h[e]);
-      cupy::store_part<R_T, VEC, NT_OUT>(sum + row * ps + c, hv, width - c);
+      mine.template store<NT_OUT>(k, sum + row * ps, hv);
 #endif
       cupy::Vec<Y_T, VEC> yv;
 #pragma unroll
@@ -160,10 +145,10 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
         yv.v[e] = fin(h[e]);
 #endif
       }
-      cupy::store_part<Y_T, VEC, NT_Y>(y + row * py + c, yv, width - c);
+      mine.template store<NT_Y>(k, y + row * py, yv);
     }
 #ifdef INT8
-    if (lane == 0) scale[row] = static_cast<float>(fin.scale);
+    if (valid && threadIdx.x % LANES == 0) scale[row] = static_cast<float>(fin.scale);
 #endif
   }
 }
@@ -276,53 +261,42 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
   constexpr int kRows = BLOCK / LANES;
   __shared__ Pair lds[2][BLOCK / 64];
   const int lane = threadIdx.x % LANES;
+  const cupy::RowShare<ITEMS, LANES, VEC, TINY> mine(lane, width);
 #ifdef WEIGHT
   cupy::Vec<W_T, VEC> wv[ITEMS];
+  mine.load(wv, w);
   A dw[ITEMS][VEC];
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const int c = (lane + k * LANES) * VEC;
-    if (c < width) wv[k] = cupy::load_part<W_T, VEC>(w + c, width - c);
+  for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[k][e] = A(0);
-  }
 #endif
   int flip = 0;
   for (long long base = (long long)blockIdx.x * kRows; base < rows;
        base += (long long)gridDim.x * kRows) {
-    const long long row = base + threadIdx.x / LANES;
-    const bool valid = kRows == 1 || row < rows;
+    const long long at = base + threadIdx.x / LANES;
+    const bool valid = kRows == 1 || at < rows;
+    const long long row = valid ? at : rows - 1;
     cupy::Vec<X_T, VEC> xv[ITEMS], gv[ITEMS];
     cupy::Vec<R_T, VEC> rv[ITEMS];
-    if (valid) {
-#pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        const int c = (lane + k * LANES) * VEC;
-        if (c < width) {
-          xv[k] = cupy::load_part<X_T, VEC, NT_IN>(x + row * px + c, width - c);
-          gv[k] = cupy::load_part<X_T, VEC, NT_IN>(g + row * pg + c, width - c);
+    mine.template load<NT_IN>(xv, x + row * px);
+    mine.template load<NT_IN>(gv, g + row * pg);
 #ifdef RESIDUAL
-          rv[k] = cupy::load_part<R_T, VEC, NT_IN>(dres + row * pr + c, width - c);
+    mine.template load<NT_IN>(rv, dres + row * pr);
 #endif
-        }
-      }
-    }
     Pair s;
     s.square = s.dot = A(0);
-    if (valid) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        if ((lane + k * LANES) * VEC >= width) continue;
+    for (int k = 0; k < ITEMS; ++k) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const A xe = static_cast<A>(xv[k].v[e]);
-          A a = static_cast<A>(gv[k].v[e]);
+      for (int e = 0; e < VEC; ++e) {
+        const A xe = mine.owns(k, e) ? static_cast<A>(xv[k].v[e]) : A(0);
+        A a = mine.owns(k, e) ? static_cast<A>(gv[k].v[e]) : A(0);
 #ifdef WEIGHT
-          a *= static_cast<A>(wv[k].v[e]);
+        a = mine.owns(k, e) ? a * static_cast<A>(wv[k].v[e]) : A(0);
 #endif
-          s.square = cupy::fma_(xe, xe, s.square);
-          s.dot = cupy::fma_(a, xe, s.dot);
-        }
+        s.square = cupy::fma_(xe, xe, s.square);
+        s.dot = cupy::fma_(a, xe, s.dot);
       }
     }
     s = cupy::row_allreduce<LANES, BLOCK>(s, JoinPair(), lds[flip]);
@@ -331,8 +305,7 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
     const Factors f(s, width, static_cast<A>(eps));
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const int c = (lane + k * LANES) * VEC;
-      if (c >= width) continue;
+      if (!mine.any(k)) continue;
       cupy::Vec<X_T, VEC> d;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -348,7 +321,7 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
 #endif
         d.v[e] = static_cast<X_T>(v);
       }
-      cupy::store_part<X_T, VEC, NT_OUT>(dx + row * pd + c, d, width - c);
+      mine.template store<NT_OUT>(k, dx + row * pd, d);
     }
   }
 #ifdef WEIGHT
@@ -356,24 +329,26 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
   if (kRows == 1) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const int c = (lane + k * LANES) * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (c + e < width) partial[(long long)blockIdx.x * width + c + e] = dw[k][e];
+        if (mine.owns(k, e)) partial[(long long)blockIdx.x * width + mine.at[k] + e] = dw[k][e];
     }
   } else {
     __shared__ A shares[kRows == 1 ? 1 : BLOCK * VEC];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       __syncthreads();
+      // (the elements in their own places, not in those they were loaded from)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) shares[threadIdx.x * VEC + e] = dw[k][e];
+      for (int e = 0; e < VEC; ++e)
+        if (mine.owns(k, e)) shares[threadIdx.x * VEC + e - mine.skip[k]] = dw[k][e];
       __syncthreads();
       for (int i = threadIdx.x; i < LANES * VEC; i += BLOCK) {
+        const int c = k * LANES * VEC + i;
+        if (c >= width) break;
         A t = A(0);
         for (int q = 0; q < kRows; ++q) t += shares[q * LANES * VEC + i];
-        const int c = k * LANES * VEC + i;
-        if (c < width) partial[(long long)blockIdx.x * width + c] = t;
+        partial[(long long)blockIdx.x * width + c] = t;
       }
     }
   }
@@ -508,14 +483,19 @@ def _geometry(width, itemsize, most_items):
     at once and the units hold many rows (16384 x 4096 float16 with residual:
     89 us with 512 lanes, 92 with 256 and two vectors; 9001 x 2047 float32: 50.5
     with 512, 52.8 with 256; 4096 x 8192 to int8: 66 with 1024, 75 with 512, 84
-    with 256).  Rows of up to 64 vectors share a workgroup of 256 threads."""
+    with 256).  Rows of up to 64 vectors share a workgroup of 256 threads, longer
+    ones take whole waves."""
     vec = 16 // itemsize
     n = (width + vec - 1) // vec
-    lanes = min(1024, max(4, _oc.clp2(n)))
+    if n <= 64:
+        return max(4, _oc.clp2(n)), 256, 1, vec
+    # as many lanes for every vector of a lane, whole waves of them
+    each = -(-n // 1024)
+    lanes = min(1024, -(-n // (64 * each)) * 64)
     items = -(-n // lanes)
     if items > most_items:
         return 1024, 1024, 0, vec
-    return lanes, 256 if lanes <= 64 else lanes, items, vec
+    return lanes, lanes, items, vec
 
 
 def _check(x, weight, residual, what):
@@ -622,7 +602,7 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
         x.size * y_dtype.itemsize + (residual.nbytes if residual is not None else 0))
     defines = dict(X_T=x.dtype, R_T=x.dtype if residual is None else residual.dtype,
                    W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
-                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out,
+                   ITEMS=items, VEC=vec, TINY=width < vec, NT_IN=nt_in, NT_OUT=nt_out,
                    # (8 bits fit the cache where the rest does not)
                    NT_Y=nt_out and not int8)
     for name, on in (('INT8', int8), ('WEIGHT', weight is not None),
@@ -630,10 +610,16 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
         if on:
             defines[name] = 1
     fn = _SOURCE.function('cupy_rms_norm', **defines)
-    # a workgroup per row (or 256 / lanes of them): stores run fastest without a
-    # loop around them.  Those of 1024 threads, of which a unit holds two, loop.
+    # A workgroup per row (or 256 / lanes of them): stores run fastest without a
+    # loop around them.  Of those of more than 512 threads a unit holds two: they
+    # loop (4096 x 8192 to int8 66 us, 70 without), unless the last round of the
+    # loop would leave a twentieth of them without a row.
     grid = -(-rows // (block // lanes))
-    grid = min(grid, 2 * _oc.compute_units() if block == 1024 else 0xffffffff // block)
+    resident = 2 * _oc.compute_units()
+    rounds = -(-grid // resident)
+    if block > 512 and grid >= 0.95 * rounds * resident:
+        grid = min(grid, resident)
+    grid = min(grid, 0xffffffff // block)
     call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
                 Ref(0), Ref(i_r) if i_r is not None else 0, Ref(i_w) if i_w is not None else 0,
                 Ref(i_y), Ref(i_s) if int8 else 0, Ref(i_h) if i_h is not None else 0,
@@ -779,7 +765,7 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     nt_in, nt_out = _oc.stream_hints(3 * x.nbytes, x.nbytes)
     defines = dict(X_T=x.dtype, R_T=x.dtype if residual_grad is None else residual_grad.dtype,
                    W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
-                   ITEMS=items, VEC=vec, NT_IN=nt_in, NT_OUT=nt_out)
+                   ITEMS=items, VEC=vec, TINY=width < vec, NT_IN=nt_in, NT_OUT=nt_out)
     for name, on in (('WEIGHT', weight is not None), ('RESIDUAL', residual_grad is not None)):
         if on:
             defines[name] = 1

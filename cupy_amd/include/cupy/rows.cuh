@@ -50,19 +50,61 @@ _CUPY_DEV void store_part(T* p, const Vec<T, N>& x, int have) {
   }
 }
 
-// All-reduce over the kLanes lanes of a row: a group inside a wave, or the
-// whole workgroup of kLanes == kBlock threads through `lds` (kBlock / 64
-// values).  A workgroup that calls this repeatedly alternates between two
-// such arrays: one barrier per call is enough then, because whoever writes an
-// array for the second time has passed the barrier of the call in between.
+// The kItems vectors of a row that one of kLanes lanes works on.  All of them are
+// loaded without a branch between the requests: a vector that would hang over
+// the end of the row is moved back to end with it, and one wholly behind it as
+// well.  What a moved vector shares with its neighbours is theirs: it is left
+// out of sums (`owns`), and stored twice with the same values.
+// kTiny: rows shorter than a vector, loaded and stored by elements.
+template <int kItems, int kLanes, int kVec, bool kTiny>
+struct RowShare {
+  int width;
+  int at[kItems];       // first column, as loaded
+  int skip[kItems];     // elements of it that are not this lane's
+  _CUPY_DEV RowShare(int lane, int w) : width(w) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int c = (lane + k * kLanes) * kVec;
+      at[k] = kTiny ? 0 : c + kVec <= w ? c : w - kVec;
+      const int s = c - at[k];
+      skip[k] = s < kVec ? s : kVec;
+    }
+  }
+  _CUPY_DEV bool owns(int k, int e) const { return e >= skip[k] && (!kTiny || e < width); }
+  _CUPY_DEV bool any(int k) const { return skip[k] < kVec; }
+  template <bool kStream = false, typename T>
+  _CUPY_DEV void load(Vec<T, kVec> (&v)[kItems], const T* row) const {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      v[k] = kTiny ? load_part<T, kVec>(row, width) : load_vec<T, kVec, kStream>(row + at[k]);
+  }
+  template <bool kStream, typename T>
+  _CUPY_DEV void store(int k, T* row, const Vec<T, kVec>& v) const {
+    if (kTiny) store_part<T, kVec>(row, v, width);
+    else store_vec<T, kVec, kStream>(row + at[k], v);
+  }
+};
+
+constexpr int _ceil_pow2(int n, int p = 1) { return p >= n ? p : _ceil_pow2(n, 2 * p); }
+
+// All-reduce over the kLanes lanes of a row: a group inside a wave (a power of
+// two), or the whole workgroup of kLanes == kBlock threads, any number of
+// waves, through `lds` (a value per wave).  A value of zeros has to be the
+// identity of `op`.  A workgroup that calls this repeatedly alternates between
+// two such arrays: one barrier per call is enough then, because whoever writes
+// an array for the second time has passed the barrier of the call in between.
 template <int kLanes, int kBlock, typename T, typename Op>
 _CUPY_DEV T row_allreduce(T v, Op op, T* lds) {
   if (kLanes <= 64) return group_allreduce<(kLanes <= 64 ? kLanes : 64)>(v, op);
   constexpr int kWaves = kBlock / 64 > 0 ? kBlock / 64 : 1;
+  constexpr int kGroup = _ceil_pow2(kWaves);
   v = group_allreduce<64>(v, op);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  return group_allreduce<kWaves>(lds[threadIdx.x & (kWaves - 1)], op);
+  const int from = threadIdx.x & (kGroup - 1);
+  T w = lds[from < kWaves ? from : 0];
+  if (from >= kWaves) w = T();
+  return group_allreduce<kGroup>(w, op);
 }
 
 }  // namespace cupy

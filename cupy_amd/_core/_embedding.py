@@ -33,30 +33,30 @@ cupy_embedding(const X_T* table, const I_T* ids, X_T* out, const long long n, co
   for (long long t = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t < n; t += step) {
     const long long id = ids[t];
     const bool met = id >= 0 && id < rows;
+    const X_T* row = table + (met ? id : 0) * pt;      // (the table has a row)
     cupy::Vec<X_T, VEC> v[ITEMS];
+    int c[ITEMS];
+    // A vector over the end of the row moves back to end with it: what it shares
+    // with its neighbour is stored twice.  Nothing stands between the requests.
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const long long c = ((long long)(blockIdx.y * ITEMS + k) * LANES + lane) * VEC;
-      if (c >= width) continue;
-      if (met) {
-        v[k] = cupy::load_part<X_T, VEC>(table + id * pt + c, width - c < VEC ? (int)(width - c) : VEC);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[k].v[e] = static_cast<X_T>(0.0f);
-      }
+      c[k] = ((blockIdx.y * ITEMS + k) * LANES + lane) * VEC;
+      const int at = TINY ? 0 : c[k] + VEC <= width ? c[k] : width - VEC;
+      v[k] = TINY ? cupy::load_part<X_T, VEC>(row, width) : cupy::load_vec<X_T, VEC>(row + at);
     }
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const long long c = ((long long)(blockIdx.y * ITEMS + k) * LANES + lane) * VEC;
-      if (c >= width) continue;
-#ifdef SCALE
-      if (met) {
+      if (c[k] >= width) break;
+      const int at = TINY ? 0 : c[k] + VEC <= width ? c[k] : width - VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          v[k].v[e] = static_cast<X_T>(static_cast<A>(v[k].v[e]) * static_cast<A>(scale));
-      }
+      for (int e = 0; e < VEC; ++e) {
+#ifdef SCALE
+        v[k].v[e] = static_cast<X_T>(static_cast<A>(v[k].v[e]) * static_cast<A>(scale));
 #endif
-      cupy::store_part<X_T, VEC, NT_OUT>(out + t * po + c, v[k], width - c < VEC ? (int)(width - c) : VEC);
+        if (!met) v[k].v[e] = static_cast<X_T>(0.0f);
+      }
+      if (TINY) cupy::store_part<X_T, VEC>(out + t * po, v[k], width);
+      else cupy::store_vec<X_T, VEC, NT_OUT>(out + t * po + at, v[k]);
     }
   }
 }
@@ -344,9 +344,12 @@ cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
   constexpr int UNROLL = 8;
   const A scale = static_cast<A>(scale_);
   const long long ch = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  const long long c = ((long long)blockIdx.y * LANES + threadIdx.x % LANES) * VEC;
+  int c = (blockIdx.y * LANES + threadIdx.x % LANES) * VEC;
   if (ch >= chunks || c >= width) return;
-  const int have = width - c < VEC ? (int)(width - c) : VEC;
+  // (a vector over the end of the row moves back to end with it: the columns it
+  // shares with its neighbour are summed and stored twice, alike)
+  if (!TINY && c + VEC > width) c = width - VEC;
+  const int have = TINY ? width : VEC;
   const u32* keys = temp + at_pairs;
   const u32* pos = keys + n;
   A* partial = reinterpret_cast<A*>(temp + at_partial);
@@ -377,8 +380,8 @@ cupy_embedding_sums(const G_T* g, u32* temp, O_T* out, const long long at_pairs,
     // (positions are in range whatever their token: nothing to wait for)
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      v[u] = WHOLE ? cupy::load_vec<G_T, VEC>(g + (long long)at[u] * pg + c)
-                   : cupy::load_part<G_T, VEC>(g + (long long)at[u] * pg + c, have);
+      v[u] = TINY ? cupy::load_part<G_T, VEC>(g + (long long)at[u] * pg + c, have)
+                  : cupy::load_vec<G_T, VEC>(g + (long long)at[u] * pg + c);
     const long long ahead = t + UNROLL < t1 ? t + UNROLL : t;
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -484,7 +487,7 @@ cupy_embedding_join(const u32* temp, O_T* out, const long long at_pairs,
 ''')
 
 # most pairs that are put in order by comparing all of them
-_RANKED = 8192
+_RANKED = 12288
 
 _plans = {}
 _plans_grad = {}
@@ -527,8 +530,11 @@ def embedding(table, ids, scale=1.0, *, out=None):
     call = _oc.Call(_plans, key, arrays, 2)
     i_out = 2 if out is not None else call.allocate(shape, table.dtype)
     n = ids.size
-    if n == 0 or width == 0:
+    if n == 0 or width == 0 or rows == 0:
+        # (the kernel reads some row for every id: without rows it is not run)
         call.key = None
+        if call.refs[i_out].size:
+            call.refs[i_out].fill(0)
         call.begin()
         return call.finish(i_out)
     call.convert(1, _oc.as_index(call.refs[1]))
@@ -545,7 +551,7 @@ def embedding(table, ids, scale=1.0, *, out=None):
     grid_x = min(-(-n // per), (1 << 24) - 1)
     nt_out = _oc.stream_hints(n * width * table.dtype.itemsize, n * width * table.dtype.itemsize)[1]
     defines = dict(X_T=table.dtype, I_T=call.refs[1].dtype, LANES=lanes, ITEMS=items, VEC=vec,
-                   NT_OUT=nt_out)
+                   TINY=width < vec, NT_OUT=nt_out)
     if scale != 1.0:
         defines['SCALE'] = 1
     fn = _LOOKUP.function('cupy_embedding', **defines)
@@ -663,7 +669,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
                         cuts[2 * p + 1], cuts[2 * p + 2])
     vec = 16 // grad.dtype.itemsize
     lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
-    defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec, WHOLE=width % vec == 0)
+    defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec, TINY=width < vec)
     fn = _SUMS.function('cupy_embedding_sums', **defines)
     call.launch(fn, (-(-chunks // (256 // lanes)), -(-width // (lanes * vec)), 1), 256,
                 'PPPqqqIiqqiid', Ref(0), Ref(i_t), Ref(i_out), at, words, n, num_rows, width,

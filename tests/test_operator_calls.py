@@ -324,3 +324,13 @@ def test_records_are_found_by_layout_not_by_address():
     keys = {_op_calls.replay({}, [x], e)[1] for x, e in
             ((a, (1,)), (a, (2,)), (a[:, ::2], (1,)), (arr((4, 8), 'float16'), (1,)))}
     assert len(keys) == 4
+
+
+@dry
+def test_no_kernel_reads_a_table_of_no_rows():
+    _dryrun.launches.clear()
+    out = cp.embedding(arr((0, 4)), arr(3, 'int64'))
+    cp.embedding(arr((0, 4)), arr(3, 'int64'), out=out)
+    cp.embedding_grad(out, arr(3, 'int64'), 0)
+    assert out.shape == (3, 4)
+    assert not [l for l in _dryrun.launches if l[0].startswith('cupy_embedding')]

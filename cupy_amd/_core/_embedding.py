@@ -10,6 +10,7 @@ Runs that cross the border of a chunk leave partial sums that a last kernel
 joins, in order.  The reference scatters such gradients atomically
 (cupy/_core/_routines_indexing.pyx:899-1120 ``_scatter_op``).
 """
+import math
 import operator
 
 import numpy
@@ -513,7 +514,8 @@ def embedding(table, ids, scale=1.0, *, out=None):
     """
     scale = float(scale)
     arrays = [table, ids] if out is None else [table, ids, out]
-    result, key = _oc.replay(_plans, arrays, (scale, len(arrays)))
+    # (0.0 and -0.0 are one key, but two results)
+    result, key = _oc.replay(_plans, arrays, (scale, math.copysign(1.0, scale)))
     if result is not _oc._NOTHING:
         return result
     _oc.check_float(table, 'table')
@@ -580,8 +582,14 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
             both ``out`` and ``dtype``.
     """
     scale = float(scale)
+    num_rows = operator.index(num_rows)
+    if dtype is not None:
+        if out is not None:
+            raise TypeError('embedding_grad() takes `out` or `dtype`, but both were provided.')
+        dtype = numpy.dtype(dtype)
     arrays = [grad, ids] if out is None else [grad, ids, out]
-    result, key = _oc.replay(_plans_grad, arrays, (scale, len(arrays), num_rows, dtype))
+    result, key = _oc.replay(
+        _plans_grad, arrays, (scale, math.copysign(1.0, scale), num_rows, dtype))
     if result is not _oc._NOTHING:
         return result
     _oc.check_float(grad, 'grad')
@@ -591,21 +599,18 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     if grad.ndim != ids.ndim + 1 or grad._shape[:-1] != ids._shape:
         raise ValueError('grad has the shape %r, ids the shape %r: one row per id is expected'
                          % (grad._shape, ids._shape))
-    num_rows = operator.index(num_rows)
     if not 0 <= num_rows < (1 << 31) - 1:
         raise ValueError('num_rows must be at least 0 and below 2**31 - 1')
     width = grad._shape[-1]
     n = ids.size
     _check_width(width)
-    if n >= 1 << 31:
-        raise ValueError('2**31 ids and more are not supported')
+    if n >= 1 << 30:
+        raise ValueError('2**30 ids and more are not supported')
     if out is not None:
-        if dtype is not None:
-            raise TypeError('embedding_grad() takes `out` or `dtype`, but both were provided.')
         _oc.check_array(out, 'out')
         dt = out.dtype
     else:
-        dt = grad.dtype if dtype is None else numpy.dtype(dtype)
+        dt = grad.dtype if dtype is None else dtype
     if dt != grad.dtype and not (grad.dtype.char == 'e' and dt.char == 'f'):
         raise TypeError('a gradient of type %s is not summed into %s: its own type, or float32 '
                         'with float16' % (grad.dtype, dt))

@@ -8,7 +8,6 @@ take a few launches: the squares are summed per piece of 32 KiB, a single
 workgroup joins the pieces' sums in order and derives the factor, and the
 scaling reads it from device memory: nothing waits for the host.
 """
-import functools
 import struct
 
 import numpy
@@ -110,7 +109,7 @@ struct Add {
 // float16: 64 squares, at most 2^32 each, are added in 32 bits, the rest in 64.
 // float32: the squares are taken in 64 bits, where none over- or underflows.
 extern "C" __global__ void __launch_bounds__(BLOCK)
-cupy_square_sums(const Table t, const int entries, double* sums) {
+cupy_square_sums(const Table t, const int entries, double* temp, const long long at) {
   __shared__ double lds[BLOCK / 64];
   const int k = entry_of(t, entries, blockIdx.x);
   const Entry e = t.e[k];
@@ -138,15 +137,15 @@ cupy_square_sums(const Table t, const int entries, double* sums) {
       }
   }
   total = cupy::row_allreduce<BLOCK, BLOCK>(total, Add(), lds);
-  if (threadIdx.x == 0) sums[blockIdx.x] = total;
+  if (threadIdx.x == 0) temp[at + blockIdx.x] = total;
 }
 
 extern "C" __global__ void __launch_bounds__(BLOCK)
-cupy_scale_arrays(const Table t, const int entries, const int blocks, const double* factor_) {
+cupy_scale_arrays(const Table t, const int entries, const int blocks, const double* temp) {
   // last pieces first: they are what the sums have left in the cache
   const unsigned int block = blocks - 1 - blockIdx.x;
   const Entry e = t.e[entry_of(t, entries, block)];
-  const A factor = static_cast<A>(*factor_);
+  const A factor = static_cast<A>(temp[0]);
   if (factor == A(1) && e.src == e.dst) return;       // what is there is the result
   Piece p;
   p.load(e, block - e.first);
@@ -165,11 +164,13 @@ _FINISH = _oc.Source(r'''
 struct Add {
   template <typename T> _CUPY_DEV T operator()(T a, T b) const { return a + b; }
 };
-// One workgroup: every thread a run of the sums, the threads by a tree.
+// One workgroup: every thread a run of the sums, which follow the place of the
+// factor, the threads by a tree.
 extern "C" __global__ void __launch_bounds__(1024)
-cupy_norm_of_sums(const double* sums, const long long n, N_T* norm, double* factor,
-                  const double max_norm, const double eps) {
+cupy_norm_of_sums(double* temp, const long long n, N_T* norm, const double max_norm,
+                  const double eps) {
   __shared__ double lds[16];
+  const double* sums = temp + 1;
   double t = 0.0;
   for (long long i = threadIdx.x; i < n; i += 8 * 1024) {
     double v[8];
@@ -183,7 +184,7 @@ cupy_norm_of_sums(const double* sums, const long long n, N_T* norm, double* fact
     const double r = __builtin_sqrt(t);
     *norm = static_cast<N_T>(r);
     const double q = max_norm / (r + eps);
-    *factor = q >= 1.0 ? 1.0 : q;       // (a NaN stays one)
+    temp[0] = q >= 1.0 ? 1.0 : q;       // (a NaN stays one)
   }
 }
 ''')
@@ -265,8 +266,28 @@ def _tables(src, dst):
     return found
 
 
-def _launch(fn, blocks, block, *parts):
-    fn.launch_packed((blocks, 1, 1), (block, 1, 1), b''.join(parts), 0)
+class _Temporary:
+    """``words`` doubles for the launches of one call, or the runtime library's
+    static array where nothing may be allocated."""
+
+    def __init__(self, words):
+        self.nbytes = 8 * words
+        self.static = _memory.static_scratch_active()
+        if not self.static:
+            self.memory = _memory.alloc(self.nbytes)
+        elif self.nbytes > _rt.RT_SCRATCH_MAX_BYTES:
+            raise RuntimeError(
+                'static_scratch: the call needs %d bytes of scratch memory, the runtime '
+                'library holds %d' % (self.nbytes, _rt.RT_SCRATCH_MAX_BYTES))
+
+    def launch(self, fn, blocks, block, before, after=b''):
+        """``before`` and ``after`` are the arguments around the temporary's address."""
+        if self.static:
+            fn.launch_packed_scratch((blocks, 1, 1), (block, 1, 1), before + bytes(8) + after,
+                                     len(before), self.nbytes)
+        else:
+            fn.launch_packed((blocks, 1, 1), (block, 1, 1),
+                             before + struct.pack('<Q', self.memory.ptr) + after)
 
 
 def _defines(dtype, nbytes):
@@ -311,22 +332,21 @@ def _run(arrays, targets, norm_out, max_norm, eps):
             src, dst = _describe(reads, 'arrays'), _describe(writes, 'out')
     tables = _tables(src, dst)
     total = sum(blocks for _, launches, _ in tables for _, _, blocks in launches)
-    temp = _memory.alloc((total + 1) * 8)     # the factor, then the sums
-    word = functools.partial(struct.pack, '<Q')
-    at = temp.ptr + 8
+    temp = _Temporary(total + 1)              # the factor, then the sums
+    at = 1
     for t, launches, nbytes in tables:
         fn = _SOURCE.function('cupy_square_sums', **_defines(t, nbytes))
         for table, n, blocks in launches:
-            _launch(fn, blocks, _BLOCK, table, word(n), word(at))
-            at += blocks * 8
+            temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, 0), struct.pack('<q', at))
+            at += blocks
     fn = _FINISH.function('cupy_norm_of_sums', N_T=dtype)
-    _launch(fn, 1, 1024, struct.pack('<QqQQdd', temp.ptr + 8, total, norm_out.data.ptr, temp.ptr,
-                                     0.0 if max_norm is None else max_norm, eps))
+    temp.launch(fn, 1, 1024, b'', struct.pack('<qQdd', total, norm_out.data.ptr,
+                                              0.0 if max_norm is None else max_norm, eps))
     if max_norm is not None:
         for t, launches, nbytes in reversed(tables):
             fn = _SOURCE.function('cupy_scale_arrays', **_defines(t, nbytes))
             for table, n, blocks in reversed(launches):
-                _launch(fn, blocks, _BLOCK, table, struct.pack('<iiQ', n, blocks, temp.ptr))
+                temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, blocks))
         for i in aside:
             elementwise_copy(writes[i], finals[i])
     return norm_out

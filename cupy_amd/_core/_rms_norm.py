@@ -659,8 +659,8 @@ def rms_norm_int8(x, weight=None, residual=None, eps=1e-6, *, out=None, scale_ou
 
     ``scale = max(|y|) / 127`` over the row (float32) and
     ``q = rint(y / scale)``, ties to even: ``q * scale`` is ``y`` to half a
-    step.  A row of zeros has the scale 0; in a row with a NaN or an infinity
-    the scale is NaN.
+    step.  A row of zeros has the scale 0 (``eps`` above 0); in a row with a NaN
+    or an infinity the scale is NaN.
 
     Returns:
         ``(q, scale)``, or ``(q, scale, h)`` with a residual: int8 shaped like

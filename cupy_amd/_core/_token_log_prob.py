@@ -10,6 +10,7 @@ one pass over the row with a running maximum ``m``, the sum ``s`` of
 them from reductions (cupyx/scipy/special/_softmax.py, _logsumexp.py).
 """
 import collections
+import operator
 
 import numpy
 
@@ -192,9 +193,10 @@ _CUPY_DEV Key key_at(const cupy::Vec<X_T, VEC>& v, int j, int i, const RowVecs& 
   return key_of(static_cast<A>(v.v[i]), (u32)(vecs.column(j) + i));
 }
 
-constexpr int kMost = 1024;     // keys that are ranked against each other
-
+// kMost: keys that are ranked against each other
+template <int kMost_>
 struct TopState {
+  static constexpr int kMost = kMost_;
   Key sample[64];               // (no two alike)
   Key key[kMost];
   Key last;
@@ -202,7 +204,8 @@ struct TopState {
 };
 
 // The TOP-th best of the 64 sample keys: at least TOP keys are as good.
-_CUPY_DEV Key bar(const TopState& t) {
+template <typename State>
+_CUPY_DEV Key bar(const State& t) {
   const Key me = t.sample[threadIdx.x & 63];
   int rank = 0;
 #pragma unroll 8
@@ -211,10 +214,11 @@ _CUPY_DEV Key bar(const TopState& t) {
 }
 
 // Keeps an element that is as good as `least` (a NaN is none: its row has no order).
-_CUPY_DEV void offer(TopState& t, A value, const Key& k, const Key& least) {
+template <typename State>
+_CUPY_DEV void offer(State& t, A value, const Key& k, const Key& least) {
   if (better(least, k) | !(value == value)) return;
   const u32 at = atomicAdd(&t.n, 1u);
-  if (at < kMost) t.key[at] = k;
+  if (at < State::kMost) t.key[at] = k;
 }
 #endif
 '''
@@ -222,8 +226,8 @@ _CUPY_DEV void offer(TopState& t, A value, const Key& k, const Key& least) {
 _SOURCE = _oc.Source(_COMMON + r'''
 #if TOP > 0
 // Writes the n <= kMost keys collected in t by rank, the best TOP of them.
-template <typename Put>
-_CUPY_DEV void put_ranked(const TopState& t, u32 n, Put put) {
+template <typename State, typename Put>
+_CUPY_DEV void put_ranked(const State& t, u32 n, Put put) {
   for (u32 q = threadIdx.x; q < n; q += blockDim.x) {
     const Key me = t.key[q];
     int rank = 0;
@@ -284,7 +288,8 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
   constexpr int kWaves = BLOCK / 64;
   __shared__ Run lds[kWaves];
 #if TOP > 0
-  __shared__ TopState ts;
+  constexpr int kMost = BLOCK < 256 ? 4 * BLOCK : 1024;
+  __shared__ TopState<kMost> ts;
 #endif
   Outputs out;
   out.log_prob = log_prob;
@@ -479,7 +484,10 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
   run.s = from[1];
   run.u = from[2];
 #if TOP > 0
-  __shared__ TopState ts;
+  // (the TOP-th best of the first of every part: at most TOP parts have keys as
+  // good, TOP each)
+  constexpr int kMost = MAX_TOP * MAX_TOP;
+  __shared__ TopState<kMost> ts;
   const Key* keys = reinterpret_cast<const Key*>(runs + at_keys) + row * parts * TOP;
   constexpr int kEach = (64 * TOP + 255) / 256;
   Key mine[kEach];
@@ -515,7 +523,7 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
     if (!is_none(mine[q])) offer(ts, value_of(mine[q]), mine[q], least);
   __syncthreads();
   const double lse_ = run.lse();
-  put_ranked(ts, ts.n < kMost ? ts.n : kMost,
+  put_ranked(ts, ts.n,
              [&](int rank, const Key& k) { put_top(out, run, lse_, row, rank, k); });
 #endif
 }
@@ -628,20 +636,21 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         exponentials, which the gradient takes), ``entropy``, ``top_log_prob``
         and ``top_token``; float32 (float64 for float64) and int64.
     """
-    entropy = bool(entropy)
+    entropy, top = bool(entropy), operator.index(top)
     arrays = [logits, tokens]
+    given = None
     if out is not None:
-        arrays.extend([a for a in out if a is not None])
-    result, key = _oc.replay(_plans, arrays, (entropy, top, out is None))
+        if type(out) is not TokenLogProb:
+            raise TypeError('out must be a TokenLogProb')
+        arrays += [a for a in out if a is not None]
+        given = (out.entropy is None, out.top_log_prob is None, out.top_token is None)
+    result, key = _oc.replay(_plans, arrays, (entropy, top, given))
     if result is not _oc._NOTHING:
         return _named(result, entropy, top)
-    given, tokens = tokens, _oc.index_array(tokens, 'tokens')
-    if given is not tokens:
+    as_given, tokens = tokens, _oc.index_array(tokens, 'tokens')
+    if as_given is not tokens:
         key, arrays[1] = None, tokens
     width = _check_logits(logits, tokens)
-    if isinstance(top, bool) or not isinstance(top, (int, numpy.integer)):
-        raise TypeError('top must be an integer')
-    top = int(top)
     if not 0 <= top <= min(MAX_TOP, width):
         raise ValueError('top must be between 0 and %d, got %d' % (min(MAX_TOP, width), top))
     acc = _oc.acc_dtype(logits.dtype)
@@ -653,8 +662,6 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         specs.append((lead + (top,), acc, 'top_log_prob'))
         specs.append((lead + (top,), numpy.dtype(numpy.int64), 'top_token'))
     if out is not None:
-        if not isinstance(out, TokenLogProb):
-            raise TypeError('out must be a TokenLogProb')
         asked = {name for _, _, name in specs}
         for name, a in zip(out._fields, out):
             if (a is None) == (name in asked):
@@ -679,10 +686,10 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         call.dense(i)
     call.begin()
     vec = 16 // logits.dtype.itemsize
-    block, unroll, parts = _geometry(rows, max(1, width // vec), top)
+    block, unroll, parts = _geometry(rows, max(1, width // vec))
     nt_in = _oc.stream_hints(logits.nbytes, 0)[0] and not top
     defines = dict(X_T=logits.dtype, I_T=call.refs[1].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
-                   TOP=top, SMALL_KEYS=int(acc == numpy.float32), NT_IN=nt_in, NT_OUT=False)
+                   TOP=top, MAX_TOP=MAX_TOP, SMALL_KEYS=int(acc == numpy.float32), NT_IN=nt_in, NT_OUT=False)
     if entropy:
         defines['ENTROPY'] = 1
     slots = [Ref(i) for i in at[:2]]
@@ -704,16 +711,26 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
     return _named(call.finish(ret), entropy, top)
 
 
-def _geometry(rows, vecs, top):
+def _geometry(rows, vecs):
     """(threads of a workgroup, vectors a thread requests at a time, parts of a row)"""
     units = _oc.compute_units()
-    # A workgroup per row: of 256 threads, so that a unit holds eight whose
-    # reductions do not wait for each other (8192 rows of 50257 float16 with
-    # entropy: 178 us with 256, 187 with 512, 225 with 1024).  Rows too few to
-    # fill the device are cut into parts, of at least two vectors per thread.
     block, parts = 256, 1
-    if rows < 2 * units and vecs > 512:
+    if rows < 2 * units and vecs > 8192:
+        # Rows too few to fill the device are cut into parts; a second launch
+        # joins them, which costs about 5 us (64 rows of 32000 float16: 13.5 us
+        # in parts, 11.5 in one launch; 8 rows of 131072 float32: 12.5 against 25).
         parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
+    elif rows < 4 * units:
+        # (300 rows of 32000 float32: 19 us with 512 threads to a row, 21 with
+        # 256; 1000 rows of 16000 float16: 22.9 and 19.7)
+        block = 512 if vecs > 2048 else 256
+    elif vecs <= 512:
+        # Short rows: one wave to each, whose reductions meet no barrier (16384
+        # rows of 1500 float16: 18.5 us; 23.9 with two waves, 31.2 with four; with
+        # 5 alternatives 38.9, 55 and 83).  Long ones: four waves, so that a unit
+        # holds eight rows (8192 rows of 50257 float16 with entropy: 140 us; 175
+        # with eight waves, 220 with sixteen).
+        block = 64
     return block, 4, parts
 
 
@@ -777,7 +794,8 @@ def token_log_prob_grad(grad, logits, tokens, lse, *, entropy=None, entropy_grad
         call.begin()
         return call.finish(i_out)
     for i, _ in per_row:
-        call.convert(i, call.refs[i].astype(acc, copy=False))
+        if call.refs[i].dtype != acc:
+            call.convert(i, call.refs[i].astype(acc))
         call.dense(i)
     call.convert(2, _oc.as_index(call.refs[2]))
     pitch, po = call.rows(1), call.rows(i_out)
@@ -785,8 +803,9 @@ def token_log_prob_grad(grad, logits, tokens, lse, *, entropy=None, entropy_grad
     rows = tokens.size
     vec = 16 // logits.dtype.itemsize
     vecs = max(1, width // vec)
-    block = 256
+    # four vectors a thread; short rows: as many waves as take a vector per lane
     unroll = 4 if vecs > 1024 else 2 if vecs > 256 else 1
+    block = min(256, -(-vecs // 64) * 64)
     blocks = -(-vecs // (block * unroll))
     nt_in, nt_out = _oc.stream_hints(logits.nbytes, logits.nbytes)
     defines = dict(X_T=logits.dtype, I_T=call.refs[2].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,

@@ -160,3 +160,22 @@ def test_streams():
     for n, outs in results:
         assert np.array_equal(n.get(), want)
         assert all(np.array_equal(o.get(), f) for o, f in zip(outs, first))
+
+
+def test_static_scratch():
+    arrays = [cp.asarray(a) for a in make([(300, 70), (17,), (5, 9)], 'float16', 1)]
+    outs, n = [cp.empty_like(a) for a in arrays], cp.empty((), 'float32')
+    cp.clip_by_global_norm(arrays, 1.0, out=outs, norm_out=n)
+    want, want_n = [o.get() for o in outs], n.get()
+    for o in outs:
+        o.fill(0)
+    n.fill(0)
+    with cp.cuda.memory.static_scratch():
+        cp.clip_by_global_norm(arrays, 1.0, out=outs, norm_out=n)
+    assert np.array_equal(n.get(), want_n)
+    assert all(np.array_equal(o.get(), w) for o, w in zip(outs, want))
+    with cp.cuda.memory.static_scratch():
+        with pytest.raises(RuntimeError):
+            cp.clip_by_global_norm(arrays, 1.0, out=outs)
+        with pytest.raises(RuntimeError):
+            cp.clip_by_global_norm([a.T[::2] for a in arrays[:1]], 1.0, norm_out=n)

@@ -114,7 +114,8 @@ def test_captured_into_a_graph():
     r = cp.TokenLogProb(cp.empty(N, 'float32'), cp.empty(N, 'float32'), cp.empty(N, 'float32'),
                         cp.empty((N, 4), 'float32'), cp.empty((N, 4), 'int64'))
     dy, dh, dw = cp.empty((N, V), 'float32'), cp.empty((N, V), 'float32'), cp.empty(V, 'float32')
-    b = cp.empty((N, V), 'float32')
+    b, table_grad, norm = cp.empty((N, V), 'float32'), cp.empty((V, V), 'float32'), cp.empty((), 'float32')
+    clipped = [cp.empty((V, V), 'float32'), cp.empty(V, 'float32')]
 
     def work():
         cp.embedding(dev[0], dev[3], SCALE, out=x)
@@ -123,12 +124,14 @@ def test_captured_into_a_graph():
         cp.token_log_prob(y, dev[4], entropy=True, top=4, out=r)
         cp.token_log_prob_grad(g, y, dev[4], r.lse, out=dy)
         cp.rms_norm_grad(dy, h, dev[2], EPS, out=dh, weight_out=dw)
+        cp.embedding_grad(dh, dev[3], V, SCALE, out=table_grad)
+        cp.clip_by_global_norm([table_grad, dw], 1e-3, out=clipped, norm_out=norm)
 
     stream = cp.cuda.Stream(non_blocking=True)
     with stream:
         work()
     stream.synchronize()
-    outs = [x, b, y, h, dy, dh, dw] + list(r)
+    outs = [x, b, y, h, dy, dh, dw, table_grad, norm] + clipped + list(r)
     want = [a.get() for a in outs]
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(torch.cuda.ExternalStream(stream.ptr)):

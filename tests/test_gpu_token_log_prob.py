@@ -52,8 +52,9 @@ class Exact:
 
 
 def chain(width):
-    # additions a lane makes (at least 256 lanes, or a vector each), and joins
-    return width / 256 + 40
+    # additions a lane makes (64 lanes to rows of up to 512 vectors of 8 elements,
+    # at least 256 to longer ones), and joins
+    return width / (64 if width <= 4104 else 256) + 40
 
 
 def check(x, tokens, got, top=0):
@@ -89,7 +90,8 @@ def check(x, tokens, got, top=0):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('shape', [(1, 1), (3, 2), (5, 33), (40, 64), (700, 1001), (4, 3, 257),
-                                   (2, 50257), (600, 8193), (1, 200003), (130, 5000), (17,)])
+                                   (2, 50257), (600, 8193), (1, 200003), (130, 5000), (17,),
+                                   (1100, 1), (1030, 40), (2000, 1001), (1200, 4095), (1024, 9000)])
 def test_log_prob(shape, dtype):
     x, t = logits_of(shape, dtype), tokens_of(shape)
     xd, td = cp.asarray(x), cp.asarray(t)
@@ -138,9 +140,11 @@ def test_ties_masks_and_bands(dtype, width):
     for top in (1, 7, 32):
         check(x, t, cp.token_log_prob(xd, td, entropy=True, top=top), top)
     # many rows: a workgroup each
-    big = np.tile(x, (60, 1))
-    check(big, np.tile(t, 60), cp.token_log_prob(cp.asarray(big), cp.asarray(np.tile(t, 60)),
-                                                 entropy=True, top=9), 9)
+    for n in (60, 104 if width < 20000 else 0):
+        big = np.tile(x, (n, 1))
+        if n:
+            check(big, np.tile(t, n), cp.token_log_prob(cp.asarray(big), cp.asarray(np.tile(t, n)),
+                                                        entropy=True, top=9), 9)
 
 
 @pytest.mark.parametrize('dtype', TYPES)
@@ -159,6 +163,15 @@ def test_the_best_in_the_vectors_of_one_thread(dtype):
         got = cp.token_log_prob(cp.asarray(x), cp.asarray(t), top=20)
         order = np.argsort(-x[0].astype(np.float64), kind='stable')[:20]
         assert np.array_equal(got.top_token.get(), np.broadcast_to(order, (rows, 20)))
+    # a wave to each row: all of the best in 16 of its lanes
+    rows, width = 1100, 64 * vec * 8 + 3
+    x = np.full((rows, width), -3.0, dtype)
+    cols = np.arange(width)
+    high = (cols // vec) % 64 < 16
+    x[:, high] = (np.arange(high.sum()) % 500 / 100).astype(dtype)
+    got = cp.token_log_prob(cp.asarray(x), cp.zeros(rows, 'int64'), top=20)
+    order = np.argsort(-x[0].astype(np.float64), kind='stable')[:20]
+    assert np.array_equal(got.top_token.get(), np.broadcast_to(order, (rows, 20)))
 
 
 def test_rows_with_nothing_left_and_with_nan():
@@ -211,7 +224,7 @@ def check_grad(got, x, t, lse, g, h=None, gh=None):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('shape', [(1, 1), (3, 2), (5, 33), (600, 1001), (4, 3, 257), (2, 50257),
-                                   (33, 5000), (17,)])
+                                   (33, 5000), (17,), (50, 130), (40, 600), (30, 2300)])
 def test_gradient(shape, dtype):
     x, t = logits_of(shape, dtype, 4), tokens_of(shape, 5)
     if t.ndim == 1 and len(t) > 2:

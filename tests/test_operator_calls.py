@@ -334,3 +334,42 @@ def test_no_kernel_reads_a_table_of_no_rows():
     cp.embedding_grad(out, arr(3, 'int64'), 0)
     assert out.shape == (3, 4)
     assert not [l for l in _dryrun.launches if l[0].startswith('cupy_embedding')]
+
+
+@dry
+@pytest.mark.parametrize('which', range(8))
+def test_calls_on_arrays_as_they_are_are_recorded(which):
+    from cupy_amd._core import _embedding, _rms_norm, _token_log_prob
+    tables = [_rms_norm._plans, _rms_norm._plans_int8, _rms_norm._plans_grad, _embedding._plans,
+              _embedding._plans_grad, _token_log_prob._plans, _token_log_prob._plans_grad]
+    for t in tables:
+        t.clear()
+    call = calls()[which]
+    call(), call()
+    assert sum(len(t) for t in tables) == 1
+
+
+@dry
+def test_options_that_compare_equal_are_not_mixed_up():
+    table, ids = arr((10, 4)), arr((3,), 'int64')
+    scales = []
+    for scale in (0.0, -0.0, 0.0):
+        _dryrun.launches.clear()
+        cp.embedding(table, ids, scale)
+        scales.append(struct.unpack_from('<d', _dryrun.launches[-1][4], 64)[0])
+    assert [str(s) for s in scales] == ['0.0', '-0.0', '0.0']
+    cp.embedding_grad(arr((3, 4)), ids, 10)
+    with pytest.raises(TypeError):
+        cp.embedding_grad(arr((3, 4)), ids, 10.0)
+    x, t = arr((4, 50)), arr((4,), 'int64')
+    cp.token_log_prob(x, t, top=1)
+    with pytest.raises(TypeError):
+        cp.token_log_prob(x, t, top=1.0)
+    # an array in the place of another result of the same shape and type
+    out = cp.TokenLogProb(arr(4), arr(4), arr(4), None, None)
+    cp.token_log_prob(x, t, entropy=True, out=out)
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, t, entropy=True,
+                          out=cp.TokenLogProb(arr(4), arr(4), None, arr(4), None))
+    with pytest.raises(TypeError):
+        cp.token_log_prob(x, t, out=(arr(4), arr(4), None, None, None))

@@ -194,9 +194,6 @@ _TYPES = [numpy.dtype(c) for c in _oc.FLOATS]
 
 def _describe(arrays, name):
     """Addresses, sizes, types and layouts of a list of arrays, checked."""
-    for a in arrays:
-        if not isinstance(a, ndarray):
-            raise TypeError('%s must hold cupy.ndarrays, got %s' % (name, type(a).__name__))
     d = numpy.frombuffer(_rt.hot.describe(arrays, _TYPES), _DESCRIPTION)
     if len(d):
         if d['type'].max() >= len(_TYPES):
@@ -298,7 +295,13 @@ def _defines(dtype, nbytes):
 
 def _run(arrays, targets, norm_out, max_norm, eps):
     src = _describe(arrays, 'arrays')
-    dst = src if targets is None else _describe(targets, 'out')
+    dst = src
+    if targets is not None:
+        dst = _describe(targets, 'out')
+        i = _rt.hot.unlike(arrays, targets)
+        if i >= 0:
+            raise ValueError('out[%d] has the shape %r and type %s, expected %r %s' % (
+                i, targets[i]._shape, targets[i].dtype, arrays[i]._shape, arrays[i].dtype))
     dtype = _TYPES[2] if (src['type'] == 2).any() else _TYPES[1]
     if norm_out is None:
         norm_out = ndarray((), dtype)
@@ -394,11 +397,6 @@ def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
         out = _as_list(out, 'out')
         if len(out) != len(arrays):
             raise ValueError('out holds %d arrays, expected %d' % (len(out), len(arrays)))
-        for i, (a, b) in enumerate(zip(arrays, out)):
-            if isinstance(a, ndarray) and isinstance(b, ndarray) and (
-                    a._shape != b._shape or a.dtype != b.dtype):
-                raise ValueError('out[%d] has the shape %r and type %s, expected %r %s'
-                                 % (i, b._shape, b.dtype, a._shape, a.dtype))
     return _run(arrays, out, norm_out, max_norm, eps)
 
 

@@ -11,6 +11,7 @@ import struct
 
 import numpy
 
+from cupy_amd import _dryrun
 from cupy_amd import _rt
 from cupy_amd._core import _launch_plan
 from cupy_amd._core import _tuning
@@ -150,31 +151,30 @@ class Ref:
 
 # -- replay ---------------------------------------------------------------------------
 
-class _Plan:
-    __slots__ = ('fast', 'spans')
-
-    def __init__(self, fast, spans):
-        self.fast = fast
-        self.spans = spans
-
-
 _NOTHING = object()
+_call = _rt.hot.call
 
 
 def replay(plans, arrays, extra):
     """``(result, key)``: the result of a recorded call replayed on ``arrays``
     (``_NOTHING`` if there is none, the call has to be made in full), and the
-    key to record it under (None: not to be recorded)."""
-    key = _launch_plan.call_signature(arrays, _device.get_device_id())
-    if key is None:
+    key to record it under (None: not to be recorded).
+
+    A plan is ``(spans, record, ret, fast)``: which arrays may not overlap, the
+    launches if addresses are all that changes in them and nothing is allocated
+    (made again by the extension module without a way back here), the
+    positions of the results, and the recorded call."""
+    r = _call(plans, arrays, _device.get_device_id(), _tuning._version, extra,
+              _stream.get_current_stream_ptr())
+    if type(r) is list:
+        if len(r) == 1:
+            return _NOTHING, r[0]
+        return r[1][3].run(arrays), r[0]
+    if r is None:
         return _NOTHING, None
-    key += extra
-    plan = plans.get(key)
-    if plan is None:
-        return _NOTHING, key
-    if plan.spans is not None and _rt.hot.overlap(arrays, plan.spans):
-        return _NOTHING, None
-    return plan.fast.run(arrays), key
+    if type(r) is int:
+        _rt.check(r)
+    return r, None
 
 
 def _span(a):
@@ -312,7 +312,10 @@ class Call:
         if self.rec is not None and self.rec.launches:
             fast = _launch_plan.FastCall(
                 len(self.user), [(a._shape, a.dtype) for a in self.made], self.rec, ret)
-            _launch_plan.remember(self.plans, self.key, _Plan(fast, self._spans))
+            direct = (not self.made and not self.rec.temps and fast.quick is not None
+                      and ret is not None and not _dryrun.enabled())
+            _launch_plan.remember(self.plans, self.key, (
+                self._spans, fast.quick[0] if direct else None, ret, fast))
         held = self.user + self.made
         if isinstance(ret, tuple):
             return tuple(held[r] for r in ret)

@@ -312,6 +312,52 @@ done:
   return out;
 }
 
+/* The signature of a call's arguments (a tuple or list): device, version, then
+ * per argument what launch decisions may depend on: arrays contribute (dtype,
+ * shape, strides, alignment of the address), scalars their type.  NULL with no
+ * error set when the call must take the full path. */
+static PyObject* signature_of(PyObject* call, PyObject* dev_id, PyObject* version) {
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(call);
+  PyObject* sig = PyTuple_New(n + 2);
+  if (!sig) return NULL;
+  Py_INCREF(dev_id);
+  PyTuple_SET_ITEM(sig, 0, dev_id);
+  Py_INCREF(version);
+  PyTuple_SET_ITEM(sig, 1, version);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* a = PySequence_Fast_GET_ITEM(call, i);
+    PyTypeObject* t = Py_TYPE(a);
+    PyObject* item = NULL;
+    if (t == array_type) {
+      item = array_signature(a, dev_id);
+      if (!item) {
+        Py_DECREF(sig);
+        return NULL;
+      }
+    } else if (t == &PyFloat_Type || t == &PyBool_Type || t == &PyComplex_Type) {
+      item = (PyObject*)t;
+      Py_INCREF(item);
+    } else if (t == &PyLong_Type) {
+      int overflow = 0;
+      (void)PyLong_AsLongLongAndOverflow(a, &overflow);
+      if (overflow) {
+        Py_DECREF(sig);
+        return NULL;
+      }
+      item = (PyObject*)t;
+      Py_INCREF(item);
+    } else if (PyType_IsSubtype(t, generic_type)) {
+      item = (PyObject*)t;
+      Py_INCREF(item);
+    } else {
+      Py_DECREF(sig);
+      return NULL;
+    }
+    PyTuple_SET_ITEM(sig, i + 2, item);
+  }
+  return sig;
+}
+
 /* signature(args: tuple or list, device id, tuning version) -> tuple, or None when the
  * call must take the full path: everything about the arguments that launch
  * decisions may depend on.  Arrays contribute (dtype, shape, strides,
@@ -326,83 +372,40 @@ static PyObject* hp_signature(PyObject* self, PyObject* const* args, Py_ssize_t 
     PyErr_SetString(PyExc_RuntimeError, "signature: setup() has not been called");
     return NULL;
   }
-  PyObject* call = args[0];
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(call);
-  PyObject* sig = PyTuple_New(n + 2);
-  if (!sig) return NULL;
-  Py_INCREF(args[1]);
-  PyTuple_SET_ITEM(sig, 0, args[1]);
-  Py_INCREF(args[2]);
-  PyTuple_SET_ITEM(sig, 1, args[2]);
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    PyObject* a = PySequence_Fast_GET_ITEM(call, i);
-    PyTypeObject* t = Py_TYPE(a);
-    PyObject* item = NULL;
-    if (t == array_type) {
-      item = array_signature(a, args[1]);
-      if (!item) {
-        Py_DECREF(sig);
-        if (PyErr_Occurred()) return NULL;
-        Py_RETURN_NONE;
-      }
-    } else if (t == &PyFloat_Type || t == &PyBool_Type || t == &PyComplex_Type) {
-      item = (PyObject*)t;
-      Py_INCREF(item);
-    } else if (t == &PyLong_Type) {
-      int overflow = 0;
-      (void)PyLong_AsLongLongAndOverflow(a, &overflow);
-      if (overflow) {
-        Py_DECREF(sig);
-        Py_RETURN_NONE;
-      }
-      item = (PyObject*)t;
-      Py_INCREF(item);
-    } else if (PyType_IsSubtype(t, generic_type)) {
-      item = (PyObject*)t;
-      Py_INCREF(item);
-    } else {
-      Py_DECREF(sig);
-      Py_RETURN_NONE;
-    }
-    PyTuple_SET_ITEM(sig, i + 2, item);
-  }
+  PyObject* sig = signature_of(args[0], args[1], args[2]);
+  if (!sig && !PyErr_Occurred()) Py_RETURN_NONE;
   return sig;
 }
 
-/* overlap(arrays: tuple or list, spec: bytes) -> True if any listed pair of
- * arrays shares memory.  spec: u32 n_arrays, u32 n_pairs, per array the lowest
- * and one-past-highest byte it touches relative to its address (i64 each; both
- * 0: it touches nothing), per pair two u32 positions; the top bit of the second
- * says that the pair may start at the very same address (the same memory, laid
- * out alike).  Reads addresses only. */
-static PyObject* hp_overlap(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
-  (void)self;
-  if (nargs != 2 || !(PyTuple_Check(args[0]) || PyList_Check(args[0])) || !PyBytes_Check(args[1])) {
-    PyErr_SetString(PyExc_TypeError, "overlap(arrays: tuple or list, spec: bytes)");
-    return NULL;
-  }
-  const unsigned char* spec = (const unsigned char*)PyBytes_AS_STRING(args[1]);
-  const size_t size = (size_t)PyBytes_GET_SIZE(args[1]);
+
+/* Whether any pair that `spec` lists of the arrays of `call` (a tuple or list)
+ * shares memory; -1 with an error set on failure.  spec: u32 n_arrays, u32
+ * n_pairs, per array the lowest and one-past-highest byte it touches relative to
+ * its address (i64 each; both 0: it touches nothing), per pair two u32
+ * positions; the top bit of the second says that the pair may start at the very
+ * same address (the same memory, laid out alike).  Reads addresses only. */
+static int overlap_of(PyObject* call, PyObject* spec_bytes) {
+  const unsigned char* spec = (const unsigned char*)PyBytes_AS_STRING(spec_bytes);
+  const size_t size = (size_t)PyBytes_GET_SIZE(spec_bytes);
   uint32_t n, pairs;
+  uint64_t stack_at[64];
+  uint64_t* at = stack_at;
+  int found = 0;
   if (size < 8) goto malformed;
   memcpy(&n, spec, 4);
   memcpy(&pairs, spec + 4, 4);
   if (size != 8 + 16 * (size_t)n + 8 * (size_t)pairs ||
-      (Py_ssize_t)n > PySequence_Fast_GET_SIZE(args[0]))
+      (Py_ssize_t)n > PySequence_Fast_GET_SIZE(call))
     goto malformed;
-  uint64_t stack_at[64];
-  uint64_t* at = stack_at;
   if (n > 64) {
     at = (uint64_t*)PyMem_Malloc((size_t)n * 8);
-    if (!at) return PyErr_NoMemory();
-  }
-  int found = 0;
-  for (uint32_t i = 0; i < n; ++i) {
-    if (address_of(PySequence_Fast_GET_ITEM(args[0], i), 1, &at[i]) < 0) {
-      found = -1;
-      break;
+    if (!at) {
+      PyErr_NoMemory();
+      return -1;
     }
   }
+  for (uint32_t i = 0; i < n && found == 0; ++i)
+    if (address_of(PySequence_Fast_GET_ITEM(call, i), 1, &at[i]) < 0) found = -1;
   for (uint32_t k = 0; k < pairs && found == 0; ++k) {
     uint32_t a, b;
     memcpy(&a, spec + 8 + 16 * (size_t)n + 8 * (size_t)k, 4);
@@ -424,12 +427,150 @@ static PyObject* hp_overlap(PyObject* self, PyObject* const* args, Py_ssize_t na
       found = 1;
   }
   if (at != stack_at) PyMem_Free(at);
-  if (found == -1) return NULL;
-  if (found == -2) goto malformed;
-  return PyBool_FromLong(found);
+  if (found != -2) return found;
 malformed:
   PyErr_SetString(PyExc_ValueError, "malformed overlap specification");
-  return NULL;
+  return -1;
+}
+
+/* overlap(arrays: tuple or list, spec: bytes) -> whether a listed pair shares memory */
+static PyObject* hp_overlap(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 2 || !(PyTuple_Check(args[0]) || PyList_Check(args[0])) || !PyBytes_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "overlap(arrays: tuple or list, spec: bytes)");
+    return NULL;
+  }
+  const int found = overlap_of(args[0], args[1]);
+  return found < 0 ? NULL : PyBool_FromLong(found);
+}
+
+/* call(plans: dict, arrays: list, device id, version, extra: tuple, stream): a recorded call of
+ * an operator made again on `arrays`.  `plans` is keyed by the arrays' signature
+ * followed by `extra`; a plan is (overlap spec or None, launch record or None,
+ * position(s) of the results among the arrays, the recorded call).  Returns
+ *   None                the call has to be made in full and not to be recorded;
+ *   [key]               ... and recorded under `key`;
+ *   [key, plan]         the plan has no launch record: the caller replays it;
+ *   an int              the status of a launch that failed;
+ *   else                the result. */
+static PyObject* hp_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 6 || !PyDict_Check(args[0]) || !PyList_Check(args[1]) || !PyTuple_Check(args[4])) {
+    PyErr_SetString(PyExc_TypeError,
+                    "call(plans: dict, arrays: list, device id, version, extra: tuple, stream)");
+    return NULL;
+  }
+  if (!array_type) {
+    PyErr_SetString(PyExc_RuntimeError, "call: setup() has not been called");
+    return NULL;
+  }
+  PyObject* arrays = args[1];
+  uint64_t stream;
+  if (as_u64(args[5], &stream) < 0) return NULL;
+  PyObject* sig = signature_of(arrays, args[2], args[3]);
+  if (!sig) {
+    if (PyErr_Occurred()) return NULL;
+    Py_RETURN_NONE;
+  }
+  PyObject* key = PySequence_Concat(sig, args[4]);
+  Py_DECREF(sig);
+  if (!key) return NULL;
+  PyObject* plan = PyDict_GetItemWithError(args[0], key);
+  PyObject* out = NULL;
+  if (!plan) {
+    if (!PyErr_Occurred()) {
+      out = PyList_New(1);
+      if (out) PyList_SET_ITEM(out, 0, key);
+      else Py_DECREF(key);
+    } else {
+      Py_DECREF(key);
+    }
+    return out;
+  }
+  Py_INCREF(plan);
+  if (!PyTuple_Check(plan) || PyTuple_GET_SIZE(plan) != 4) {
+    PyErr_SetString(PyExc_ValueError, "malformed plan");
+    goto done;
+  }
+  PyObject* spans = PyTuple_GET_ITEM(plan, 0);
+  PyObject* record = PyTuple_GET_ITEM(plan, 1);
+  PyObject* ret = PyTuple_GET_ITEM(plan, 2);
+  if (spans != Py_None) {
+    if (!PyBytes_Check(spans)) {
+      PyErr_SetString(PyExc_ValueError, "malformed plan");
+      goto done;
+    }
+    const int found = overlap_of(arrays, spans);
+    if (found < 0) goto done;
+    if (found) {
+      out = Py_None;
+      Py_INCREF(out);
+      goto done;
+    }
+  }
+  if (!PyBytes_Check(record)) {
+    out = PyList_New(2);
+    if (out) {
+      Py_INCREF(key);
+      Py_INCREF(plan);
+      PyList_SET_ITEM(out, 0, key);
+      PyList_SET_ITEM(out, 1, plan);
+    }
+    goto done;
+  }
+  PyObject* launched = walk_record(record, arrays, (long)PyList_GET_SIZE(arrays), stream, NULL);
+  if (!launched) goto done;
+  if (PyLong_AsLong(launched) != 0) {
+    out = launched;
+    goto done;
+  }
+  Py_DECREF(launched);
+  /* the results: one position, or a tuple of them */
+  const Py_ssize_t count = PyTuple_Check(ret) ? PyTuple_GET_SIZE(ret) : 1;
+  PyObject* results = PyTuple_Check(ret) ? PyTuple_New(count) : NULL;
+  if (PyTuple_Check(ret) && !results) goto done;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const Py_ssize_t at = PyLong_AsSsize_t(results ? PyTuple_GET_ITEM(ret, i) : ret);
+    if (at < 0 || at >= PyList_GET_SIZE(arrays)) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "malformed plan");
+      Py_XDECREF(results);
+      goto done;
+    }
+    PyObject* a = PyList_GET_ITEM(arrays, at);
+    Py_INCREF(a);
+    if (results) PyTuple_SET_ITEM(results, i, a);
+    else out = a;
+  }
+  if (results) out = results;
+done:
+  Py_DECREF(key);
+  Py_DECREF(plan);
+  return out;
+}
+
+/* unlike(a: list of arrays, b: list of arrays) -> first position at which shapes or
+ * types differ, -1 if there is none */
+static PyObject* hp_unlike(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 2 || !PyList_Check(args[0]) || !PyList_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "unlike(a: list, b: list)");
+    return NULL;
+  }
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]) && i < PyList_GET_SIZE(args[1]); ++i) {
+    PyObject* pair[2] = {PyList_GET_ITEM(args[0], i), PyList_GET_ITEM(args[1], i)};
+    int same = 1;
+    PyObject* names[2] = {str_shape, str_dtype};
+    for (int k = 0; k < 2 && same == 1; ++k) {
+      PyObject* a = PyObject_GetAttr(pair[0], names[k]);
+      PyObject* b = a ? PyObject_GetAttr(pair[1], names[k]) : NULL;
+      same = b ? PyObject_RichCompareBool(a, b, Py_EQ) : -1;
+      Py_XDECREF(a);
+      Py_XDECREF(b);
+    }
+    if (same < 0) return NULL;
+    if (same == 0) return PyLong_FromSsize_t(i);
+  }
+  return PyLong_FromLong(-1);
 }
 
 /* describe(arrays: list, types: list of dtypes) -> bytes, per array: u64 address,
@@ -448,6 +589,11 @@ static PyObject* hp_describe(PyObject* self, PyObject* const* args, Py_ssize_t n
   for (Py_ssize_t i = 0; i < n; ++i, to += 32) {
     if (i >= PyList_GET_SIZE(args[0])) break;
     PyObject* a = PyList_GET_ITEM(args[0], i);
+    if (!array_type || !PyObject_TypeCheck(a, array_type)) {
+      PyErr_Format(PyExc_TypeError, "expected cupy.ndarrays, got %.100s", Py_TYPE(a)->tp_name);
+      Py_DECREF(out);
+      return NULL;
+    }
     PyObject *data = NULL, *ptr = NULL, *dev = NULL, *size = NULL, *dtype = NULL;
     PyObject *c_order = NULL, *f_order = NULL;
     int ok = 0;
@@ -498,6 +644,10 @@ static PyObject* hp_describe(PyObject* self, PyObject* const* args, Py_ssize_t n
 }
 
 static PyMethodDef methods[] = {
+    {"call", (PyCFunction)(void (*)(void))hp_call, METH_FASTCALL,
+     "call(plans, arrays, device id, version, extra, stream) -> result of a recorded call made again"},
+    {"unlike", (PyCFunction)(void (*)(void))hp_unlike, METH_FASTCALL,
+     "unlike(a, b) -> first position at which shapes or types differ, or -1"},
     {"describe", (PyCFunction)(void (*)(void))hp_describe, METH_FASTCALL,
      "describe(arrays, types) -> addresses, sizes, types and layouts as bytes"},
     {"overlap", (PyCFunction)(void (*)(void))hp_overlap, METH_FASTCALL,

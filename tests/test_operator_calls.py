@@ -242,8 +242,13 @@ def test_descriptions():
     assert list(d['n']) == [24, 24, 12, 1, 0, 3]
     assert list(d['dense']) == [1, 2, 0, 3, 3, 3]
     assert [int(p) for p in d['ptr']] == [x.data.ptr for x in arrays]
-    with pytest.raises(AttributeError):
+    with pytest.raises(TypeError):
         _rt.hot.describe([None], _global_norm._TYPES)
+    assert _rt.hot.unlike(arrays, arrays) == -1
+    assert _rt.hot.unlike([a, a], [arr((6, 4), 'float16'), a.T]) == 1
+    assert _rt.hot.unlike([a, a], [arr((6, 4)), a]) == 0
+    with pytest.raises(AttributeError):
+        _rt.hot.unlike([a], [3])
     with pytest.raises(TypeError):
         _rt.hot.describe(arrays, 3)
 
@@ -373,3 +378,43 @@ def test_options_that_compare_equal_are_not_mixed_up():
                           out=cp.TokenLogProb(arr(4), arr(4), None, arr(4), None))
     with pytest.raises(TypeError):
         cp.token_log_prob(x, t, out=(arr(4), arr(4), None, None, None))
+
+
+def test_recorded_calls_made_by_the_extension():
+    """hot.call without a launch: records of no launches."""
+    a, b, c = arr((4, 8)), arr((4, 8)), arr(3)
+    nothing = struct.pack('<II', 0, 0)
+    plans = {}
+
+    def call(arrays, extra=(1,), table=None):
+        return _rt.hot.call(plans if table is None else table, arrays, 0, 0, extra, 0)
+    miss = call([a, b])
+    assert type(miss) is list and len(miss) == 1
+    key = miss[0]
+    plans[key] = (None, nothing, 1, None)
+    assert call([a, b]) is b and call([b, a]) is a
+    plans[key] = (None, nothing, (1, 0), None)
+    assert call([a, b])[0] is b
+    assert call([a, b])[1] is a
+    assert type(call([a, b], (2,))) is list and type(call([a, c])) is list
+    plans[key] = (None, None, 0, 'recorded')
+    found = call([a, b])
+    assert found[0] == key and found[1][3] == 'recorded'
+    plans[key] = (_op_calls._pack_spans([a, b], [(0, 1, False)]), nothing, 0, None)
+    assert call([a, b]) is a
+    assert call([a, a]) is None                 # the pair overlaps
+    assert call([a, 'x']) is None               # of no signature
+    plans[key] = (_op_calls._pack_spans([a, b], [(0, 1, True)]), nothing, 0, None)
+    assert call([a, a]) is a
+    for bad in (3, (None, nothing, 0), (3, nothing, 0, None), (None, nothing, 2, None),
+                (None, nothing, -1, None), (None, nothing, (0, 5), None), (None, b'1', 0, None),
+                (b'1234', nothing, 0, None)):
+        plans[key] = bad
+        with pytest.raises(ValueError):
+            call([a, b])
+    with pytest.raises(TypeError):
+        _rt.hot.call([], [a], 0, 0, (), 0)
+    with pytest.raises(TypeError):
+        _rt.hot.call({}, [a], 0, 0, ([],), 0)       # a key that cannot be looked up
+    with pytest.raises(TypeError):
+        _rt.hot.call({}, [a], 0, 0, ())

@@ -235,32 +235,38 @@ def _hit_by(src, dst):
     return numpy.flatnonzero(last - first > own)
 
 
-def _tables(src, dst):
-    """[(dtype, [(table, arrays in it, workgroups)], bytes)] per type."""
-    found = []
-    for code, dtype in enumerate(_TYPES):
-        at = numpy.flatnonzero((src['type'] == code) & (src['n'] > 0))
-        if not len(at):
-            continue
-        item = dtype.itemsize
-        ptr, n = src['ptr'][at], src['n'][at]
-        phase = (ptr.astype(numpy.int64) & 15) // item
-        per = 16 // item * _BLOCK * _UNROLL
-        blocks = (phase + n.astype(numpy.int64) + (per - 1)) // per
-        table = numpy.zeros(-(-len(at) // _MAX) * _MAX, _ENTRY)
-        table['src'][:len(at)] = ptr
-        table['dst'][:len(at)] = dst['ptr'][at]
-        table['n'][:len(at)] = n
-        launches = []
-        for lo in range(0, len(at), _MAX):
-            these = blocks[lo:lo + _MAX]
-            ends = numpy.cumsum(these)
-            if int(ends[-1]) > 0xffffffff // _BLOCK:
-                raise ValueError('more than 2**39 bytes of arrays in one launch')
-            table['first'][lo:lo + len(these)] = ends - these
-            launches.append((table[lo:lo + _MAX].tobytes(), len(these), int(ends[-1])))
-        found.append((dtype, launches, int(n.sum()) * item))
-    return found
+def _prepare(arrays, targets, write):
+    """Arrays the kernels cannot take as they are: refused, or replaced by
+    copies.  Returns (arrays to read, arrays to write, positions of those made
+    beside their target)."""
+    src = _describe(arrays, 'arrays')
+    if not write:
+        return [a if d else a.copy('C') for a, d in zip(arrays, src['dense'])], None, ()
+    finals, dst = arrays, src
+    if targets is not None:
+        finals, dst = targets, _describe(targets, 'out')
+        for i, (a, b) in enumerate(zip(arrays, targets)):
+            if a._shape != b._shape or a.dtype != b.dtype:
+                raise ValueError('out[%d] has the shape %r and type %s, expected %r %s'
+                                 % (i, b._shape, b.dtype, a._shape, a.dtype))
+    ranges = _ranges(finals, dst)
+    _check_apart(*ranges)
+    reads, writes = list(arrays), list(finals)
+    if targets is not None:
+        for i in _hit_by(_ranges(arrays, src), ranges):
+            reads[i] = arrays[i].copy('K')
+    # an array and its result are walked in the order they are stored in: where
+    # these differ, or are no order at all, the result is made aside
+    aside = numpy.flatnonzero((src['dense'] & dst['dense']) == 0)
+    for i in aside:
+        reads[i] = arrays[i].copy('C')
+        writes[i] = ndarray(arrays[i]._shape, arrays[i].dtype)
+    return reads, writes, aside
+
+
+def _tables(arrays, targets, write, beside=None):
+    return _rt.hot.tables(arrays, targets, _TYPES, _MAX, _BLOCK * _UNROLL,
+                          _device.get_device_id(), write, beside)
 
 
 class _Temporary:
@@ -294,65 +300,50 @@ def _defines(dtype, nbytes):
 
 
 def _run(arrays, targets, norm_out, max_norm, eps):
-    src = _describe(arrays, 'arrays')
-    dst = src
-    if targets is not None:
-        dst = _describe(targets, 'out')
-        i = _rt.hot.unlike(arrays, targets)
-        if i >= 0:
-            raise ValueError('out[%d] has the shape %r and type %s, expected %r %s' % (
-                i, targets[i]._shape, targets[i].dtype, arrays[i]._shape, arrays[i].dtype))
-    dtype = _TYPES[2] if (src['type'] == 2).any() else _TYPES[1]
+    write = max_norm is not None
+    finals, aside = arrays if targets is None else targets, ()
+    tables = _tables(arrays, targets, write, norm_out)
+    if tables is None:
+        if write and norm_out is not None:
+            _check_beside(norm_out, finals)
+        arrays, targets, aside = _prepare(arrays, targets, write)
+        tables = _tables(arrays, targets, write)
+    dtype = _TYPES[2 if tables and tables[-1][0] == 2 else 1]
     if norm_out is None:
         norm_out = ndarray((), dtype)
     else:
         _oc.check_out(norm_out, (), dtype, 'norm_out')
-    reads, writes, aside = arrays, arrays, ()
-    if max_norm is None:
-        if (src['dense'] == 0).any():
-            reads = writes = [a if d else a.copy('C') for a, d in zip(arrays, src['dense'])]
-            src = dst = _describe(reads, 'arrays')
-    else:
-        finals = arrays if targets is None else targets
-        ranges = _ranges(finals, dst)
-        _check_apart(*ranges)
-        at = norm_out.data.ptr
-        if ((ranges[0] < at + dtype.itemsize) & (at < ranges[1])).any():
-            raise ValueError('norm_out overlaps an array to write')
-        hit = ()
-        if targets is not None:
-            hit = _hit_by(_ranges(arrays, src), ranges)
-        # an array and its result are walked in the order they are stored in:
-        # where these differ, or are no order at all, the result is made aside
-        aside = numpy.flatnonzero((src['dense'] & dst['dense']) == 0)
-        if len(hit) or len(aside):
-            reads, writes = list(arrays), list(finals)
-            for i in hit:
-                reads[i] = arrays[i].copy('K')
-            for i in aside:
-                reads[i] = arrays[i].copy('C')
-                writes[i] = ndarray(arrays[i]._shape, arrays[i].dtype)
-            src, dst = _describe(reads, 'arrays'), _describe(writes, 'out')
-    tables = _tables(src, dst)
     total = sum(blocks for _, launches, _ in tables for _, _, blocks in launches)
     temp = _Temporary(total + 1)              # the factor, then the sums
     at = 1
     for t, launches, nbytes in tables:
-        fn = _SOURCE.function('cupy_square_sums', **_defines(t, nbytes))
+        if not launches:
+            continue
+        fn = _SOURCE.function('cupy_square_sums', **_defines(_TYPES[t], nbytes))
         for table, n, blocks in launches:
             temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, 0), struct.pack('<q', at))
             at += blocks
     fn = _FINISH.function('cupy_norm_of_sums', N_T=dtype)
     temp.launch(fn, 1, 1024, b'', struct.pack('<qQdd', total, norm_out.data.ptr,
-                                              0.0 if max_norm is None else max_norm, eps))
-    if max_norm is not None:
+                                              max_norm if write else 0.0, eps))
+    if write:
         for t, launches, nbytes in reversed(tables):
-            fn = _SOURCE.function('cupy_scale_arrays', **_defines(t, nbytes))
+            if not launches:
+                continue
+            fn = _SOURCE.function('cupy_scale_arrays', **_defines(_TYPES[t], nbytes))
             for table, n, blocks in reversed(launches):
                 temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, blocks))
         for i in aside:
-            elementwise_copy(writes[i], finals[i])
+            elementwise_copy(targets[i], finals[i])
     return norm_out
+
+
+def _check_beside(norm_out, arrays):
+    _oc.check_array(norm_out, 'norm_out')
+    for a in arrays:
+        _oc.check_array(a, 'arrays')
+        if _rt.hot.overlap([a, norm_out], _oc._pack_spans([a, norm_out], [(0, 1, False)])):
+            raise ValueError('norm_out overlaps an array to write')
 
 
 def global_norm(arrays, *, norm_out=None):

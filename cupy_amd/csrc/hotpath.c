@@ -15,6 +15,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include "mi355rt.h"
@@ -26,6 +27,7 @@ static PyObject* str_shape;
 static PyObject* str_strides;
 static PyObject* str_device_id;
 static PyObject* str_size;
+static PyObject* str_itemsize;
 static PyObject* str_c_contiguous;
 static PyObject* str_f_contiguous;
 static PyTypeObject* array_type;      /* the package's ndarray, set by setup() */
@@ -548,29 +550,256 @@ done:
   return out;
 }
 
-/* unlike(a: list of arrays, b: list of arrays) -> first position at which shapes or
- * types differ, -1 if there is none */
-static PyObject* hp_unlike(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+/* -- tables of arrays for the kernels that take many arrays in one launch ---------- */
+
+typedef struct {
+  uint64_t start, bytes;       /* its memory, for an array stored in one piece */
+  uint64_t elements;
+  uint32_t type, dense;        /* position in `types`; 1 C order | 2 Fortran order */
+  int64_t device;
+} Description;
+
+/* What `a` is; 0, or -1 with an error set.  `item` are the sizes of the types. */
+static int describe_one(PyObject* a, PyObject* types, const uint64_t* item, Description* d) {
+  if (!array_type || !PyObject_TypeCheck(a, array_type)) {
+    PyErr_Format(PyExc_TypeError, "expected cupy.ndarrays, got %.100s", Py_TYPE(a)->tp_name);
+    return -1;
+  }
+  PyObject *data = NULL, *ptr = NULL, *dev = NULL, *size = NULL, *dtype = NULL;
+  PyObject *c_order = NULL, *f_order = NULL;
+  int rc = -1;
+  data = PyObject_GetAttr(a, str_data);
+  if (data) {
+    ptr = PyObject_GetAttr(data, str_ptr);
+    dev = PyObject_GetAttr(data, str_device_id);
+  }
+  size = PyObject_GetAttr(a, str_size);
+  dtype = PyObject_GetAttr(a, str_dtype);
+  c_order = PyObject_GetAttr(a, str_c_contiguous);
+  f_order = PyObject_GetAttr(a, str_f_contiguous);
+  if (ptr && dev && size && dtype && c_order && f_order && as_u64(ptr, &d->start) == 0 &&
+      as_u64(size, &d->elements) == 0) {
+    const Py_ssize_t n_types = PyList_GET_SIZE(types);
+    uint32_t type = 0;
+    for (; (Py_ssize_t)type < n_types; ++type)
+      if (PyObject_RichCompareBool(dtype, PyList_GET_ITEM(types, type), Py_EQ) != 0) break;
+    const int c = PyObject_IsTrue(c_order), f = PyObject_IsTrue(f_order);
+    d->device = (int64_t)PyLong_AsLongLong(dev);
+    if (!PyErr_Occurred()) {
+      d->type = type;
+      d->dense = (c ? 1u : 0u) | (f ? 2u : 0u);
+      d->bytes = (Py_ssize_t)type < n_types ? d->elements * item[type] : 0;
+      rc = 0;
+    }
+  }
+  Py_XDECREF(data);
+  Py_XDECREF(ptr);
+  Py_XDECREF(dev);
+  Py_XDECREF(size);
+  Py_XDECREF(dtype);
+  Py_XDECREF(c_order);
+  Py_XDECREF(f_order);
+  return rc;
+}
+
+#define MAX_TYPES 8
+
+/* The sizes of the elements of `types`; -1 with an error set on failure. */
+static int item_sizes(PyObject* types, uint64_t* item) {
+  const Py_ssize_t n = PyList_GET_SIZE(types);
+  if (n > MAX_TYPES) {
+    PyErr_SetString(PyExc_ValueError, "too many types");
+    return -1;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyObject_GetAttr(PyList_GET_ITEM(types, i), str_itemsize);
+    const int rc = o ? as_u64(o, &item[i]) : -1;
+    Py_XDECREF(o);
+    if (rc < 0) return -1;
+    if (item[i] == 0 || item[i] > 16) {
+      PyErr_SetString(PyExc_ValueError, "unsupported type");
+      return -1;
+    }
+  }
+  return 0;
+}
+
+static int by_start(const void* a, const void* b) {
+  const Description *x = *(const Description* const*)a, *y = *(const Description* const*)b;
+  return x->start < y->start ? -1 : x->start > y->start;
+}
+
+/* 1 if no two of the n outputs share memory and no input shares memory with an
+ * output other than its own, whose very memory it may be.  `sorted`: room for n. */
+static int are_apart(const Description* src, const Description* dst, Py_ssize_t n,
+                     const Description** sorted) {
+  Py_ssize_t m = 0;
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (dst[i].bytes) sorted[m++] = &dst[i];
+  qsort(sorted, (size_t)m, sizeof(*sorted), by_start);
+  for (Py_ssize_t k = 1; k < m; ++k)
+    if (sorted[k]->start < sorted[k - 1]->start + sorted[k - 1]->bytes) return 0;
+  if (src == dst) return 1;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!src[i].bytes) continue;
+    const uint64_t lo = src[i].start, hi = lo + src[i].bytes;
+    Py_ssize_t a = 0, b = m;               /* the first output that ends behind `lo` */
+    while (a < b) {
+      const Py_ssize_t mid = (a + b) / 2;
+      if (sorted[mid]->start + sorted[mid]->bytes > lo) b = mid;
+      else a = mid + 1;
+    }
+    for (; a < m && sorted[a]->start < hi; ++a)
+      if (sorted[a] != &dst[i] || dst[i].start != lo) return 0;
+  }
+  return 1;
+}
+
+typedef struct {
+  uint64_t src, dst, n;
+  uint32_t first, pad;
+} TableEntry;
+
+/* tables(arrays: list, targets: list or None, types: list of dtypes, entries,
+ * vectors, device id, write, beside) -> per type met (position of the type, [(table,
+ * arrays in it, workgroups)], bytes), or None for arrays that need preparation: of
+ * another type or device, not stored in one piece in the order of their targets
+ * (None: themselves), of other shapes or types than these, or (with `write`)
+ * sharing memory where it is written, with each other or with the array `beside`
+ * (if not None).  A table holds `entries` TableEntry, zeros
+ * behind the last; a workgroup takes `vectors` vectors of 16 bytes that start on
+ * 16-byte borders of the source.  Empty arrays are left out. */
+static PyObject* hp_tables(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   (void)self;
-  if (nargs != 2 || !PyList_Check(args[0]) || !PyList_Check(args[1])) {
-    PyErr_SetString(PyExc_TypeError, "unlike(a: list, b: list)");
+  if (nargs != 8 || !PyList_Check(args[0]) || !(args[1] == Py_None || PyList_Check(args[1])) ||
+      !PyList_Check(args[2])) {
+    PyErr_SetString(PyExc_TypeError,
+                    "tables(arrays: list, targets: list or None, types: list, entries, vectors, "
+                    "device id, write, beside)");
     return NULL;
   }
-  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]) && i < PyList_GET_SIZE(args[1]); ++i) {
-    PyObject* pair[2] = {PyList_GET_ITEM(args[0], i), PyList_GET_ITEM(args[1], i)};
-    int same = 1;
-    PyObject* names[2] = {str_shape, str_dtype};
-    for (int k = 0; k < 2 && same == 1; ++k) {
-      PyObject* a = PyObject_GetAttr(pair[0], names[k]);
-      PyObject* b = a ? PyObject_GetAttr(pair[1], names[k]) : NULL;
-      same = b ? PyObject_RichCompareBool(a, b, Py_EQ) : -1;
-      Py_XDECREF(a);
-      Py_XDECREF(b);
-    }
-    if (same < 0) return NULL;
-    if (same == 0) return PyLong_FromSsize_t(i);
+  uint64_t item[MAX_TYPES], entries, vectors;
+  if (item_sizes(args[2], item) < 0) return NULL;
+  if (as_u64(args[3], &entries) < 0 || as_u64(args[4], &vectors) < 0) return NULL;
+  const long long device = PyLong_AsLongLong(args[5]);
+  if (device == -1 && PyErr_Occurred()) return NULL;
+  const int write = PyObject_IsTrue(args[6]);
+  if (write < 0) return NULL;
+  if (entries == 0 || entries > 4096 || vectors == 0 || vectors > (1u << 24)) {
+    PyErr_SetString(PyExc_ValueError, "tables: entries or vectors out of range");
+    return NULL;
   }
-  return PyLong_FromLong(-1);
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  const Py_ssize_t n_types = PyList_GET_SIZE(args[2]);
+  const int own = args[1] == Py_None;
+  if (!own && PyList_GET_SIZE(args[1]) != n) {
+    PyErr_SetString(PyExc_ValueError, "tables: as many targets as arrays are expected");
+    return NULL;
+  }
+  PyObject* result = NULL;
+  TableEntry* table = NULL;
+  Description* src = PyMem_New(Description, (size_t)(2 * n + 1));
+  const Description** sorted = PyMem_New(const Description*, (size_t)(n + 1));
+  Description* dst = own || !src ? src : src + n;
+  if (!src || !sorted) {
+    PyErr_NoMemory();
+    goto done;
+  }
+  int plain = 1;
+  for (Py_ssize_t i = 0; i < n && plain; ++i) {
+    if (i >= PyList_GET_SIZE(args[0]) || (!own && i >= PyList_GET_SIZE(args[1]))) {
+      PyErr_SetString(PyExc_RuntimeError, "tables: a list changed on the way");
+      goto done;
+    }
+    PyObject* a = PyList_GET_ITEM(args[0], i);
+    if (describe_one(a, args[2], item, &src[i]) < 0) goto done;
+    if (!own) {
+      PyObject* b = PyList_GET_ITEM(args[1], i);
+      if (describe_one(b, args[2], item, &dst[i]) < 0) goto done;
+      PyObject* sa = PyObject_GetAttr(a, str_shape);
+      PyObject* sb = sa ? PyObject_GetAttr(b, str_shape) : NULL;
+      const int same = sb ? PyObject_RichCompareBool(sa, sb, Py_EQ) : -1;
+      Py_XDECREF(sa);
+      Py_XDECREF(sb);
+      if (same < 0) goto done;
+      if (!same || src[i].type != dst[i].type || dst[i].device != device) plain = 0;
+    }
+    if ((Py_ssize_t)src[i].type >= n_types || src[i].device != device ||
+        !(src[i].dense & dst[i].dense))
+      plain = 0;
+  }
+  if (plain && write && args[7] != Py_None) {
+    Description one;
+    if (describe_one(args[7], args[2], item, &one) < 0) goto done;
+    /* (a type that is not listed: as if it were one of 16 bytes) */
+    const uint64_t bytes = one.bytes ? one.bytes : one.elements * 16;
+    if (!one.dense) plain = 0;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (dst[i].start < one.start + bytes && one.start < dst[i].start + dst[i].bytes) plain = 0;
+  }
+  if (!plain || (write && !are_apart(src, dst, n, sorted))) {
+    result = Py_None;
+    Py_INCREF(result);
+    goto done;
+  }
+  table = PyMem_New(TableEntry, (size_t)entries);
+  if (!table) {
+    PyErr_NoMemory();
+    goto done;
+  }
+  result = PyList_New(0);
+  for (Py_ssize_t t = 0; result && t < n_types; ++t) {
+    PyObject* launches = NULL;           /* (empty where all arrays of a type are) */
+    uint64_t used = 0, blocks = 0, bytes = 0;
+    int failed = 0;
+    for (Py_ssize_t i = 0; i <= n && !failed; ++i) {
+      const int last = i == n;
+      if (!last && (Py_ssize_t)src[i].type != t) continue;
+      if (!last && !launches && !(launches = PyList_New(0))) {
+        failed = 1;
+        break;
+      }
+      if (!last && src[i].elements == 0) continue;
+      if (used && (last || used == entries)) {
+        /* (the kernels count workgroups of 256 threads in 32 bits) */
+        if (blocks > 0xffffffffull / 256) {
+          PyErr_SetString(PyExc_ValueError, "more than 2**39 bytes of arrays in one launch");
+          failed = 1;
+          break;
+        }
+        memset(table + used, 0, (size_t)(entries - used) * sizeof(TableEntry));
+        PyObject* one = Py_BuildValue("y#KK", (const char*)table,
+                                      (Py_ssize_t)(entries * sizeof(TableEntry)),
+                                      (unsigned long long)used, (unsigned long long)blocks);
+        if (!one || PyList_Append(launches, one) < 0) failed = 1;
+        Py_XDECREF(one);
+        used = blocks = 0;
+      }
+      if (last || failed) break;
+      const uint64_t per = 16 / item[t] * vectors;
+      const uint64_t count = ((src[i].start & 15) / item[t] + src[i].elements + per - 1) / per;
+      TableEntry* e = &table[used++];
+      e->src = src[i].start;
+      e->dst = dst[i].start;
+      e->n = src[i].elements;
+      e->first = (uint32_t)blocks;
+      e->pad = 0;
+      blocks += count;
+      bytes += src[i].bytes;
+    }
+    if (!failed && launches) {
+      PyObject* one = Py_BuildValue("nOK", t, launches, (unsigned long long)bytes);
+      if (!one || PyList_Append(result, one) < 0) failed = 1;
+      Py_XDECREF(one);
+    }
+    Py_XDECREF(launches);
+    if (failed) Py_CLEAR(result);
+  }
+done:
+  PyMem_Free(table);
+  PyMem_Free((void*)sorted);
+  PyMem_Free(src);
+  return result;
 }
 
 /* describe(arrays: list, types: list of dtypes) -> bytes, per array: u64 address,
@@ -582,63 +811,24 @@ static PyObject* hp_describe(PyObject* self, PyObject* const* args, Py_ssize_t n
     PyErr_SetString(PyExc_TypeError, "describe(arrays: list, types: list)");
     return NULL;
   }
+  uint64_t item[MAX_TYPES];
+  if (item_sizes(args[1], item) < 0) return NULL;
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
   PyObject* out = PyBytes_FromStringAndSize(NULL, n * 32);
   if (!out) return NULL;
   unsigned char* to = (unsigned char*)PyBytes_AS_STRING(out);
-  for (Py_ssize_t i = 0; i < n; ++i, to += 32) {
-    if (i >= PyList_GET_SIZE(args[0])) break;
-    PyObject* a = PyList_GET_ITEM(args[0], i);
-    if (!array_type || !PyObject_TypeCheck(a, array_type)) {
-      PyErr_Format(PyExc_TypeError, "expected cupy.ndarrays, got %.100s", Py_TYPE(a)->tp_name);
+  memset(to, 0, (size_t)n * 32);
+  for (Py_ssize_t i = 0; i < n && i < PyList_GET_SIZE(args[0]); ++i, to += 32) {
+    Description d;
+    if (describe_one(PyList_GET_ITEM(args[0], i), args[1], item, &d) < 0) {
       Py_DECREF(out);
       return NULL;
     }
-    PyObject *data = NULL, *ptr = NULL, *dev = NULL, *size = NULL, *dtype = NULL;
-    PyObject *c_order = NULL, *f_order = NULL;
-    int ok = 0;
-    uint64_t address, elements;
-    data = PyObject_GetAttr(a, str_data);
-    if (data) {
-      ptr = PyObject_GetAttr(data, str_ptr);
-      dev = PyObject_GetAttr(data, str_device_id);
-    }
-    size = PyObject_GetAttr(a, str_size);
-    dtype = PyObject_GetAttr(a, str_dtype);
-    c_order = PyObject_GetAttr(a, str_c_contiguous);
-    f_order = PyObject_GetAttr(a, str_f_contiguous);
-    if (ptr && dev && size && dtype && c_order && f_order && as_u64(ptr, &address) == 0 &&
-        as_u64(size, &elements) == 0) {
-      uint32_t type = 0;
-      const Py_ssize_t n_types = PyList_GET_SIZE(args[1]);
-      for (; (Py_ssize_t)type < n_types; ++type) {
-        const int same = PyObject_RichCompareBool(dtype, PyList_GET_ITEM(args[1], type), Py_EQ);
-        if (same != 0) break;          /* the same, or an error */
-      }
-      const int c = PyObject_IsTrue(c_order), f = PyObject_IsTrue(f_order);
-      const int64_t device = (int64_t)PyLong_AsLongLong(dev);
-      if (!PyErr_Occurred()) {
-        const uint32_t dense = (c ? 1u : 0u) | (f ? 2u : 0u);
-        memcpy(to, &address, 8);
-        memcpy(to + 8, &elements, 8);
-        memcpy(to + 16, &type, 4);
-        memcpy(to + 20, &dense, 4);
-        memcpy(to + 24, &device, 8);
-        ok = 1;
-      }
-    }
-    Py_XDECREF(data);
-    Py_XDECREF(ptr);
-    Py_XDECREF(dev);
-    Py_XDECREF(size);
-    Py_XDECREF(dtype);
-    Py_XDECREF(c_order);
-    Py_XDECREF(f_order);
-    if (!ok) {
-      Py_DECREF(out);
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "describe: no array");
-      return NULL;
-    }
+    memcpy(to, &d.start, 8);
+    memcpy(to + 8, &d.elements, 8);
+    memcpy(to + 16, &d.type, 4);
+    memcpy(to + 20, &d.dense, 4);
+    memcpy(to + 24, &d.device, 8);
   }
   return out;
 }
@@ -646,8 +836,8 @@ static PyObject* hp_describe(PyObject* self, PyObject* const* args, Py_ssize_t n
 static PyMethodDef methods[] = {
     {"call", (PyCFunction)(void (*)(void))hp_call, METH_FASTCALL,
      "call(plans, arrays, device id, version, extra, stream) -> result of a recorded call made again"},
-    {"unlike", (PyCFunction)(void (*)(void))hp_unlike, METH_FASTCALL,
-     "unlike(a, b) -> first position at which shapes or types differ, or -1"},
+    {"tables", (PyCFunction)(void (*)(void))hp_tables, METH_FASTCALL,
+     "tables(arrays, targets, types, entries, vectors, device id, write, beside) -> tables or None"},
     {"describe", (PyCFunction)(void (*)(void))hp_describe, METH_FASTCALL,
      "describe(arrays, types) -> addresses, sizes, types and layouts as bytes"},
     {"overlap", (PyCFunction)(void (*)(void))hp_overlap, METH_FASTCALL,
@@ -681,10 +871,11 @@ PyMODINIT_FUNC PyInit__hotpath(void) {
   str_strides = PyUnicode_InternFromString("_strides");
   str_device_id = PyUnicode_InternFromString("device_id");
   str_size = PyUnicode_InternFromString("size");
+  str_itemsize = PyUnicode_InternFromString("itemsize");
   str_c_contiguous = PyUnicode_InternFromString("_c_contiguous");
   str_f_contiguous = PyUnicode_InternFromString("_f_contiguous");
   if (!str_data || !str_ptr || !str_dtype || !str_shape || !str_strides || !str_device_id ||
-      !str_size || !str_c_contiguous || !str_f_contiguous)
+      !str_size || !str_itemsize || !str_c_contiguous || !str_f_contiguous)
     return NULL;
   return PyModule_Create(&module);
 }

@@ -188,6 +188,11 @@ def test_global_norm_refuses():
     with pytest.raises(ValueError):
         cp.clip_by_global_norm([flat], 1.0, norm_out=flat[3:4].reshape(()))
     cp.global_norm([x, x])       # read twice is no harm
+    with pytest.raises(TypeError):
+        cp.clip_by_global_norm([x], 1.0, norm_out=3)
+    with pytest.raises(TypeError):
+        cp.clip_by_global_norm([x], 1.0, norm_out=arr((), 'int32'))
+    assert cp.global_norm([x, arr(0, 'float64')]).dtype == 'float64'
 
 
 # -- rows, overlap, descriptions ----------------------------------------------------------
@@ -244,11 +249,6 @@ def test_descriptions():
     assert [int(p) for p in d['ptr']] == [x.data.ptr for x in arrays]
     with pytest.raises(TypeError):
         _rt.hot.describe([None], _global_norm._TYPES)
-    assert _rt.hot.unlike(arrays, arrays) == -1
-    assert _rt.hot.unlike([a, a], [arr((6, 4), 'float16'), a.T]) == 1
-    assert _rt.hot.unlike([a, a], [arr((6, 4)), a]) == 0
-    with pytest.raises(AttributeError):
-        _rt.hot.unlike([a], [3])
     with pytest.raises(TypeError):
         _rt.hot.describe(arrays, 3)
 
@@ -261,9 +261,8 @@ def test_tables_cover_every_array(item, dtype):
     flat = arr(1 << 20, dtype)
     cuts = np.sort(rng.integers(0, 1 << 20, 500))
     arrays = [flat[a:b] for a, b in zip(cuts[:-1], cuts[1:])]
-    d = _global_norm._describe(arrays, 'arrays')
-    (found, launches, nbytes), = _global_norm._tables(d, d)
-    assert found == np.dtype(dtype) and nbytes == (cuts[-1] - cuts[0]) * item
+    (found, launches, nbytes), = _global_norm._tables(arrays, None, True)
+    assert _global_norm._TYPES[found] == np.dtype(dtype) and nbytes == (cuts[-1] - cuts[0]) * item
     per = 16 // item * 256 * 8
     seen = 0
     for table, n, blocks in launches:
@@ -418,3 +417,33 @@ def test_recorded_calls_made_by_the_extension():
         _rt.hot.call({}, [a], 0, 0, ([],), 0)       # a key that cannot be looked up
     with pytest.raises(TypeError):
         _rt.hot.call({}, [a], 0, 0, ())
+
+
+def test_tables_of_what_needs_preparation():
+    def tables(arrays, targets=None, write=True):
+        return _global_norm._tables(arrays, targets, write)
+    a, b = arr((6, 4)), arr((6, 4))
+    assert tables([a, b]) and tables([a], [b]) and tables([a, b], [a, b]) and tables([a, a], None, False)
+    assert tables([]) == []
+    assert tables([arr((0, 3)), arr(0, 'float64')]) == [(1, [], 0), (2, [], 0)]
+    assert _global_norm._tables([a], None, True, b[2, 2]) and not _global_norm._tables([a], None, True, a[2, 2])
+    assert _global_norm._tables([a], None, False, a[2, 2])
+    assert tables([a.T], [arr((6, 4)).T]) and tables([arr((0, 3)), a], [arr((0, 3)), b])
+    for case in (([a, a],), ([a, b], [b, a]), ([a], [a.T]), ([a], [b.T.reshape(6, 4)[::1, ::-1]]),
+                 ([a[:, ::2]],), ([a], [arr((4, 6))]), ([a], [arr((6, 4), 'float16')]),
+                 ([arr(3, 'int32')],), ([a[:4], a[2:]],), ([a[:3], b[:3]], [a[2:5], b[3:]]),
+                 ([a[:3], b[:3]], [b[:3], a[:3]])):
+        assert tables(*case) is None
+    # the same pieces shifted by one: each input is another array's output
+    flat = arr(100)
+    assert tables([flat[10:20], flat[20:30]], [flat[20:30], flat[10:20]]) is None
+    assert tables([flat[10:20], flat[20:30]], [flat[30:40], flat[40:50]])
+    mixed = tables([arr(5, 'float64'), arr(70000, 'float16'), a, arr(3, 'float16')])
+    assert [t for t, _, _ in mixed] == [0, 1, 2] and [n for _, l, _ in mixed for _, n, _ in l] == [2, 1, 1]
+    with pytest.raises(TypeError):
+        tables([3])
+    with pytest.raises(ValueError):
+        tables([a], [])
+    for bad in ((0, 5), (5, 0), (5000, 5)):
+        with pytest.raises(ValueError):
+            _rt.hot.tables([a], None, _global_norm._TYPES, *bad, 0, True, None)

@@ -534,8 +534,9 @@ _GRAD = _oc.Source(_COMMON + r'''
 _CUPY_DEV X_T gradient(X_T logit, A norm, A gain, A gh, A h, bool hit, bool empty) {
   const A lp = static_cast<A>(logit) - norm, p = exp2_(lp * A(LOG2E));
 #ifdef ENTROPY
-  // (p = 0 where log p = -inf: kept finite, so that the product is 0)
-  A r = -p * cupy::fma_(gh, max_(lp, A(-1e30)) + h, gain);
+  // (p = 0 long before log p is at -30000: kept there, so that the product with a
+  // large gradient is finite and 0)
+  A r = -p * cupy::fma_(gh, max_(lp, A(-30000)) + h, gain);
 #else
   A r = -p * gain;
 #endif

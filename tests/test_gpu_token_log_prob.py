@@ -263,6 +263,23 @@ def test_gradient_against_differences():
         assert abs((loss(x + e) - loss(x - e)) / 2e-5 - grad[at]) <= 1e-7
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_large_gradients_of_the_entropy(dtype):
+    # what is ruled out has the gradient 0, however large the row's is: the second
+    # row's only token has p = 1, log p = 0 and the entropy 0
+    x = np.full((2, 40), -np.inf, dtype)
+    x[0, 3], x[0, 30], x[1, 7] = 1, 1, 2
+    x[1, 20] = np.finfo(dtype).min
+    xd, td = cp.asarray(x), cp.asarray([3, 7])
+    r = cp.token_log_prob(xd, td, entropy=True)
+    gh = cp.asarray(np.full(2, 1e12, acc(dtype)))
+    got = cp.token_log_prob_grad(cp.zeros(2, acc(dtype)), xd, td, r.lse, entropy=r.entropy,
+                                 entropy_grad=gh, out=cp.empty_like(xd)).get()
+    assert not np.isnan(got).any()
+    got[0, [3, 30]] = got[1, 7] = 0            # (rounding errors, times the gradient)
+    assert not got.any()
+
+
 @pytest.mark.parametrize('dtype', ['float16', 'float32'])
 def test_layouts(dtype):
     base = logits_of((30, 4100), dtype, 8)

@@ -183,8 +183,9 @@ cupy_norm_of_sums(double* temp, const long long n, N_T* norm, const double max_n
   if (threadIdx.x == 0) {
     const double r = __builtin_sqrt(t);
     *norm = static_cast<N_T>(r);
-    const double q = max_norm / (r + eps);
-    temp[0] = q >= 1.0 ? 1.0 : q;       // (a NaN stays one)
+    // (compared before the division: 0 / 0 and inf / inf leave the arrays as they
+    // are; the factor of a NaN is one)
+    temp[0] = max_norm >= r + eps ? 1.0 : max_norm / (r + eps);
   }
 }
 ''')
@@ -366,7 +367,8 @@ def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
 
     Every array is multiplied by ``min(1, max_norm / (norm + eps))`` and rounded
     once.  Where the norm is infinite the factor is 0, where it is NaN the
-    factor is NaN.
+    factor is NaN.  Arrays whose norm plus ``eps`` does not exceed ``max_norm``,
+    which may be infinite, keep their bits.
 
     Args:
         arrays: sequence of float16, float32 and float64 arrays; scaled in

@@ -112,6 +112,14 @@ def test_large_small_and_missing_values():
     assert not x[0].get().any()
 
 
+def test_bounds_that_are_met_exactly():
+    for values, bound in (([0.0, 0.0], 0.0), ([3.0, 4.0], 5.0), ([3.0, 4.0], np.inf), ([np.inf, 1.0], np.inf)):
+        x = cp.asarray(np.array(values, 'float32'))
+        n = cp.clip_by_global_norm([x], bound, eps=0.0)
+        assert n.get() == np.sqrt(np.sum(np.square(values)))
+        assert np.array_equal(x.get(), np.array(values, 'float32'))
+
+
 @pytest.mark.parametrize('dtype', ['float16', 'float32'])
 def test_arrays_that_start_anywhere(dtype):
     flat = np.random.default_rng(1).standard_normal(200000).astype(dtype)

@@ -307,6 +307,7 @@ def _run(arrays, targets, norm_out, max_norm, eps):
     if tables is None:
         if write and norm_out is not None:
             _check_beside(norm_out, finals)
+            _check_beside(norm_out, arrays)
         arrays, targets, aside = _prepare(arrays, targets, write)
         tables = _tables(arrays, targets, write)
     dtype = _TYPES[2 if tables and tables[-1][0] == 2 else 1]
@@ -344,7 +345,7 @@ def _check_beside(norm_out, arrays):
     for a in arrays:
         _oc.check_array(a, 'arrays')
         if _rt.hot.overlap([a, norm_out], _oc._pack_spans([a, norm_out], [(0, 1, False)])):
-            raise ValueError('norm_out overlaps an array to write')
+            raise ValueError('norm_out overlaps an array to scale or to write')
 
 
 def global_norm(arrays, *, norm_out=None):
@@ -377,7 +378,8 @@ def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
         eps (float): added to the norm in the quotient.
         out: sequence of arrays that receive the results, of the same shapes
             and types; each may be the array it belongs to.
-        norm_out (cupy.ndarray): receives the norm, of shape ``()``.
+        norm_out (cupy.ndarray): receives the norm, of shape ``()``; it may not
+            lie in any of the arrays.
 
     Returns:
         cupy.ndarray: the norm before scaling, as :func:`global_norm` returns it.

@@ -665,8 +665,9 @@ typedef struct {
  * arrays in it, workgroups)], bytes), or None for arrays that need preparation: of
  * another type or device, not stored in one piece in the order of their targets
  * (None: themselves), of other shapes or types than these, or (with `write`)
- * sharing memory where it is written, with each other or with the array `beside`
- * (if not None).  A table holds `entries` TableEntry, zeros
+ * sharing memory where it is written, with each other, or with the array `beside`
+ * (if not None), which is written between the reading of the arrays for their norm
+ * and that for their scaling.  A table holds `entries` TableEntry, zeros
  * behind the last; a workgroup takes `vectors` vectors of 16 bytes that start on
  * 16-byte borders of the source.  Empty arrays are left out. */
 static PyObject* hp_tables(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
@@ -735,7 +736,9 @@ static PyObject* hp_tables(PyObject* self, PyObject* const* args, Py_ssize_t nar
     const uint64_t bytes = one.bytes ? one.bytes : one.elements * 16;
     if (!one.dense) plain = 0;
     for (Py_ssize_t i = 0; i < n; ++i)
-      if (dst[i].start < one.start + bytes && one.start < dst[i].start + dst[i].bytes) plain = 0;
+      if ((dst[i].start < one.start + bytes && one.start < dst[i].start + dst[i].bytes) ||
+          (src[i].start < one.start + bytes && one.start < src[i].start + src[i].bytes))
+        plain = 0;
   }
   if (!plain || (write && !are_apart(src, dst, n, sorted))) {
     result = Py_None;

@@ -195,6 +195,18 @@ def test_global_norm_refuses():
     assert cp.global_norm([x, arr(0, 'float64')]).dtype == 'float64'
 
 
+def test_the_norm_is_written_beside_what_is_scaled():
+    # (the norm is written between the two readings of an array)
+    flat, into = arr(10), arr(10)
+    for a, b in ((flat, into), (flat[::2], into[::2])):
+        with pytest.raises(ValueError):
+            cp.clip_by_global_norm([a], 1.0, out=[b], norm_out=flat[4:5].reshape(()))
+        with pytest.raises(ValueError):
+            cp.clip_by_global_norm([a], 1.0, out=[b], norm_out=into[4:5].reshape(()))
+    cp.clip_by_global_norm([flat], 1.0, out=[into], norm_out=arr(()))
+    cp.global_norm([flat], norm_out=flat[4:5].reshape(()))        # (read once, before)
+
+
 # -- rows, overlap, descriptions ----------------------------------------------------------
 
 def test_row_form():

@@ -559,6 +559,18 @@ typedef struct {
   int64_t device;
 } Description;
 
+/* The attribute `name` of `a`, looked for among its own attributes `own` before
+ * those of its type (145 arrays: 16 us, 18.5 the other way round; lists of
+ * hundreds of gradients are described per call). */
+static PyObject* attribute(PyObject* a, PyObject* own, PyObject* name) {
+  PyObject* v = PyDict_GetItemWithError(own, name);
+  if (v) {
+    Py_INCREF(v);
+    return v;
+  }
+  return PyErr_Occurred() ? NULL : PyObject_GetAttr(a, name);
+}
+
 /* What `a` is; 0, or -1 with an error set.  `item` are the sizes of the types. */
 static int describe_one(PyObject* a, PyObject* types, const uint64_t* item, Description* d) {
   if (!array_type || !PyObject_TypeCheck(a, array_type)) {
@@ -568,15 +580,18 @@ static int describe_one(PyObject* a, PyObject* types, const uint64_t* item, Desc
   PyObject *data = NULL, *ptr = NULL, *dev = NULL, *size = NULL, *dtype = NULL;
   PyObject *c_order = NULL, *f_order = NULL;
   int rc = -1;
-  data = PyObject_GetAttr(a, str_data);
+  PyObject* own = PyObject_GenericGetDict(a, NULL);
+  if (!own) return -1;
+  data = attribute(a, own, str_data);
   if (data) {
     ptr = PyObject_GetAttr(data, str_ptr);
     dev = PyObject_GetAttr(data, str_device_id);
   }
-  size = PyObject_GetAttr(a, str_size);
-  dtype = PyObject_GetAttr(a, str_dtype);
-  c_order = PyObject_GetAttr(a, str_c_contiguous);
-  f_order = PyObject_GetAttr(a, str_f_contiguous);
+  size = attribute(a, own, str_size);
+  dtype = attribute(a, own, str_dtype);
+  c_order = attribute(a, own, str_c_contiguous);
+  f_order = attribute(a, own, str_f_contiguous);
+  Py_DECREF(own);
   if (ptr && dev && size && dtype && c_order && f_order && as_u64(ptr, &d->start) == 0 &&
       as_u64(size, &d->elements) == 0) {
     const Py_ssize_t n_types = PyList_GET_SIZE(types);
@@ -634,23 +649,26 @@ static int by_start(const void* a, const void* b) {
 static int are_apart(const Description* src, const Description* dst, Py_ssize_t n,
                      const Description** sorted) {
   Py_ssize_t m = 0;
-  for (Py_ssize_t i = 0; i < n; ++i)
-    if (dst[i].bytes) sorted[m++] = &dst[i];
-  qsort(sorted, (size_t)m, sizeof(*sorted), by_start);
+  int in_order = 1;                        /* (as arrays cut from one piece are) */
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!dst[i].bytes) continue;
+    if (m && dst[i].start < sorted[m - 1]->start) in_order = 0;
+    sorted[m++] = &dst[i];
+  }
+  if (!in_order) qsort(sorted, (size_t)m, sizeof(*sorted), by_start);
   for (Py_ssize_t k = 1; k < m; ++k)
     if (sorted[k]->start < sorted[k - 1]->start + sorted[k - 1]->bytes) return 0;
   if (src == dst) return 1;
   for (Py_ssize_t i = 0; i < n; ++i) {
-    if (!src[i].bytes) continue;
     const uint64_t lo = src[i].start, hi = lo + src[i].bytes;
+    if (!src[i].bytes || lo == dst[i].start) continue;
     Py_ssize_t a = 0, b = m;               /* the first output that ends behind `lo` */
     while (a < b) {
       const Py_ssize_t mid = (a + b) / 2;
       if (sorted[mid]->start + sorted[mid]->bytes > lo) b = mid;
       else a = mid + 1;
     }
-    for (; a < m && sorted[a]->start < hi; ++a)
-      if (sorted[a] != &dst[i] || dst[i].start != lo) return 0;
+    if (a < m && sorted[a]->start < hi) return 0;
   }
   return 1;
 }

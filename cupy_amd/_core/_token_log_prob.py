@@ -288,7 +288,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
   constexpr int kWaves = BLOCK / 64;
   __shared__ Run lds[kWaves];
 #if TOP > 0
-  constexpr int kMost = BLOCK < 256 ? 4 * BLOCK : 1024;
+  constexpr int kMost = TOP == 1 ? 1 : BLOCK < 256 ? 4 * BLOCK : 1024;
   __shared__ TopState<kMost> ts;
 #endif
   Outputs out;
@@ -355,20 +355,20 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
 #if TOP > 0
     // The best key of every thread, then of 64 groups of threads.
     Key mine = no_key(0);
-    if (once) {
+    if (best_at < j1) {
+      cupy::Vec<X_T, VEC> from = v[0];
+      if (once) {
 #pragma unroll
-      for (int k = UNROLL - 1; k >= 0; --k)
-#pragma unroll
-        for (int i = VEC - 1; i >= 0; --i) {
-          const int j = j0 + k * BLOCK + threadIdx.x;
-          if (j == best_at && j < j1 && static_cast<A>(v[k].v[i]) == best)
-            mine = key_at(v[k], j, i, vecs);
-        }
-    } else if (best_at < j1) {
-      const cupy::Vec<X_T, VEC> w = vecs.load(best_at);
+        for (int k = 1; k < UNROLL; ++k)
+          from = cupy::select_value(best_at == j0 + k * BLOCK + (int)threadIdx.x, v[k], from);
+      } else {
+        from = vecs.load(best_at);
+      }
+      int at = -1;
 #pragma unroll
       for (int i = VEC - 1; i >= 0; --i)
-        if (static_cast<A>(w.v[i]) == best) mine = key_at(w, best_at, i, vecs);
+        if (static_cast<A>(from.v[i]) == best) at = i;
+      if (at >= 0) mine = key_of(best, (u32)(vecs.column(best_at) + at));
     }
     Key other = no_key(0);
     if (single >= 0 && alone == alone) {
@@ -394,29 +394,6 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     }
 #if TOP > 0
     const Key least = bar(ts);
-    // whoever may hold one of the best looks through its vectors again
-    if (!better(least, mine)) {
-      if (single >= 0) offer(ts, static_cast<A>(alone), other, least);
-      if (once) {
-#pragma unroll
-        for (int k = 0; k < UNROLL; ++k) {
-          const int j = j0 + k * BLOCK + threadIdx.x;
-          if (j >= j1) break;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            offer(ts, static_cast<A>(v[k].v[i]), key_at(v[k], j, i, vecs), least);
-        }
-      } else {
-        for (int j = j0 + threadIdx.x; j < j1; j += BLOCK) {
-          const cupy::Vec<X_T, VEC> w = vecs.load(j);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            offer(ts, static_cast<A>(w.v[i]), key_at(w, j, i, vecs), least);
-        }
-      }
-    }
-    __syncthreads();
-    const u32 found = ts.n;
     Key* keys = reinterpret_cast<Key*>(runs + at_keys) + w * TOP;
     const double lse_ = run.lse();
     auto put = [&](int rank, const Key& k) {
@@ -426,6 +403,58 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
         keys[rank] = k;
       }
     };
+#if TOP == 1
+    if (threadIdx.x == 0) put(0, least);
+#else
+    // The vectors of whoever may hold one of the best are looked through again.
+    const bool look = !better(least, mine);
+    const A enough = is_none(least) ? -__builtin_inff() : value_of(least);
+    if (look && single >= 0) offer(ts, static_cast<A>(alone), other, least);
+    if (once) {
+      if (look) {
+#pragma unroll
+        for (int k = 0; k < UNROLL; ++k) {
+          const int j = j0 + k * BLOCK + threadIdx.x;
+          if (j >= j1) break;
+          if (!(largest(v[k]) >= enough)) continue;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            offer(ts, static_cast<A>(v[k].v[i]), key_at(v[k], j, i, vecs), least);
+        }
+      }
+    } else {
+      // They are not at hand any more: all lanes of a wave share those of its
+      // threads (216 rows of 155176 float32, 5 of them: AGAIN us; 38 with every thread
+      // after its own, 50 of them one by one).
+      const int lane = threadIdx.x & 63;
+      const unsigned long long lookers = __ballot(look), below = (1ull << lane) - 1;
+      const int count = __popcll(lookers);
+      // lane r is told the r-th of them
+      const int to = look ? __popcll(lookers & below) : count + __popcll(~lookers & below);
+      const int list = __builtin_amdgcn_ds_permute(to * 4, (int)threadIdx.x);
+      const u32 trips = (j1 - j0 + BLOCK - 1) / BLOCK, items = count * trips;
+      constexpr int kAgain = 4;
+      for (u32 base = 0; base < items; base += 64 * kAgain) {
+        cupy::Vec<X_T, VEC> again[kAgain];
+        int at[kAgain];
+#pragma unroll
+        for (int k = 0; k < kAgain; ++k) {
+          const u32 item = base + k * 64 + lane, who = item / trips;
+          at[k] = j0 + (int)(item - who * trips) * BLOCK + cupy::shfl_idx(list, (int)(who & 63));
+          if (item >= items || at[k] >= j1) at[k] = -1;
+          again[k] = vecs.load(at[k] < 0 ? j1 - 1 : at[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kAgain; ++k) {
+          if (at[k] < 0 || !(largest(again[k]) >= enough)) continue;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            offer(ts, static_cast<A>(again[k].v[i]), key_at(again[k], at[k], i, vecs), least);
+        }
+      }
+    }
+    __syncthreads();
+    const u32 found = ts.n;
     if (found <= kMost) {
       put_ranked(ts, found, put);
     } else {
@@ -457,6 +486,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
         }
       }
     }
+#endif
 #endif
     __syncthreads();
   }
@@ -518,13 +548,17 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
 #if TOP > 0
   __syncthreads();
   const Key least = bar(ts);
+  const double lse_ = run.lse();
+#if TOP == 1
+  if (threadIdx.x == 0) put_top(out, run, lse_, row, 0, least);
+#else
 #pragma unroll
   for (int q = 0; q < kEach; ++q)
     if (!is_none(mine[q])) offer(ts, value_of(mine[q]), mine[q], least);
   __syncthreads();
-  const double lse_ = run.lse();
   put_ranked(ts, ts.n,
              [&](int rank, const Key& k) { put_top(out, run, lse_, row, rank, k); });
+#endif
 #endif
 }
 ''')

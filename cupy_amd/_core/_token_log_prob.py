@@ -103,7 +103,8 @@ struct Run {
   _CUPY_DEV double log2_sum() const { return log2((double)s); }
   _CUPY_DEV double lse() const {
     if (s == A(0)) return -__builtin_inf();          // every element is -inf
-    if (half()) return ((double)(m * A(LOG2E)) + log2_sum()) / (double)A(LOG2E);
+    constexpr double back = 1.0 / (double)A(LOG2E);
+    if (half()) return ((double)(m * A(LOG2E)) + log2_sum()) * back;
     return (double)m + log2_sum() * LN2;
   }
   _CUPY_DEV double entropy() const {
@@ -200,6 +201,7 @@ struct TopState {
   Key sample[64];               // (no two alike)
   Key key[kMost];
   Key last;
+  double lse;
   u32 n;
 };
 
@@ -213,10 +215,17 @@ _CUPY_DEV Key bar(const State& t) {
   return cupy::shfl_idx(me, __ffsll(__ballot(rank == TOP - 1)) - 1);
 }
 
-// Keeps an element that is as good as `least` (a NaN is none: its row has no order).
+// The value that an element as good as `least` has at least.
+_CUPY_DEV A value_at_least(const Key& least) {
+  return is_none(least) ? -__builtin_inff() : value_of(least);
+}
+// Keeps an element that is as good as `least`, whose value is `enough` (a NaN is
+// none: its row has no order).  The values are compared first: few pass.
 template <typename State>
-_CUPY_DEV void offer(State& t, A value, const Key& k, const Key& least) {
-  if (better(least, k) | !(value == value)) return;
+_CUPY_DEV void offer(State& t, A value, u32 column, const Key& least, A enough) {
+  if (!(value >= enough)) return;
+  const Key k = key_of(value, column);
+  if (better(least, k)) return;
   const u32 at = atomicAdd(&t.n, 1u);
   if (at < State::kMost) t.key[at] = k;
 }
@@ -254,9 +263,8 @@ _CUPY_DEV A logit_of(const X_T* x, long long token, int width) {
 }
 
 // A row's results from its joined statistics, by one thread.
-_CUPY_DEV void put_row(const Outputs& o, const Run& run, A logit, long long token, long long row,
-                       int width) {
-  const double lse = run.lse();
+_CUPY_DEV void put_row(const Outputs& o, const Run& run, double lse, A logit, long long token,
+                       long long row, int width) {
   o.lse[row] = static_cast<A>(lse);
   double lp = 0.0;
   if (token >= 0 && token < width)
@@ -353,9 +361,10 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     run = join_lanes<64>(run);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = run;
 #if TOP > 0
-    // The best key of every thread, then of 64 groups of threads.
-    Key mine = no_key(0);
+    // The best of every thread, then of 64 groups of threads.
+    Key mine = no_key(0), most = no_key(0);
     if (best_at < j1) {
+#if TOP == 1
       cupy::Vec<X_T, VEC> from = v[0];
       if (once) {
 #pragma unroll
@@ -369,11 +378,18 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
       for (int i = VEC - 1; i >= 0; --i)
         if (static_cast<A>(from.v[i]) == best) at = i;
       if (at >= 0) mine = key_of(best, (u32)(vecs.column(best_at) + at));
+#else
+      // Which element of its vector it is stays open, so that nothing is loaded:
+      // the key is `mine` at least and `most` at most.
+      mine = key_of(best, (u32)(vecs.column(best_at) + VEC - 1));
+      most = key_of(best, (u32)vecs.column(best_at));
+#endif
     }
     Key other = no_key(0);
     if (single >= 0 && alone == alone) {
       other = key_of(static_cast<A>(alone), (u32)single);
       mine = BestKey()(mine, other);
+      most = BestKey()(most, other);
     }
     const Key group = cupy::group_allreduce<kWaves>(mine, BestKey());
     if (threadIdx.x % kWaves == 0)
@@ -384,7 +400,11 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     run = join_lanes<kWaves>(lds[threadIdx.x & (kWaves - 1)]);
     if (threadIdx.x == 0) {
       if (parts == 1) {
-        put_row(out, run, logit, token, row, width);
+        const double lse = run.lse();
+        put_row(out, run, lse, logit, token, row, width);
+#if TOP > 0
+        ts.lse = lse;
+#endif
       } else {
         A* to = runs + w * 3;
         to[0] = run.m;
@@ -393,23 +413,33 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
       }
     }
 #if TOP > 0
-    const Key least = bar(ts);
     Key* keys = reinterpret_cast<Key*>(runs + at_keys) + w * TOP;
-    const double lse_ = run.lse();
     auto put = [&](int rank, const Key& k) {
       if (parts == 1) {
-        put_top(out, run, lse_, row, rank, k);
+        put_top(out, run, ts.lse, row, rank, k);
       } else {
         keys[rank] = k;
       }
     };
 #if TOP == 1
-    if (threadIdx.x == 0) put(0, least);
+    if (threadIdx.x < 64) {
+      const Key b = cupy::group_allreduce<64>(ts.sample[threadIdx.x], BestKey());
+      if (threadIdx.x == 0) put(0, b);
+    }
 #else
+    // (one wave finds the bar: what every wave does here costs the most of it)
+    if (kWaves > 1) {
+      if (threadIdx.x < 64) {
+        const Key b = bar(ts);
+        if (threadIdx.x == 0) ts.last = b;
+      }
+      __syncthreads();
+    }
+    const Key least = kWaves > 1 ? ts.last : bar(ts);
     // The vectors of whoever may hold one of the best are looked through again.
-    const bool look = !better(least, mine);
-    const A enough = is_none(least) ? -__builtin_inff() : value_of(least);
-    if (look && single >= 0) offer(ts, static_cast<A>(alone), other, least);
+    const bool look = !better(least, most);
+    const A enough = value_at_least(least);
+    if (look && single >= 0) offer(ts, static_cast<A>(alone), (u32)single, least, enough);
     if (once) {
       if (look) {
 #pragma unroll
@@ -419,12 +449,12 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
           if (!(largest(v[k]) >= enough)) continue;
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            offer(ts, static_cast<A>(v[k].v[i]), key_at(v[k], j, i, vecs), least);
+            offer(ts, static_cast<A>(v[k].v[i]), (u32)(vecs.column(j) + i), least, enough);
         }
       }
     } else {
       // They are not at hand any more: all lanes of a wave share those of its
-      // threads (216 rows of 155176 float32, 5 of them: AGAIN us; 38 with every thread
+      // threads (216 rows of 155176 float32, 5 of them: 35 us; 38 with every thread
       // after its own, 50 of them one by one).
       const int lane = threadIdx.x & 63;
       const unsigned long long lookers = __ballot(look), below = (1ull << lane) - 1;
@@ -449,7 +479,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
           if (at[k] < 0 || !(largest(again[k]) >= enough)) continue;
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            offer(ts, static_cast<A>(again[k].v[i]), key_at(again[k], at[k], i, vecs), least);
+            offer(ts, static_cast<A>(again[k].v[i]), (u32)(vecs.column(at[k]) + i), least, enough);
         }
       }
     }
@@ -544,17 +574,21 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
     run.s = run.u = A(0);
   }
   run = join_lanes<64>(run);     // (by every wave for itself)
-  if (threadIdx.x == 0) put_row(out, run, logit, token, row, width);
+  const double lse_ = run.lse();
+  if (threadIdx.x == 0) put_row(out, run, lse_, logit, token, row, width);
 #if TOP > 0
   __syncthreads();
-  const Key least = bar(ts);
-  const double lse_ = run.lse();
 #if TOP == 1
-  if (threadIdx.x == 0) put_top(out, run, lse_, row, 0, least);
+  if (threadIdx.x < 64) {
+    const Key b = cupy::group_allreduce<64>(ts.sample[threadIdx.x], BestKey());
+    if (threadIdx.x == 0) put_top(out, run, lse_, row, 0, b);
+  }
 #else
+  const Key least = bar(ts);
+  const A enough = value_at_least(least);
 #pragma unroll
   for (int q = 0; q < kEach; ++q)
-    if (!is_none(mine[q])) offer(ts, value_of(mine[q]), mine[q], least);
+    if (!is_none(mine[q])) offer(ts, value_of(mine[q]), column_of(mine[q]), least, enough);
   __syncthreads();
   put_ranked(ts, ts.n,
              [&](int rank, const Key& k) { put_top(out, run, lse_, row, rank, k); });

@@ -755,7 +755,7 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
         call.dense(i)
     call.begin()
     vec = 16 // logits.dtype.itemsize
-    block, unroll, parts = _geometry(rows, max(1, width // vec))
+    block, unroll, parts = _geometry(rows, max(1, width // vec), top)
     nt_in = _oc.stream_hints(logits.nbytes, 0)[0] and not top
     defines = dict(X_T=logits.dtype, I_T=call.refs[1].dtype, BLOCK=block, UNROLL=unroll, VEC=vec,
                    TOP=top, MAX_TOP=MAX_TOP, SMALL_KEYS=int(acc == numpy.float32), NT_IN=nt_in, NT_OUT=False)
@@ -780,7 +780,7 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
     return _named(call.finish(ret), entropy, top)
 
 
-def _geometry(rows, vecs):
+def _geometry(rows, vecs, top):
     """(threads of a workgroup, vectors a thread requests at a time, parts of a row)"""
     units = _oc.compute_units()
     block, parts = 256, 1
@@ -793,13 +793,18 @@ def _geometry(rows, vecs):
         # (300 rows of 32000 float32: 19 us with 512 threads to a row, 21 with
         # 256; 1000 rows of 16000 float16: 22.9 and 19.7)
         block = 512 if vecs > 2048 else 256
-    elif vecs <= 512:
+    elif vecs <= 512 or (top > 1 and vecs <= 1024):
         # Short rows: one wave to each, whose reductions meet no barrier (16384
-        # rows of 1500 float16: 18.5 us; 23.9 with two waves, 31.2 with four; with
-        # 5 alternatives 38.9, 55 and 83).  Long ones: four waves, so that a unit
-        # holds eight rows (8192 rows of 50257 float16 with entropy: 140 us; 175
-        # with eight waves, 220 with sixteen).
+        # rows of 1500 float16: 17.5 us; 22.5 with two waves, 30 with four).  What
+        # is done for alternatives is done by every wave, so that fewer are best
+        # there (8000 rows of 8000 float16, 5 of them: 37 us; 45 with two waves, 57
+        # with four).
         block = 64
+    elif top > 1 and vecs <= 2048:
+        # (4000 rows of 8000 float32, 5 of them: 32 us; 32 with one wave, 37 with four)
+        block = 128
+    # Long ones: four waves, so that a unit holds eight rows (8192 rows of 50257
+    # float16 with entropy: 140 us; 175 with eight waves, 220 with sixteen).
     return block, 4, parts
 
 

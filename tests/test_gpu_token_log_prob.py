@@ -52,9 +52,10 @@ class Exact:
 
 
 def chain(width):
-    # additions a lane makes (64 lanes to rows of up to 512 vectors of 8 elements,
-    # at least 256 to longer ones), and joins
-    return width / (64 if width <= 4104 else 256) + 40
+    # additions a lane makes (64 lanes at least to rows of up to 1024 vectors of 8
+    # elements and a few single ones, 128 to twice as long ones, 256 to longer ones),
+    # and joins
+    return width / (64 if width <= 8208 else 128 if width <= 16400 else 256) + 40
 
 
 def check(x, tokens, got, top=0):

@@ -784,14 +784,20 @@ def _geometry(rows, vecs, top):
     """(threads of a workgroup, vectors a thread requests at a time, parts of a row)"""
     units = _oc.compute_units()
     block, parts = 256, 1
-    if rows < 2 * units and vecs > 8192:
-        # Rows too few to fill the device are cut into parts; a second launch
-        # joins them, which costs about 5 us (64 rows of 32000 float16: 13.5 us
-        # in parts, 11.5 in one launch; 8 rows of 131072 float32: 12.5 against 25).
+    if rows < units * 3 // 8 and vecs > 14336:
+        # Long rows, too few to fill the device, are cut into parts; a second
+        # launch joins them, which costs about 5 us (64 rows of 128000 float16: 15
+        # us in parts, 16.3 in one launch; 64 of 200000 float32: 19 and 24; 8 of
+        # 131072 float32: 12.5 and 18; but 100 of 64000 float32: 15.8 and 12.5, 32
+        # of 50257: 14 and 11).
         parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
+    elif rows <= units and vecs > 2048:
+        # (190 rows of 100000 float16: 16.4 us; 17.6 with 512 threads to a row, 24
+        # with 256)
+        block = 1024
     elif rows < 4 * units:
-        # (300 rows of 32000 float32: 19 us with 512 threads to a row, 21 with
-        # 256; 1000 rows of 16000 float16: 22.9 and 19.7)
+        # (300 rows of 100000 float16: 23 us with 512 threads to a row, 25 with 256,
+        # 27 with 1024; 1000 rows of 16000 float16: 22.9 and 19.7)
         block = 512 if vecs > 2048 else 256
     elif vecs <= 512 or (top > 1 and vecs <= 1024):
         # Short rows: one wave to each, whose reductions meet no barrier (16384

@@ -107,7 +107,7 @@ def test_log_prob(shape, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('width', [40, 3001, 20000, 70001])
+@pytest.mark.parametrize('width', [40, 3001, 20000, 70001, 140001])
 def test_ties_masks_and_bands(dtype, width):
     """Equal values, values in one place, ruled out elements: the likeliest tokens
     in every order of storage."""
@@ -312,8 +312,9 @@ def test_layouts(dtype):
     check(np.tile(base[0], (4, 1)), t[:4], cp.token_log_prob(one, cp.asarray(t[:4]), top=2), 2)
 
 
-def test_streams_and_replays():
-    x, t = logits_of((6, 60000), 'float16', 1), tokens_of((6, 60000))
+@pytest.mark.parametrize('width', [60000, 120000])
+def test_streams_and_replays(width):
+    x, t = logits_of((6, width), 'float16', 1), tokens_of((6, width))
     xd, td = cp.asarray(x), cp.asarray(t)
     want = [a.get() for a in cp.token_log_prob(xd, td, entropy=True, top=8)]
     streams = [cp.cuda.Stream(non_blocking=True) for _ in range(2)]

@@ -19,6 +19,7 @@ from cupy_amd._core._ufuncs import elementwise_copy
 from cupy_amd._core.core import ndarray, _byte_extent
 from cupy_amd.cuda import device as _device
 from cupy_amd.cuda import memory as _memory
+from cupy_amd.cuda import stream as _stream
 
 _MAX = 100                  # arrays to a launch: 3200 bytes of its 4 KiB of arguments
 _BLOCK = 256
@@ -190,8 +191,6 @@ cupy_norm_of_sums(double* temp, const long long n, N_T* norm, const double max_n
 }
 ''')
 
-_TYPES = [numpy.dtype(c) for c in _oc.FLOATS]
-
 
 def _describe(arrays, name):
     """Addresses, sizes, types and layouts of a list of arrays, checked."""
@@ -276,6 +275,7 @@ class _Temporary:
 
     def __init__(self, words):
         self.nbytes = 8 * words
+        self.stream = _stream.get_current_stream_ptr()
         self.static = _memory.static_scratch_active()
         if not self.static:
             self.memory = _memory.alloc(self.nbytes)
@@ -288,20 +288,29 @@ class _Temporary:
         """``before`` and ``after`` are the arguments around the temporary's address."""
         if self.static:
             fn.launch_packed_scratch((blocks, 1, 1), (block, 1, 1), before + bytes(8) + after,
-                                     len(before), self.nbytes)
+                                     len(before), self.nbytes, 0, self.stream)
         else:
             fn.launch_packed((blocks, 1, 1), (block, 1, 1),
-                             before + struct.pack('<Q', self.memory.ptr) + after)
+                             before + struct.pack('<Q', self.memory.ptr) + after, 0, self.stream)
 
 
-def _defines(dtype, nbytes):
-    return dict(X_T=dtype, MAX_ENTRIES=_MAX, BLOCK=_BLOCK, UNROLL=_UNROLL,
-                VEC=16 // dtype.itemsize, NT_IN=False,
-                NT_OUT=_oc.stream_hints(nbytes, nbytes)[1])
+_functions = {}
+
+
+def _function(name, dev, t, nbytes):
+    """The kernel for arrays of the type ``_TYPES[t]``, ``nbytes`` in all."""
+    key = name, dev, t, _oc.stream_hints(nbytes, nbytes)[1]
+    fn = _functions.get(key)
+    if fn is None:
+        fn = _functions[key] = _SOURCE.function(
+            name, X_T=_TYPES[t], MAX_ENTRIES=_MAX, BLOCK=_BLOCK, UNROLL=_UNROLL,
+            VEC=16 // _TYPES[t].itemsize, NT_IN=False, NT_OUT=key[3])
+    return fn
 
 
 def _run(arrays, targets, norm_out, max_norm, eps):
     write = max_norm is not None
+    dev = _device.get_device_id()
     finals, aside = arrays if targets is None else targets, ()
     tables = _tables(arrays, targets, write, norm_out)
     if tables is None:
@@ -321,7 +330,7 @@ def _run(arrays, targets, norm_out, max_norm, eps):
     for t, launches, nbytes in tables:
         if not launches:
             continue
-        fn = _SOURCE.function('cupy_square_sums', **_defines(_TYPES[t], nbytes))
+        fn = _function('cupy_square_sums', dev, t, nbytes)
         for table, n, blocks in launches:
             temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, 0), struct.pack('<q', at))
             at += blocks
@@ -332,7 +341,7 @@ def _run(arrays, targets, norm_out, max_norm, eps):
         for t, launches, nbytes in reversed(tables):
             if not launches:
                 continue
-            fn = _SOURCE.function('cupy_scale_arrays', **_defines(_TYPES[t], nbytes))
+            fn = _function('cupy_scale_arrays', dev, t, nbytes)
             for table, n, blocks in reversed(launches):
                 temp.launch(fn, blocks, _BLOCK, table + struct.pack('<ii', n, blocks))
         for i in aside:

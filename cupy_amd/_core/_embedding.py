@@ -7,7 +7,8 @@ of the positions: the pairs (token, position) are sorted (a stable radix sort
 with the positions as its payload), cut into chunks of equal length whatever
 the tokens are, and every chunk sums its runs of equal tokens in registers.
 Runs that cross the border of a chunk leave partial sums that a last kernel
-joins, in order.  The reference scatters such gradients atomically
+joins, in order.  Few tokens need no sort: each is compared with all others.
+The reference scatters such gradients atomically
 (cupy/_core/_routines_indexing.pyx:899-1120 ``_scatter_op``).
 """
 import math
@@ -487,6 +488,181 @@ cupy_embedding_join(const u32* temp, O_T* out, const long long at_pairs,
 }
 ''')
 
+# -- few tokens ---------------------------------------------------------------------------
+# Up to _FEW of them take one launch without a sort.  A workgroup to every
+# position (and 64 vectors of columns) compares its token with all others: the
+# first position of a token collects the later ones, in order, and sums their
+# rows.  Further workgroups clear the rows of the table that no token names,
+# which they find by marking those that are named in a bitmap of their share.
+# Bound by latency: the tokens, a row, the result are one chain (1011 tokens, 9846
+# x 178 float32: 6.5 us, 13.4 with the sort).
+
+_DIRECT = _oc.Source(r'''
+#include <cupy/rows.cuh>
+typedef cupy::acc_of<G_T>::type A;
+typedef unsigned int u32;
+typedef unsigned long long u64;
+
+constexpr int kThreads = 256;
+constexpr int kIds = FEW / kThreads;             // tokens that a thread looks at
+constexpr int kWords = FEW / 64;                 // of 64 positions
+constexpr int kSlices = 4;                       // of a long list of positions: a wave each
+constexpr int kMany = 8;                         // ... which is of more than so many
+
+// Zeros to the rows [r0, r1), stored one after the other: vectors from the first
+// cache line on, the elements before and behind them one by one.
+_CUPY_DEV void clear(O_T* out, long long r0, long long r1, int width) {
+  constexpr int kLine = 128 / sizeof(O_T);
+  const O_T zero = static_cast<O_T>(0.0f);
+  O_T* to = out + r0 * width;
+  const long long length = (r1 - r0) * width;
+  const int phase = (int)((reinterpret_cast<u64>(to) & 127) / sizeof(O_T));
+  long long head = phase ? kLine - phase : 0;
+  if (head > length) head = length;
+  const long long vecs = (length - head) / FILL_VEC;
+  cupy::Vec<O_T, FILL_VEC> zeros;
+#pragma unroll
+  for (int e = 0; e < FILL_VEC; ++e) zeros.v[e] = zero;
+  for (long long i = threadIdx.x; i < vecs; i += kThreads)
+    cupy::store_vec<O_T, FILL_VEC>(to + head + i * FILL_VEC, zeros);
+  const long long behind = head + vecs * FILL_VEC;
+  if (threadIdx.x < head) to[threadIdx.x] = zero;
+  if (threadIdx.x < length - behind) to[behind + threadIdx.x] = zero;
+}
+
+_CUPY_DEV cupy::Vec<G_T, VEC> row_part(const G_T* from, int width) {
+  return TINY ? cupy::load_part<G_T, VEC>(from, width) : cupy::load_vec<G_T, VEC>(from);
+}
+
+// The rows at the positions list[q0 .. q1 - 1], kAhead requested at a time: one
+// alone, or as many as fit, without a question between the requests.
+template <int kAhead>
+_CUPY_DEV void add_rows(A (&sum)[VEC], const G_T* g, const unsigned short* list, int q0, int q1,
+                        int width, long long pg) {
+  for (int q = q0; q < q1; q += kAhead) {
+    cupy::Vec<G_T, VEC> v[kAhead];
+    const int more = q1 - 1 - q;
+    v[0] = row_part(g + (long long)list[q] * pg, width);
+    if (more > 0) {
+#pragma unroll
+      for (int u = 1; u < kAhead; ++u)
+        v[u] = row_part(g + (long long)list[q + (u < more ? u : more)] * pg, width);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A term = static_cast<A>(v[u].v[e]);
+        sum[e] = u <= more ? sum[e] + term : sum[e];
+      }
+    }
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(kThreads)
+cupy_embedding_few(const G_T* g, const I_T* ids, O_T* out, const int n, const u32 rows,
+                   const int width, const long long pg, const long long po, const double scale_,
+                   const int clearing) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  long long id[kIds];
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    const int i = k * kThreads + (int)threadIdx.x;
+    id[k] = ids[i < n ? i : n - 1];
+  }
+  if ((int)blockIdx.x < clearing) {
+    __shared__ u32 named[64];                    // of the workgroup's rows, 2048 at most
+    if (blockIdx.y > 0) return;
+    const long long r0 = (long long)rows * blockIdx.x / clearing;
+    const long long r1 = (long long)rows * (blockIdx.x + 1) / clearing;
+    if (threadIdx.x < 64) named[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kIds; ++k)
+      if (id[k] >= r0 && id[k] < r1)
+        atomicOr(&named[(id[k] - r0) >> 5], 1u << ((id[k] - r0) & 31));
+    __syncthreads();
+    const u32 word = named[lane];
+    long long from = r0;
+    for (u64 words = __ballot(word != 0); words; words &= words - 1) {
+      const int j = __ffsll(words) - 1;
+      for (u32 bits = (u32)__builtin_amdgcn_readlane(word, j); bits; bits &= bits - 1) {
+        const long long row = r0 + j * 32 + __ffs(bits) - 1;
+        if (row > from) clear(out, from, row, width);
+        from = row + 1;
+      }
+    }
+    if (r1 > from) clear(out, from, r1, width);
+    return;
+  }
+  __shared__ u64 same[kWords];
+  __shared__ unsigned short list[FEW];
+  __shared__ cupy::Vec<A, VEC> part[kSlices][64];
+  const int t = blockIdx.x - clearing;
+  const long long token = ids[t];
+  if (token < 0 || token >= (long long)rows) return;
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    const u64 found = __ballot(id[k] == token && k * kThreads + (int)threadIdx.x < n);
+    if (lane == 0) same[k * (kThreads / 64) + wave] = found;
+  }
+  __syncthreads();
+  int count = 0, ahead[kIds];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    const u64 m = same[j];
+    // (an earlier position of the same token: its workgroup sums)
+    if (j * 64 < t && (m & (t - j * 64 < 64 ? (1ull << (t - j * 64)) - 1 : ~0ull))) return;
+    if (j % (kThreads / 64) == wave)
+      ahead[j / (kThreads / 64)] = count + __popcll(m & ((1ull << lane) - 1));
+    count += __popcll(m);
+  }
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    const int i = k * kThreads + (int)threadIdx.x;
+    if (id[k] == token && i < n) list[ahead[k]] = static_cast<unsigned short>(i);
+  }
+  __syncthreads();
+  // Few positions: one wave.  Many: a quarter of them to each of four, whose sums
+  // are added in order.
+  const bool many = count > kMany;
+  if (!many && wave > 0) return;
+  const int share = many ? (count + kSlices - 1) / kSlices : count;
+  const int q0 = wave * share, q1 = q0 + share < count ? q0 + share : count;
+  int c = (blockIdx.y * 64 + lane) * VEC;
+  const bool mine = c < width;
+  // (a vector over the end of the row moves back to end with it)
+  c = TINY || !mine ? 0 : c + VEC <= width ? c : width - VEC;
+  A sum[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[e] = A(0);
+  if (mine) {
+    if (many) add_rows<16>(sum, g + c, list, q0, q1, width, pg);
+    else add_rows<kMany>(sum, g + c, list, q0, q1, width, pg);
+  }
+  if (many) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[wave][lane].v[e] = sum[e];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int s = 1; s < kSlices; ++s)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += part[s][lane].v[e];
+  }
+  if (mine) {
+    const A scale = static_cast<A>(scale_);
+    cupy::Vec<O_T, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = static_cast<O_T>(sum[e] * scale);
+    cupy::store_part<O_T, VEC>(out + token * po + c, r, TINY ? width : VEC);
+  }
+}
+''')
+
+# Most tokens that take one launch.  (All of them one and the same are summed by four
+# waves: 1024 tokens, 9846 x 178 float32: 19 us, 17 with the sort; 8191 x 1000: 26 and 19.)
+_FEW = 1024
 # most pairs that are put in order by comparing all of them
 _RANKED = 12288
 
@@ -630,6 +806,22 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     out_vec = 16 // dt.itemsize
     nt_out = _oc.stream_hints(num_rows * width * dt.itemsize, num_rows * width * dt.itemsize)[1]
     acc = _oc.acc_dtype(grad.dtype).itemsize
+    vec = 16 // grad.dtype.itemsize
+    units = _oc.compute_units()
+    clearing = min(units, num_rows)
+    slices = -(-width // (64 * vec))
+    # One launch where the comparisons are few (1024 tokens, 8191 x 1009 float32:
+    # 11.4 us, 15.8 with the sort; x 2009: 19.7 and 18.9) and the table fits the last
+    # cache (131072 x 1024 float16, 268 MB: 50 and 51; x 1000 float32, 524 MB: 99 and 88).
+    looked = max(256, _oc.clp2(n))                     # (what every workgroup looks at)
+    if (n <= _FEW and n * slices * looked <= 1 << 22 and po == width
+            and num_rows * width * dt.itemsize <= 1 << 28 and -(-num_rows // clearing) <= 2048):
+        fn = _DIRECT.function('cupy_embedding_few', G_T=grad.dtype, O_T=dt, I_T=call.refs[1].dtype,
+                              FEW=looked, VEC=vec, FILL_VEC=out_vec, TINY=width < vec)
+        call.launch(fn, (clearing + n, slices, 1), 256, 'PPPiIiqqdi', Ref(0), Ref(1), Ref(i_out), n,
+                    num_rows, width, pg, po, scale, clearing)
+        return call.finish(i_out)
+    fill = min(units, -(-num_rows * width // (out_vec * 256)))
 
     # chunks: long enough that few runs cross their borders, short enough that
     # there are some per compute unit
@@ -653,7 +845,6 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     defines = dict(G_T=grad.dtype, O_T=dt, I_T=call.refs[1].dtype, ROUNDS=rounds,
                    FILL_VEC=out_vec, EACH=each, NT_OUT=nt_out)
     at = 0
-    fill = min(_oc.compute_units(), -(-num_rows * width // (out_vec * 256)))
     if rank:
         blocks = -(-n // (16 * each))
         fn = _GRAD.function('cupy_embedding_rank', **defines)
@@ -672,7 +863,6 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
             call.launch(move, (tiles + fill, 1, 1), 1024, 'PPqqqPqIiqiiiII', Ref(1), Ref(i_t), src,
                         at, 4 * n, Ref(i_out), n, num_rows, width, po, p * bits, bits, tiles,
                         cuts[2 * p + 1], cuts[2 * p + 2])
-    vec = 16 // grad.dtype.itemsize
     lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
     defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec, TINY=width < vec)
     fn = _SUMS.function('cupy_embedding_sums', **defines)

@@ -137,6 +137,30 @@ def test_gradient(n, rows, width, kind, dtype):
     assert np.array_equal(out.get(), got.get())
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,width', [(1, 1), (1, 40000), (70000, 1), (33333, 2), (9000, 7), (4097, 33),
+                                        (2500, 509), (700, 4100), (90, 40001)])
+def test_gradient_of_few_tokens(rows, width, dtype):
+    """Every element of the table is written once, whatever the table starts on,
+    and nothing beside it."""
+    rng = np.random.default_rng(rows)
+    for n, start in ((1, 0), (2, 1), (300, 3), (1024, 5)):
+        n = min(n, max(1, 2000000 // width))
+        ids = rng.integers(-1, rows + 1, n)
+        ids[:n // 4] = rng.integers(0, rows)
+        some = ids[n // 2:][:20]                       # the first rows, and the last
+        some[:] = np.arange(len(some)) - 3
+        ids[-1] = rows - 1
+        grad = make((n, width), dtype, n)
+        frame = cp.full(rows * width + 16, 7, dtype)
+        out = frame[start:start + rows * width].reshape(rows, width)
+        cp.embedding_grad(cp.asarray(grad), cp.asarray(ids), rows, 2.0, out=out)
+        check_grad(out, grad, ids, rows, 2.0)
+        rest = frame.get()
+        rest[start:start + rows * width] = 7
+        assert np.all(rest == 7)
+
+
 def test_gradient_types_and_layouts():
     ids = np.random.default_rng(1).integers(0, 50, (6, 40))
     grad = make((6, 40, 100), 'float16', 2)

@@ -12,6 +12,7 @@ import numpy
 
 from cupy_amd._core import _op_calls as _oc
 from cupy_amd._core._op_calls import Ref
+from cupy_amd._core.core import ndarray
 
 _SOURCE = _oc.Source(r'''
 #include <cupy/rows.cuh>
@@ -265,11 +266,13 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
 #ifdef WEIGHT
   cupy::Vec<W_T, VEC> wv[ITEMS];
   mine.load(wv, w);
+#ifndef FEW
   A dw[ITEMS][VEC];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[k][e] = A(0);
+#endif
 #endif
   int flip = 0;
   for (long long base = (long long)blockIdx.x * kRows; base < rows;
@@ -303,6 +306,9 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
     flip ^= 1;
     if (!valid) continue;
     const Factors f(s, width, static_cast<A>(eps));
+#ifdef FEW
+    if (threadIdx.x == 0) partial[row] = f.r;
+#endif
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       if (!mine.any(k)) continue;
@@ -313,7 +319,9 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
         A a = ge;
 #ifdef WEIGHT
         a *= static_cast<A>(wv[k].v[e]);
+#ifndef FEW
         dw[k][e] = cupy::fma_(ge, xe * f.r, dw[k][e]);
+#endif
 #endif
         A v = cupy::fma_(-xe, f.k, a * f.r);
 #ifdef RESIDUAL
@@ -324,7 +332,7 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
       mine.template store<NT_OUT>(k, dx + row * pd, d);
     }
   }
-#ifdef WEIGHT
+#if defined(WEIGHT) && !defined(FEW)
   // the workgroup's share of dw: its groups of lanes are added in order
   if (kRows == 1) {
 #pragma unroll
@@ -437,6 +445,42 @@ cupy_rms_norm_columns(const X_T* g, const X_T* x, A* temp, const long long rows,
   for (long long r = r0; r < r1; ++r)
     t = cupy::fma_(static_cast<A>(g[r * pg + c]), static_cast<A>(x[r * px + c]) * temp[r], t);
   temp[skip + (long long)blockIdx.y * width + c] = t;
+}
+
+// dw of few rows from what the rows were made of, which the caches still hold, and
+// their r: 64 columns by 16 slices of the rows to a workgroup, each slice in order,
+// the slices by a tree (300 x 12000 float16: 14.7 us in all; 27 with partial rows).
+extern "C" __global__ void __launch_bounds__(1024)
+cupy_rms_norm_few(const X_T* g, const X_T* x, const A* row_r, W_T* dw, const int rows,
+                  const int width, const long long pg, const long long px) {
+  constexpr int kAhead = 8, kSlices = 16;
+  __shared__ A lds[kSlices][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, from = c < width ? c : width - 1;
+  A t = A(0);
+  for (int r0 = slice; r0 < rows; r0 += kSlices * kAhead) {
+    X_T gv[kAhead], xv[kAhead];
+    A rv[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int r = r0 + kSlices * k < rows ? r0 + kSlices * k : rows - 1;
+      gv[k] = g[r * pg + from];
+      xv[k] = x[r * px + from];
+      rv[k] = row_r[r];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (r0 + kSlices * k < rows)
+        t = cupy::fma_(static_cast<A>(gv[k]), static_cast<A>(xv[k]) * rv[k], t);
+  }
+  lds[slice][lane] = t;
+  __syncthreads();
+#pragma unroll
+  for (int half = kSlices / 2; half > 0; half >>= 1) {
+    if (slice < half) lds[slice][lane] += lds[slice + half][lane];
+    __syncthreads();
+  }
+  if (slice == 0 && c < width) dw[c] = static_cast<W_T>(lds[0][lane]);
 }
 
 // dw = the sum of the partial rows: 32 columns (a cache line of float32) by 32
@@ -669,6 +713,10 @@ def rms_norm_int8(x, weight=None, residual=None, eps=1e-6, *, out=None, scale_ou
     return _norm(_plans_int8, True, x, weight, residual, eps, out, scale_out, residual_out)
 
 
+def _start_alike(a, b):
+    return isinstance(a, ndarray) and isinstance(b, ndarray) and a.data.ptr == b.data.ptr
+
+
 def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=None,
                   weight_out=None):
     """Gradients of :func:`rms_norm` with respect to its input and weight.
@@ -676,7 +724,8 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     With ``n = x / sqrt(mean(x * x) + eps)`` and ``a = grad * weight``:
     ``dx = (a - n * mean(a * n)) / sqrt(mean(x * x) + eps) + residual_grad`` and
     ``dw = sum of grad * n`` over all rows, in an order that does not change
-    from call to call.
+    from call to call (``dx`` in the place of ``grad`` or ``x`` may have another
+    order than ``dx`` elsewhere).
 
     Args:
         grad (cupy.ndarray): gradient of ``y``, of the shape and type of ``x``.
@@ -707,6 +756,8 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     if weight_out is not None:
         arrays.append(weight_out)
         flags |= 8
+    if weight is not None and (_start_alike(out, grad) or _start_alike(out, x)):
+        flags |= 16
     result, key = _oc.replay(_plans_grad, arrays, (flags, eps))
     if result is not _oc._NOTHING:
         return result
@@ -739,10 +790,20 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     width = x._shape[-1]
     rows = x.size // width if width else 0
     lanes, block, items, vec = _geometry(width, x.dtype.itemsize, 2 if x.dtype.char == 'd' else 4)
-    # rows in registers: written by the threads that have read them.  (Rows
-    # that are walked are read again for dw.)
+    # Workgroups that loop over rows, each with its sums for dw in registers: of
+    # 1536 threads to a unit (16384 x 4096 float16: 102 us; 107 with 2048, 111 to
+    # 114 with 1024), of which each adds a partial row to what is joined.
+    most = _oc.compute_units() * max(1, 1536 // block)
+    # Few long rows, a workgroup to each, none of which has anything to add up: dw
+    # follows from the inputs, unless dx takes their place (float16, 768 x 4096: 16.5
+    # us, 19.5 with partial rows; 700 x 1003 float32: 13.9 and 11.1; 256 x 16384:
+    # 18.2 and 21.8; 400 x 8192: 17.7 and 16.3).
+    few = (weight is not None and items and lanes == block and rows <= most and not flags & 16
+           and width >= rows * (5 if x.dtype.itemsize == 2 else 32))
+    # rows in registers: written by the threads that have read them.  (Where dw
+    # is a second step, that reads the inputs again.)
     places = [(i, i_d) for i in (0, 1, i_r) if i is not None and i_d is not None
-              and (items or weight is None)]
+              and (weight is None or i == i_r or (items and not few))]
     call = _oc.Call(_plans_grad, key, arrays, n_in, places)
     if i_d is None:
         i_d = call.allocate(x._shape, x.dtype)
@@ -770,10 +831,9 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
         if on:
             defines[name] = 1
     acc = _oc.acc_dtype(x.dtype).itemsize
-    # Workgroups that loop over rows, each with its sums for dw in registers: of
-    # 1536 threads to a unit (16384 x 4096 float16: 102 us; 107 with 2048, 111 to
-    # 114 with 1024), of which each adds a partial row to what is joined.
-    grid = max(1, min(-(-rows // (block // lanes)), _oc.compute_units() * max(1, 1536 // block)))
+    if few:
+        defines['FEW'] = 1
+    grid = max(1, min(-(-rows // (block // lanes)), most))
     fn = _GRAD_SOURCE.function('cupy_rms_norm_grad', **defines)
     # the temporary: the rows' r (walked rows only), then the partial sums of dw
     n_partial, skip, run = grid, 0, 0
@@ -784,12 +844,16 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
             blocks = -(-width // 256)
             run = -(-rows // max(1, min(rows, -(-_oc.compute_units() * 8 // blocks), 65535)))
             n_partial, skip = -(-rows // run), rows
-        i_t = call.temp((skip + n_partial * width) * acc)
+        i_t = call.temp((rows if few else skip + n_partial * width) * acc)
     call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
                 Ref(0), Ref(1), Ref(i_w) if i_w is not None else 0,
                 Ref(i_r) if i_r is not None else 0, Ref(i_d), Ref(i_t) if i_t is not None else 0,
                 rows, width, pg, px, pr, pd, eps)
-    if weight is not None:
+    if few:
+        fn = _GRAD_SOURCE.function('cupy_rms_norm_few', **defines)
+        call.launch(fn, (-(-width // 64), 1, 1), 1024, 'PPPPiiqq',
+                    Ref(0), Ref(1), Ref(i_t), Ref(i_dw), rows, width, pg, px)
+    elif weight is not None:
         if not items:
             fn = _GRAD_SOURCE.function('cupy_rms_norm_columns', **defines)
             call.launch(fn, (blocks, n_partial, 1), 256, 'PPPqiqqqq',

@@ -231,6 +231,33 @@ def test_outputs_on_inputs(shape):
         assert np.array_equal(got[1].get(), plain[1].get())
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', [(1, 600), (7, 1000), (50, 4099), (130, 8192)])
+def test_gradient_of_few_long_rows(shape, dtype):
+    """dw from the inputs where dx is written elsewhere, and in the place of each
+    of them, by name and by another view of the same memory; rows apart."""
+    g, x, d = inputs(shape, dtype, 1), inputs(shape, dtype, 2, 2.0), inputs(shape, dtype, 3)
+    w = inputs(shape[-1:], dtype, 4)
+    dx, dw, size, dw_size = grad64(g, x, w, 1e-5)
+    dx, size = dx + d.astype(np.float64), size + np.abs(d.astype(np.float64))
+    u, out = acc_step(dtype), half_step(dtype)
+    off = 1.5 * terms(shape[-1]) + 10
+    wide = cp.zeros((shape[0], shape[1] + 5), dtype)
+    for where in range(8):
+        args = [cp.asarray(a) for a in (g, x, d)]
+        into = (None, args[0], args[1], args[2], args[0][:], args[1].reshape(shape), args[2][:],
+                wide[:, 2:-3])[where]
+        for _ in range(2):
+            for a, b in zip(args, (g, x, d)):
+                a[...] = cp.asarray(b)
+            got, got_w = cp.rms_norm_grad(args[0], args[1], cp.asarray(w), 1e-5, residual_grad=args[2],
+                                          out=into)
+            bound = out * np.abs(dx) + off * u * size + tiny(dtype)
+            assert np.all(np.abs(got.get().astype(np.float64) - dx) <= bound)
+            bound = out * np.abs(dw) + (shape[0] + off) * u * dw_size + tiny(dtype)
+            assert np.all(np.abs(got_w.get().astype(np.float64) - dw) <= bound)
+
+
 def test_streams_and_repeated_calls():
     x, w = inputs((2000, 768), 'float16', 1), inputs((768,), 'float16', 2)
     g = inputs((2000, 768), 'float16', 3)

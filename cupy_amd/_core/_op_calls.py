@@ -161,9 +161,10 @@ def replay(plans, arrays, extra):
     key to record it under (None: not to be recorded).
 
     A plan is ``(spans, record, ret, fast)``: which arrays may not overlap, the
-    launches if addresses are all that changes in them and nothing is allocated
+    launches if addresses are all that changes in them and no result is allocated
     (made again by the extension module without a way back here), the
-    positions of the results, and the recorded call."""
+    positions of the results, the recorded call, and the temporaries if there
+    are any."""
     r = _call(plans, arrays, _device.get_device_id(), _tuning._version, extra,
               _stream.get_current_stream_ptr())
     if type(r) is list:
@@ -175,6 +176,14 @@ def replay(plans, arrays, extra):
     if type(r) is int:
         _rt.check(r)
     return r, None
+
+
+def _temporary(nbytes):
+    """Memory for a call that is made again; None under ``static_scratch``, where
+    the call is replayed by its record."""
+    if _memory._static_scratch_open and _memory.static_scratch_active():
+        return None
+    return _memory.alloc(nbytes)
 
 
 def _span(a):
@@ -312,10 +321,12 @@ class Call:
         if self.rec is not None and self.rec.launches:
             fast = _launch_plan.FastCall(
                 len(self.user), [(a._shape, a.dtype) for a in self.made], self.rec, ret)
-            direct = (not self.made and not self.rec.temps and fast.quick is not None
+            direct = (not self.made and fast.quick is not None
                       and ret is not None and not _dryrun.enabled())
-            _launch_plan.remember(self.plans, self.key, (
-                self._spans, fast.quick[0] if direct else None, ret, fast))
+            plan = self._spans, fast.quick[0] if direct else None, ret, fast
+            if direct and self.rec.temps:
+                plan += ((_temporary, *self.rec.temps),)
+            _launch_plan.remember(self.plans, self.key, plan)
         held = self.user + self.made
         if isinstance(ret, tuple):
             return tuple(held[r] for r in ret)

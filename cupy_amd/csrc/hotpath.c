@@ -449,7 +449,9 @@ static PyObject* hp_overlap(PyObject* self, PyObject* const* args, Py_ssize_t na
 /* call(plans: dict, arrays: list, device id, version, extra: tuple, stream): a recorded call of
  * an operator made again on `arrays`.  `plans` is keyed by the arrays' signature
  * followed by `extra`; a plan is (overlap spec or None, launch record or None,
- * position(s) of the results among the arrays, the recorded call).  Returns
+ * position(s) of the results among the arrays, the recorded call) and, if the
+ * launches use temporaries, (a function that allocates, their sizes ...); where
+ * the function returns None the plan counts as one without a record.  Returns
  *   None                the call has to be made in full and not to be recorded;
  *   [key]               ... and recorded under `key`;
  *   [key, plan]         the plan has no launch record: the caller replays it;
@@ -490,7 +492,10 @@ static PyObject* hp_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
     return out;
   }
   Py_INCREF(plan);
-  if (!PyTuple_Check(plan) || PyTuple_GET_SIZE(plan) != 4) {
+  PyObject* refs = NULL;                 /* the arrays, then the temporaries */
+  const Py_ssize_t parts = PyTuple_Check(plan) ? PyTuple_GET_SIZE(plan) : 0;
+  PyObject* temps = parts == 5 ? PyTuple_GET_ITEM(plan, 4) : NULL;
+  if (parts < 4 || parts > 5 || (temps && (!PyTuple_Check(temps) || !PyTuple_GET_SIZE(temps)))) {
     PyErr_SetString(PyExc_ValueError, "malformed plan");
     goto done;
   }
@@ -510,7 +515,22 @@ static PyObject* hp_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
       goto done;
     }
   }
-  if (!PyBytes_Check(record)) {
+  int replayed = PyBytes_Check(record);
+  const Py_ssize_t n_arrays = PyList_GET_SIZE(arrays);
+  if (replayed && temps) {
+    refs = PyList_GetSlice(arrays, 0, n_arrays);
+    if (!refs) goto done;
+    for (Py_ssize_t i = 1; i < PyTuple_GET_SIZE(temps) && replayed; ++i) {
+      PyObject* memory = PyObject_CallFunctionObjArgs(PyTuple_GET_ITEM(temps, 0),
+                                                      PyTuple_GET_ITEM(temps, i), NULL);
+      if (!memory) goto done;
+      if (memory == Py_None) replayed = 0;
+      const int failed = PyList_Append(refs, memory) < 0;
+      Py_DECREF(memory);
+      if (failed) goto done;
+    }
+  }
+  if (!replayed) {
     out = PyList_New(2);
     if (out) {
       Py_INCREF(key);
@@ -520,7 +540,7 @@ static PyObject* hp_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
     }
     goto done;
   }
-  PyObject* launched = walk_record(record, arrays, (long)PyList_GET_SIZE(arrays), stream, NULL);
+  PyObject* launched = walk_record(record, refs ? refs : arrays, (long)n_arrays, stream, NULL);
   if (!launched) goto done;
   if (PyLong_AsLong(launched) != 0) {
     out = launched;
@@ -545,6 +565,7 @@ static PyObject* hp_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
   }
   if (results) out = results;
 done:
+  Py_XDECREF(refs);
   Py_DECREF(key);
   Py_DECREF(plan);
   return out;

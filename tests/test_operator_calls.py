@@ -431,6 +431,40 @@ def test_recorded_calls_made_by_the_extension():
         _rt.hot.call({}, [a], 0, 0, ())
 
 
+def test_recorded_calls_with_temporaries():
+    """The extension asks for their memory, hands it to the launches behind the
+    arrays, and leaves the call to its record where there is none to be had."""
+    a, b = arr((4, 8)), arr((4, 8))
+    nothing, asked = struct.pack('<II', 0, 0), []
+
+    def allocate(nbytes):
+        asked.append(nbytes)
+        return cp.cuda.alloc(nbytes)
+    plans = {}
+    key = _rt.hot.call(plans, [a, b], 0, 0, (), 0)[0]
+    plans[key] = (None, nothing, 1, None, (allocate, 512, 64))
+    assert _rt.hot.call(plans, [a, b], 0, 0, (), 0) is b and asked == [512, 64]
+    plans[key] = (None, nothing, 1, 'recorded', (lambda nbytes: None, 512, 64))
+    assert _rt.hot.call(plans, [a, b], 0, 0, (), 0)[1][3] == 'recorded'
+    plans[key] = (None, None, 1, 'recorded', (allocate, 512))
+    assert _rt.hot.call(plans, [a, b], 0, 0, (), 0)[1][3] == 'recorded' and len(asked) == 2
+
+    def fail(nbytes):
+        raise MemoryError
+    plans[key] = (None, nothing, 1, None, (fail, 512))
+    with pytest.raises(MemoryError):
+        _rt.hot.call(plans, [a, b], 0, 0, (), 0)
+    for bad in ((None, nothing, 1, None, ()), (None, nothing, 1, None, 512),
+                (None, nothing, 1, None, (allocate, 512), 3)):
+        plans[key] = bad
+        with pytest.raises(ValueError):
+            _rt.hot.call(plans, [a, b], 0, 0, (), 0)
+    # under static_scratch the record's own path is taken
+    assert _op_calls._temporary(100).ptr is not None
+    with cp.cuda.memory.static_scratch():
+        assert _op_calls._temporary(100) is None
+
+
 def test_tables_of_what_needs_preparation():
     def tables(arrays, targets=None, write=True):
         return _global_norm._tables(arrays, targets, write)

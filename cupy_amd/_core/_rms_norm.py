@@ -78,6 +78,8 @@ _CUPY_DEV void sums_of(const cupy::Vec<X_T, N>& x, const cupy::Vec<R_T, N>& res,
 }
 
 #if ITEMS > 0
+// Bound by memory (9001 x 2047 float32 with residual: 50.5 us, 5.8 TB/s; 4096 x
+// 8192 float16 to int8: 48 us, 4.9 TB/s, where two workgroups fill a unit).
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
               const long long rows, const int width, const long long px, const long long pr,
@@ -255,6 +257,8 @@ struct Factors {
 };
 
 #if ITEMS > 0
+// Bound by memory (16384 x 4096 float16 with residual: 97 us, 5.5 TB/s).
+// FEW: every row's r is kept, for dw by a kernel of its own.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
                    A* partial, const long long rows, const int width, const long long pg,
@@ -485,7 +489,7 @@ cupy_rms_norm_few(const X_T* g, const X_T* x, const A* row_r, W_T* dw, const int
 
 // dw = the sum of the partial rows: 32 columns (a cache line of float32) by 32
 // slices of the partial rows to a workgroup; a slice is summed in order, the
-// slices by a tree.
+// slices by a tree.  768 rows of 4096: 4.7 us, three waits in a chain.
 extern "C" __global__ void __launch_bounds__(1024)
 cupy_rms_norm_join(const A* temp, W_T* dw, const long long skip, const int n, const int width) {
   constexpr int kAhead = 8;

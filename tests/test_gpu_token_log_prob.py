@@ -42,7 +42,8 @@ class Exact:
             s = e.sum(-1, keepdims=True)
             self.lse = (m + np.log(s))[..., 0]
             self.p = e / s
-            self.log_p = x - self.lse[..., None]
+            # (not x - lse: rows of the lowest value swallow log s)
+            self.log_p = np.where(np.isneginf(x), x, x - m - np.log(s))
             self.entropy = (np.log(s) + (self.p * d).sum(-1, keepdims=True))[..., 0]
             self.e1 = (self.p * d).sum(-1)
             self.e2 = (self.p * d * d).sum(-1)
@@ -262,6 +263,35 @@ def test_gradient_against_differences():
         e = np.zeros_like(x)
         e[at] = 1e-5
         assert abs((loss(x + e) - loss(x - e)) / 2e-5 - grad[at]) <= 1e-7
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width', [7, 3000, 140001])
+def test_rows_of_the_lowest_value(width, dtype):
+    """All of n equal elements have the log probability -log(n), however large."""
+    low = np.finfo(dtype).min
+    x = np.full((3, width), low, dtype)
+    x[1, 2:] = -np.inf
+    x[2] = -low
+    t = np.array([width - 1, 1, 0])
+    for top in (0, 1, 5):
+        r = cp.token_log_prob(cp.asarray(x), cp.asarray(t), entropy=True, top=top)
+        want = np.log([width, 2, width])
+        # (float16: of 65504, rounded to 32 bits on the way out of 64)
+        assert np.allclose(r.log_prob.get(), -want, rtol=0, atol=1e-4 * (dtype != 'float64') + 1e-9)
+        assert np.allclose(r.entropy.get(), want, rtol=0, atol=1e-4 * (dtype != 'float64') + 1e-9)
+        if top:
+            assert list(r.top_token.get()[0]) == list(range(top))
+            assert np.allclose(r.top_log_prob.get()[0], -want[0], rtol=0, atol=1e-4)
+    g = cp.asarray(np.full(3, 2.0, acc(dtype)))
+    d = cp.token_log_prob_grad(g, cp.asarray(x), cp.asarray(t), r.lse, entropy=r.entropy, entropy_grad=g).get()
+    if dtype == 'float16':
+        # (each p to half a step of lse near 65504, 2^-9, and of the result, 2^-11)
+        want = -2.0 / np.array([width, 2, width])
+        assert np.allclose(d[0, :2], want[0], rtol=5e-3, atol=1e-7) and np.allclose(d[1, 0], want[1], rtol=5e-3)
+        assert np.allclose(d[1, 1], 2 + want[1], rtol=5e-3) and not d[1, 2:].any()
+    else:
+        assert not d[:2].any()
 
 
 @pytest.mark.parametrize('dtype', TYPES)

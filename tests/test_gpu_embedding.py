@@ -137,6 +137,17 @@ def test_gradient(n, rows, width, kind, dtype):
     assert np.array_equal(out.get(), got.get())
 
 
+# the counting of up to 4096, 8192 and 12288 pairs, the first sort behind it; 4, 8 and
+# 16 pairs to a thread of the sort, and more than 64 tiles of the largest kind
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+@pytest.mark.parametrize('n,rows,width', [(4096, 300, 24), (4097, 300, 24), (8192, 200, 24), (8193, 200, 24),
+                                          (12288, 70000, 20), (12289, 70000, 20), (131073, 700, 8),
+                                          (300000, 262150, 4), (600000, 513, 5), (1100000, 70000, 4)])
+@pytest.mark.parametrize('kind', ['spread', 'same', 'falling'])
+def test_gradient_of_many_tokens(n, rows, width, kind, dtype):
+    test_gradient(n, rows, width, kind, dtype)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows,width', [(1, 1), (1, 40000), (70000, 1), (33333, 2), (9000, 7), (4097, 33),
                                         (2500, 509), (700, 4100), (90, 40001)])

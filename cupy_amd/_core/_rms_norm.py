@@ -247,12 +247,14 @@ struct JoinPair {
 };
 
 // With n = x r, a = g w and m = mean(a n):  dx = r (a - n m) = r a - x k,
-// k = r^3 sum(a x) / width;  dw = sum over the rows of g n.
+// k = r^3 sum(a x) / width;  dw = sum over the rows of g n.  The sum is as large as
+// r is small: r is multiplied to it one by one, for r^3 alone leaves the range of
+// float32 from rows of 1e13 (and 1e-13) on, where k does not.
 struct Factors {
   A r, k;
   _CUPY_DEV Factors(const Pair& s, int width, A eps) {
     r = A(1) / cupy::sqrt_(s.square / A(width) + eps);
-    k = r * r * r * (s.dot / A(width));
+    k = r * (r * (r * (s.dot / A(width))));
   }
 };
 

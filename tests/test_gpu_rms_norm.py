@@ -151,6 +151,43 @@ def test_gradient(shape, dtype):
         assert np.all(np.abs(got.get().astype(np.float64) - dx) <= bound)
 
 
+# a row shorter than a vector, rows that share a wave, dw from the inputs, partial rows
+# of dw, rows walked twice
+FORMS = [(3, 5), (300, 64), (7, 1000), (600, 4100), (2, 40001)]
+
+
+def check_scaled_gradient(shape, dtype, power, eps):
+    """Rows of the size 2**power against the formula at the size 1, where nothing
+    leaves the range of float64: dx(s x, eps) = dx(x, eps / s^2) / s, and dw is the
+    same.  ``dx`` is rounded by half a subnormal more where it is one."""
+    s = 2.0 ** power
+    g, x, w = inputs(shape, dtype, 1), inputs(shape, dtype, 2, 2.0), inputs(shape[-1:], dtype, 3)
+    rows = x.size // shape[-1]
+    u, out, off = acc_step(dtype), half_step(dtype), 1.5 * terms(shape[-1]) + 10
+    scaled = np.ldexp(x, power)
+    x = np.ldexp(scaled.astype(np.float64), -power)          # (subnormals have lost bits)
+    for weight in (None, w):
+        dx, dw, size, dw_size = grad64(g, x, weight, eps / s / s)
+        got = cp.rms_norm_grad(cp.asarray(g), cp.asarray(scaled),
+                               None if weight is None else cp.asarray(weight), eps)
+        if weight is not None:
+            got, got_w = got
+            bound = out * np.abs(dw) + (rows + off) * u * dw_size + tiny(dtype)
+            assert np.all(np.abs(got_w.get().astype(np.float64) - dw) <= bound)
+        bound = (out * np.abs(dx) + off * u * size) / s + 2 * tiny(dtype)
+        assert np.all(np.abs(got.get().astype(np.float64) - dx / s) <= bound)
+
+
+@pytest.mark.parametrize('shape', FORMS)
+@pytest.mark.parametrize('dtype,power,eps', [
+    ('float32', 50, 1e-6), ('float32', 54, 1e-6), ('float32', -46, 0.0),
+    ('float64', 430, 1e-6), ('float64', -365, 0.0)])
+def test_gradient_of_large_and_small_rows(shape, dtype, power, eps):
+    """Powers of the inverse root of the mean square (the third enters dx) leave the
+    type's range long before that root, its square and dx do."""
+    check_scaled_gradient(shape, dtype, power, eps)
+
+
 @pytest.mark.parametrize('shape', [(4, 7), (3, 300), (2, 9000)])
 def test_gradient_against_differences(shape):
     """f = sum(c * y) in float64: (f(x + h e) - f(x - h e)) / 2h, h = 1e-5, is off

@@ -313,6 +313,9 @@ def _function(name, dev, t, nbytes):
 def _run(arrays, targets, norm_out, max_norm, eps):
     write = max_norm is not None
     dev = _device.get_device_id()
+    if norm_out is not None:
+        _oc.check_array(norm_out, 'norm_out')
+        _check_peer_access(norm_out, dev)
     finals, aside = arrays if targets is None else targets, ()
     tables = _tables(arrays, targets, write, norm_out)
     if tables is None:

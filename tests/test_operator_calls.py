@@ -207,6 +207,43 @@ def test_the_norm_is_written_beside_what_is_scaled():
     cp.global_norm([flat], norm_out=flat[4:5].reshape(()))        # (read once, before)
 
 
+def elsewhere(a):
+    """An array like ``a`` on another device (never read)."""
+    memory = cp.cuda.memory.UnownedMemory(a.data.ptr, max(a.nbytes, 1), a, a.data.device_id + 1)
+    return cp.ndarray(a.shape, a.dtype, cp.cuda.memory.MemoryPointer(memory, 0))
+
+
+def test_arrays_of_another_device_are_refused():
+    x, w, r, y, h = arr((4, 8)), arr(8), arr((4, 8)), arr((4, 8)), arr((4, 8))
+    q, s, ids, table, n = arr((4, 8), 'int8'), arr(4), arr(4, 'int64'), arr((9, 8)), arr(())
+    stats = [arr(4) for _ in range(5)]
+    top = [arr((4, 2)), arr((4, 2), 'int64')]
+    calls = [
+        (lambda x, w, r, y, h: cp.rms_norm(x, w, r, out=y, residual_out=h), [x, w, r, y, h]),
+        (lambda x, w, r, q, s, h: cp.rms_norm_int8(x, w, r, out=q, scale_out=s, residual_out=h),
+         [x, w, r, q, s, h]),
+        (lambda g, x, w, r, y, d: cp.rms_norm_grad(g, x, w, residual_grad=r, out=y, weight_out=d),
+         [x, r, w, h, y, arr(8)]),
+        (lambda t, i, y: cp.embedding(t, i, out=y), [table, ids, y]),
+        (lambda g, i, t: cp.embedding_grad(g, i, 9, out=t), [y, ids, table]),
+        (lambda x, i, *o: cp.token_log_prob(x, i, entropy=True, top=2, out=cp.TokenLogProb(*o)),
+         [x, ids] + stats[:3] + top),
+        (lambda g, x, i, l, e, d, y: cp.token_log_prob_grad(g, x, i, l, entropy=e, entropy_grad=d, out=y),
+         [stats[0], x, ids, stats[1], stats[2], stats[3], y]),
+        (lambda x, r, n: cp.global_norm([x, r], norm_out=n), [x, r, n]),
+        (lambda x, r, n: cp.clip_by_global_norm([x, r], 1.0, norm_out=n), [x, r, n]),
+        (lambda x, r, y, h, n: cp.clip_by_global_norm([x, r], 1.0, out=[y, h], norm_out=n), [x, r, y, h, n]),
+    ]
+    for call, arrays in calls:
+        for _ in range(2):                        # (the second time beside a record)
+            for k in range(len(arrays)):
+                given = list(arrays)
+                given[k] = elsewhere(given[k])
+                with pytest.raises(ValueError, match='device'):
+                    call(*given)
+            call(*arrays)
+
+
 # -- rows, overlap, descriptions ----------------------------------------------------------
 
 def test_row_form():

@@ -16,6 +16,7 @@ import operator
 
 import numpy
 
+from cupy_amd import _rt
 from cupy_amd._core import _op_calls as _oc
 from cupy_amd._core._op_calls import Ref
 
@@ -743,13 +744,32 @@ def embedding(table, ids, scale=1.0, *, out=None):
     return call.finish(i_out)
 
 
+def _chunk(n, pairs, partial, groups, across):
+    """Sorted pairs that one group of lanes sums: of n, which take ``pairs`` bytes of
+    the temporary beside ``partial`` for each chunk's sums; a workgroup takes
+    ``groups`` chunks, ``across`` workgroups the columns."""
+    # long enough that few runs cross the borders, short enough that there are some
+    # per compute unit
+    chunk = min(128, max(8, _oc.clp2(n // 512)))
+    # ... and so long that ``static_scratch`` holds the temporary, where that leaves
+    # sixteen workgroups to a unit (with eight, 262144 tokens of 4096 float16 take 619 us,
+    # 603 with twice as many)
+    longer = chunk
+    while pairs + -(-n // longer) * partial > _rt.RT_SCRATCH_MAX_BYTES and longer < n:
+        longer *= 2
+    if -(-(-(-n // longer)) // groups) * across >= 16 * _oc.compute_units():
+        chunk = longer
+    return chunk
+
+
 def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     """Gradient of :func:`embedding` with respect to its table.
 
     ``out[v] = scale * (sum of grad[t] over all t with ids[t] == v)``; rows
     that no id selects are zeros, ids outside ``[0, num_rows)`` have no part.
     The sums are held in 32 bits (64 for float64), their order is fixed:
-    repeated calls give the same bits.
+    repeated calls give the same bits.  Under ``cuda.memory.static_scratch``
+    about 8 million ids can be taken (16 bytes for each, and the partial sums).
 
     Args:
         grad (cupy.ndarray): gradient of the looked up rows, of shape
@@ -828,10 +848,6 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
         return call.finish(i_out)
     fill = min(units, -(-num_rows * width // (out_vec * 256)))
 
-    # chunks: long enough that few runs cross their borders, short enough that
-    # there are some per compute unit
-    chunk = min(128, max(8, _oc.clp2(n // 512)))
-    chunks = -(-n // chunk)
     position_bits = max(1, (n - 1).bit_length())
     rank = n <= _RANKED and num_rows.bit_length() + position_bits <= 32
     each = _oc.clp2(-(-n // 4096)) if rank else 1     # (it holds 4096 * each pairs)
@@ -846,6 +862,9 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
     # the temporary: sorted pairs (two copies and counts if sorted by digits), partial sums
     words = 2 * n if rank else 4 * n + tiles * 512
     words += words & 1
+    lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
+    chunk = _chunk(n, words * 4, 2 * width * acc, 256 // lanes, -(-width // (lanes * vec)))
+    chunks = -(-n // chunk)
     i_t = call.temp(words * 4 + chunks * 2 * width * acc)
     defines = dict(G_T=grad.dtype, O_T=dt, I_T=call.refs[1].dtype, ROUNDS=rounds,
                    FILL_VEC=out_vec, EACH=each, NT_OUT=nt_out)
@@ -868,7 +887,6 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
             call.launch(move, (tiles + fill, 1, 1), 1024, 'PPqqqPqIiqiiiII', Ref(1), Ref(i_t), src,
                         at, 4 * n, Ref(i_out), n, num_rows, width, po, p * bits, bits, tiles,
                         cuts[2 * p + 1], cuts[2 * p + 2])
-    lanes = min(256, max(4, _oc.clp2(-(-width // vec))))
     defines = dict(G_T=grad.dtype, O_T=dt, LANES=lanes, VEC=vec, TINY=width < vec)
     fn = _SUMS.function('cupy_embedding_sums', **defines)
     call.launch(fn, (-(-chunks // (256 // lanes)), -(-width // (lanes * vec)), 1), 256,

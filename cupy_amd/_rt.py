@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, '_lib', 'libmi355rt.so')
 RT_ERR_RTC_BASE = 10000
 RT_ERR_POOL_OOM = 20001
 RT_ERR_INVALID = 20002
-RT_SCRATCH_MAX_BYTES = 8 << 20      # size of the library's static scratch array per GPU
+RT_SCRATCH_MAX_BYTES = 128 << 20     # size of the library's static scratch array per GPU
 
 MEMCPY_H2H, MEMCPY_H2D, MEMCPY_D2H, MEMCPY_D2D, MEMCPY_DEFAULT = range(5)
 

@@ -20,7 +20,10 @@
 // allocate.  Every GPU the library runs on holds its own copy until the
 // process ends.  In host code this name is a stand-in, not an address: the
 // address on a device comes from hipGetSymbolAddress (scratch_address below)
-// and only that pointer is ever handed to a kernel.
+// and only that pointer is ever handed to a kernel.  Its size: a reduction's
+// partial results take 8 MiB at most, the partial rows of a norm's weight gradient
+// 32 MiB (one per compute unit of 32768 columns), those of a table's gradient as
+// many as their number is chosen for.
 static __device__ __align__(256) unsigned char scratch[RT_SCRATCH_MAX_BYTES];
 
 namespace {

@@ -182,7 +182,7 @@ int rt_launch_packed_timed(void* function,
  * nothing needs clearing), and two calls that overlap in time on one GPU --
  * different streams or threads -- race on it.
  */
-#define RT_SCRATCH_MAX_BYTES (8u << 20)
+#define RT_SCRATCH_MAX_BYTES (128u << 20)
 #define RT_SCRATCH_MAX_ARG_BLOCK 4096
 int rt_launch_packed_scratch(void* function,
                              unsigned gx, unsigned gy, unsigned gz,

@@ -156,3 +156,51 @@ def test_captured_into_a_graph():
             work()
         stream.synchronize()
         want = [a.get() for a in outs]
+
+
+def test_captured_at_training_sizes():
+    """The gradients of a norm and of a table, whose partial sums take 12.6 and 17.4 MB
+    (34 where a weight has 32768 columns), captured together: every replay, with eager work
+    of the program between them, gives the bits of the calls themselves."""
+    torch = pytest.importorskip('torch')
+    rng = np.random.default_rng(2)
+    cases = []
+    for rows, width, table in ((16384, 1024, 5000), (8192, 4096, 5000), (600, 32768, 300)):
+        g, x = (cp.asarray(rng.standard_normal((rows, width), dtype=np.float32).astype('float16')) for _ in range(2))
+        w = cp.asarray((1 + rng.random(width)).astype('float16'))
+        ids = cp.asarray(rng.integers(-1, table, rows))
+        cases.append((g, x, w, ids, cp.empty_like(x), cp.empty_like(w), cp.empty((table, width), 'float16')))
+
+    def work():
+        for g, x, w, ids, dx, dw, dt in cases:
+            cp.rms_norm_grad(g, x, w, out=dx, weight_out=dw)
+            cp.embedding_grad(dx, ids, len(dt), out=dt)
+
+    stream = cp.cuda.Stream(non_blocking=True)
+    outs = [a for case in cases for a in case[4:]]
+    with stream:
+        work()
+    stream.synchronize()
+    want = [a.get() for a in outs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream.ptr)):
+        graph.capture_begin()
+        try:
+            with stream, cp.cuda.memory.static_scratch():
+                work()
+        finally:
+            graph.capture_end()
+    for k in range(3):
+        for a in outs:
+            a.fill(0)
+        cp.cuda.Stream.null.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, wanted in zip(outs, want):
+            assert np.array_equal(a.get(), wanted)
+        for case in cases:
+            case[0][...] = case[0] * np.float16(-1.5)
+        with stream:
+            work()
+        stream.synchronize()
+        want = [a.get() for a in outs]

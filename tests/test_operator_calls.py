@@ -502,6 +502,37 @@ def test_recorded_calls_with_temporaries():
         assert _op_calls._temporary(100) is None
 
 
+@dry
+def test_training_sizes_run_under_static_scratch():
+    """The temporaries of a step's calls fit the runtime library's static array, up to
+    32768 columns of a norm and millions of tokens; what does not fit says so."""
+    def twice(call):
+        counts = []
+        call()
+        for _ in range(2):
+            _dryrun.launches.clear()
+            with cp.cuda.memory.static_scratch():
+                call()
+            counts.append(len(_dryrun.launches))
+        assert counts[0] == counts[1] > 0
+    for rows, width, kind in ((16384, 4096, 'float16'), (8192, 2048, 'float16'), (4096, 1024, 'float16'),
+                              (100000, 32768, 'float16'), (20000, 16384, 'float32'), (9000, 4096, 'float64'),
+                              (5000, 40001, 'float16'), (3, 1000000, 'float32'), (300, 12000, 'float16')):
+        g, x, w = arr((rows, width), kind), arr((rows, width), kind), arr(width, kind)
+        dx, dw = arr((rows, width), kind), arr(width, kind)
+        twice(lambda: cp.rms_norm_grad(g, x, w, out=dx, weight_out=dw))
+    for n, width, rows, kind in ((16384, 2048, 131072, 'float16'), (8192, 4096, 131072, 'float16'),
+                                 (262144, 4096, 131072, 'float16'), (1 << 20, 2048, 50257, 'float32'),
+                                 (65536, 8192, 32768, 'float32'), (3000000, 512, 50257, 'float32'),
+                                 (4001, 509, 8191, 'float32'), (1000, 178, 9846, 'float32')):
+        g, ids, t = arr((n, width), kind), arr(n, 'int64'), arr((rows, width), kind)
+        twice(lambda: cp.embedding_grad(g, ids, rows, out=t))
+    g, ids, t = arr((10000000, 8), 'float16'), arr(10000000, 'int64'), arr((100, 8), 'float16')
+    cp.embedding_grad(g, ids, 100, out=t)
+    with cp.cuda.memory.static_scratch(), pytest.raises(RuntimeError, match='bytes of scratch'):
+        cp.embedding_grad(g, ids, 100, out=t)
+
+
 def test_tables_of_what_needs_preparation():
     def tables(arrays, targets=None, write=True):
         return _global_norm._tables(arrays, targets, write)

@@ -142,21 +142,29 @@ cupy_square_sums(const Table t, const int entries, double* temp, const long long
   if (threadIdx.x == 0) temp[at + blockIdx.x] = total;
 }
 
+// What elements are multiplied by.  float32: the product is taken in 64 bits, for a
+// factor may lie below the range of float32 where its product with them does not (a
+// norm of 1e40 scaled to 1), and is rounded once.  float16: any factor that a
+// float32 cannot hold takes all of them to 0.
+template <typename T> struct factor_of { typedef double type; };
+template <> struct factor_of<float16> { typedef float type; };
+
 // Bound by memory: the same arrays, 198 us in two launches, 6.1 TB/s.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_scale_arrays(const Table t, const int entries, const int blocks, const double* temp) {
   // last pieces first: they are what the sums have left in the cache
   const unsigned int block = blocks - 1 - blockIdx.x;
   const Entry e = t.e[entry_of(t, entries, block)];
-  const A factor = static_cast<A>(temp[0]);
-  if (factor == A(1) && e.src == e.dst) return;       // what is there is the result
+  typedef factor_of<X_T>::type F;
+  const F factor = static_cast<F>(temp[0]);
+  if (factor == F(1) && e.src == e.dst) return;       // what is there is the result
   Piece p;
   p.load(e, block - e.first);
 #pragma unroll
   for (int k = 0; k < UNROLL; ++k) {
     cupy::Vec<X_T, VEC> r;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) r.v[i] = static_cast<X_T>(static_cast<A>(p.v[k].v[i]) * factor);
+    for (int i = 0; i < VEC; ++i) r.v[i] = static_cast<X_T>(static_cast<F>(p.v[k].v[i]) * factor);
     p.store(e.dst, k, r);
   }
 }
@@ -380,8 +388,8 @@ def global_norm(arrays, *, norm_out=None):
 def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
     """Scales arrays down so that their :func:`global_norm` is ``max_norm`` at most.
 
-    Every array is multiplied by ``min(1, max_norm / (norm + eps))`` and rounded
-    once.  Where the norm is infinite the factor is 0, where it is NaN the
+    Every array is multiplied by ``min(1, max_norm / (norm + eps))``, a factor of 64
+    bits (rounded to 32 for float16 arrays), and rounded once.  Where the norm is infinite the factor is 0, where it is NaN the
     factor is NaN.  Arrays whose norm plus ``eps`` does not exceed ``max_norm``,
     which may be infinite, keep their bits.
 

@@ -112,6 +112,24 @@ def test_large_small_and_missing_values():
     assert not x[0].get().any()
 
 
+def test_factors_below_the_range_of_float32():
+    """What float32 arrays are multiplied by need not be a float32: a norm of 9.5e39
+    scaled to 1e-3, a norm of 1e60 (of a float64 array beside them) to 1e20.  The
+    factor is off by 2^-40, the product is rounded once."""
+    values = np.linspace(-3e38, 3e38, 1001).astype('float32')
+    for beside, bound in (([], 1e-3), ([np.full(3, 1e60)], 1e20)):
+        host = [values] + beside
+        want = norm64(host)
+        dev = [cp.asarray(a) for a in host]
+        outs = [cp.empty_like(a) for a in dev]
+        cp.clip_by_global_norm(dev, bound, out=outs)
+        cp.clip_by_global_norm(dev, bound)
+        for a, o, d in zip(host, outs, dev):
+            exact = a.astype(np.float64) * (bound / (want + 1e-6))
+            assert np.all(np.abs(o.get() - exact) <= (half_step(a.dtype) + 2.0 ** -40) * np.abs(exact))
+            assert np.array_equal(o.get(), d.get())
+
+
 def test_bounds_that_are_met_exactly():
     for values, bound in (([0.0, 0.0], 0.0), ([3.0, 4.0], 5.0), ([3.0, 4.0], np.inf), ([np.inf, 1.0], np.inf)):
         x = cp.asarray(np.array(values, 'float32'))

@@ -228,19 +228,24 @@ def _ranges(arrays, d):
     return start, end
 
 
-def _check_apart(start, end):
+def _check_apart(arrays, start, end):
     """The arrays to write may not share memory with each other."""
     order = numpy.argsort(start, kind='stable')
-    if (start[order][1:] < numpy.maximum.accumulate(end[order])[:-1]).any():
-        raise ValueError('two of the arrays to write overlap in memory')
+    reach = numpy.maximum.accumulate(end[order])
+    for k in numpy.flatnonzero(start[order][1:] < reach[:-1]) + 1:
+        # some array before it goes on behind its beginning
+        for j in range(k):
+            if end[order[j]] > start[order[k]] and _oc.share_elements(arrays[order[j]], arrays[order[k]]):
+                raise ValueError('two of the arrays to write overlap in memory')
 
 
 def _hit_by(src, dst):
-    """Positions of the inputs that share memory with an output other than
-    their own (which may be the very same memory)."""
-    order = numpy.argsort(dst[0], kind='stable')
-    first = numpy.searchsorted(dst[1][order], src[0], 'right')
-    last = numpy.searchsorted(dst[0][order], src[1], 'left')
+    """Positions of the inputs whose range of addresses meets that of an output
+    other than their own (which may be the very same memory)."""
+    # (outputs may lie inside each other's ranges: those that begin before the end of
+    # an input, less those that end before its beginning)
+    first = numpy.searchsorted(numpy.sort(dst[1]), src[0], 'right')
+    last = numpy.searchsorted(numpy.sort(dst[0]), src[1], 'left')
     own = (src[0] == dst[0]) & (src[1] == dst[1])
     return numpy.flatnonzero(last - first > own)
 
@@ -260,7 +265,7 @@ def _prepare(arrays, targets, write):
                 raise ValueError('out[%d] has the shape %r and type %s, expected %r %s'
                                  % (i, b._shape, b.dtype, a._shape, a.dtype))
     ranges = _ranges(finals, dst)
-    _check_apart(*ranges)
+    _check_apart(finals, *ranges)
     reads, writes = list(arrays), list(finals)
     if targets is not None:
         for i in _hit_by(_ranges(arrays, src), ranges):
@@ -366,7 +371,7 @@ def _check_beside(norm_out, arrays):
     _oc.check_array(norm_out, 'norm_out')
     for a in arrays:
         _oc.check_array(a, 'arrays')
-        if _rt.hot.overlap([a, norm_out], _oc._pack_spans([a, norm_out], [(0, 1, False)])):
+        if _oc.share_elements(a, norm_out):
             raise ValueError('norm_out overlaps an array to scale or to write')
 
 

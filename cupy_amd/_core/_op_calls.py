@@ -7,6 +7,7 @@ the same signature (``_launch_plan``: types, shapes, strides, alignment,
 device; never an address).  Otherwise a :class:`Call` checks and converts the
 arrays, launches, and records what it launched.
 """
+import functools
 import struct
 
 import numpy
@@ -198,6 +199,34 @@ def _pack_spans(arrays, pairs):
                        for a, b, same in pairs))
 
 
+class _Geometry:
+    """An array's place in memory, for NumPy to look at and nobody to read."""
+
+    def __init__(self, address, shape, strides, itemsize):
+        self.__array_interface__ = {'version': 3, 'data': (address, True), 'shape': shape,
+                                    'strides': strides, 'typestr': '|V%d' % itemsize}
+
+
+@functools.lru_cache(maxsize=4096)
+def _share(offset, a, b):
+    base = 1 << 60                        # (no address: ``offset`` may be negative)
+    try:
+        return numpy.shares_memory(numpy.asarray(_Geometry(base, *a)),
+                                   numpy.asarray(_Geometry(base + offset, *b)), max_work=1 << 20)
+    except numpy.exceptions.TooHardError:
+        return True
+
+
+def share_elements(a, b):
+    """Whether any byte belongs to elements of both arrays.  Column blocks of one
+    matrix, or its odd and even rows, overlap as ranges of addresses and share
+    nothing.  (A question too hard to answer counts as yes.)"""
+    if not _rt.hot.overlap([a, b], _pack_spans([a, b], [(0, 1, False)])):
+        return False
+    return _share(b.data.ptr - a.data.ptr, (a._shape, a._strides, a.dtype.itemsize),
+                  (b._shape, b._strides, b.dtype.itemsize))
+
+
 class Call:
     """One call made in full.
 
@@ -233,14 +262,16 @@ class Call:
             self._separate()
 
     def _separate(self):
-        """Inputs that overlap an output are copied; outputs have to be apart."""
+        """Inputs that share elements with an output are copied; outputs have to be
+        apart."""
         self.key = None
         for pair in self._pairs:
             i, o, _ = pair
-            if _rt.hot.overlap(self.user, _pack_spans(self.user, [pair])):
+            a, b = self.user[i], self.user[o]
+            if _rt.hot.overlap(self.user, _pack_spans(self.user, [pair])) and share_elements(a, b):
                 if i >= self.n_in:
                     raise ValueError('two outputs of one call overlap in memory')
-                self.refs[i] = self.user[i].copy()
+                self.refs[i] = a.copy()
 
     def convert(self, i, a):
         """The kernels are given ``a`` in the place of array ``i``."""

@@ -171,6 +171,31 @@ def test_results_that_overlap_inputs():
     assert np.allclose(d.get()[:30000], want[0], rtol=1e-6)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_views_beside_each_other(dtype):
+    """Column blocks of one matrix, odd and even rows, every second element, and an
+    array between the elements of another: scaled in place and into views, with the
+    rest left as it was."""
+    host = np.random.default_rng(3).standard_normal((40, 130)).astype(dtype)
+    for cut in ((lambda a: [a[:, :64], a[:, 64:100], a[:, 101:]]), (lambda a: [a[::2], a[1::2, :50]]),
+                (lambda a: [a[:, ::2], a[:, 1::2]]), (lambda a: [a[3::9, 5], a[4, 6:90], a[5:11].T])):
+        parts = cut(host)
+        want = norm64(parts)
+        exact = host.astype(np.float64)
+        for part in cut(exact):
+            part *= 1.0 / (want + 1e-6)
+        bound = ((half_step(dtype) + off([dtype]) + 2.0 ** -24 * (dtype == 'float16')) * np.abs(exact)
+                 + float(np.finfo(dtype).smallest_subnormal) / 2)
+        for place in range(2):
+            d = cp.asarray(host)
+            n = cp.clip_by_global_norm(cut(d) if place else [cp.asarray(p) for p in parts], 1.0, out=cut(d))
+            assert abs(float(n.get()) - want) <= (2.0 ** -24 + off([dtype])) * want
+            assert np.all(np.abs(d.get() - exact) <= bound)
+        d = cp.asarray(host)
+        cp.clip_by_global_norm(cut(d), 1.0)
+        assert np.all(np.abs(d.get() - exact) <= bound)
+
+
 def test_streams():
     arrays = [cp.asarray(a) for a in make([(1000, 300), (17,)] * 5, 'float32', 1)]
     want = cp.global_norm(arrays).get()

@@ -268,6 +268,26 @@ def test_outputs_on_inputs(shape):
         assert np.array_equal(got[1].get(), plain[1].get())
 
 
+@pytest.mark.parametrize('width', [48, 1000, 40000])
+def test_outputs_beside_inputs_and_each_other(width):
+    """Column blocks and odd and even rows of one array: nothing is shared."""
+    x, w, r = inputs((6, width), 'float16', 1), inputs((width,), 'float16', 2), inputs((6, width), 'float16', 3)
+    wd = cp.asarray(w)
+    want, want_h = (a.get() for a in cp.rms_norm(cp.asarray(x), wd, cp.asarray(r)))
+    for place in ((lambda a, k: a[:, 3 + k * (width + 1):][:, :width]),
+                  (lambda a, k: a[:].reshape(-1)[:24 * width].reshape(24, width)[k::4])):
+        for _ in range(2):
+            a = cp.full((6, 4 * (width + 1) + 3), 9, 'float16')
+            xd, rd, y, h = (place(a, k) for k in range(4))
+            xd[...], rd[...] = cp.asarray(x), cp.asarray(r)
+            before = a.get()
+            got = cp.rms_norm(xd, wd, rd, out=y, residual_out=h)
+            assert got[0] is y and got[1] is h
+            assert np.array_equal(y.get(), want) and np.array_equal(h.get(), want_h)
+            y[...], h[...] = 9, 9
+            assert np.array_equal(a.get(), before)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('shape', [(1, 600), (7, 1000), (50, 4099), (130, 8192)])
 def test_gradient_of_few_long_rows(shape, dtype):

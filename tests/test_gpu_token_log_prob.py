@@ -342,6 +342,18 @@ def test_layouts(dtype):
     check(np.tile(base[0], (4, 1)), t[:4], cp.token_log_prob(one, cp.asarray(t[:4]), top=2), 2)
 
 
+@pytest.mark.parametrize('shape', [(1000, 300), (5, 100001)])
+def test_results_in_columns_of_one_array(shape):
+    x, t = logits_of(shape, 'float32', 1), tokens_of(shape)
+    r = cp.full((shape[0], 5), 9, 'float32')
+    out = cp.TokenLogProb(r[:, 0], r[:, 2], r[:, 1], None, None)
+    for _ in range(2):
+        r[...] = 9
+        assert cp.token_log_prob(cp.asarray(x), cp.asarray(t), entropy=True, out=out).lse is out.lse
+        check(x, t, out)
+        assert np.all(r[:, 3:].get() == 9)
+
+
 @pytest.mark.parametrize('width', [60000, 120000])
 def test_streams_and_replays(width):
     x, t = logits_of((6, width), 'float16', 1), tokens_of((6, width))

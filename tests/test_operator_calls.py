@@ -288,6 +288,85 @@ def test_overlap_of_listed_pairs():
         _rt.hot.overlap([1], _op_calls._pack_spans([a], []))
 
 
+def test_sharing_elements_is_decided_exactly():
+    """Views of one piece of memory, against the sets of bytes they touch."""
+    rng = np.random.default_rng(1)
+    flat = arr(4000, 'float16')
+    host = np.arange(8000, dtype=np.int64)
+
+    def view(base, shape, start, steps):
+        return np.lib.stride_tricks.as_strided(base[2 * start:], shape, [16 * t for t in steps])
+    cases = []
+    for _ in range(400):
+        shape = tuple(int(n) for n in rng.integers(1, 7, 2))
+        steps = [int(t) for t in rng.choice([1, 2, 3, 7, 10, 40, -1, -3], 2)]
+        start = 1000 + int(rng.integers(0, 60))
+        first = view(host, shape, start, steps)
+        touched = set(first.ravel()) | set(first.ravel() + 1)
+        a = cp.ndarray(shape, 'float16', flat.data + 2 * start, strides=[2 * t for t in steps])
+        cases.append((a, touched))
+    met = [0, 0]
+    for (a, p), (b, q) in zip(cases[:200], cases[200:]):
+        want = bool(p & q)
+        met[want] += 1
+        assert _op_calls.share_elements(a, b) == _op_calls.share_elements(b, a) == want
+    assert min(met) > 20
+    # of different types: the bytes count
+    assert _op_calls.share_elements(flat[1:2], flat[:4].view('float32')[:1])
+    assert not _op_calls.share_elements(flat[2:3], flat[:4].view('float32')[:1])
+    assert not _op_calls.share_elements(flat[:0], flat)
+
+
+def test_outputs_beside_each_other_are_no_overlap():
+    """Column blocks, odd and even rows, every second element of one array."""
+    a, w = arr((8, 128)), arr(64)
+    x, ids = arr((4, 128)), arr(4, 'int64')
+    for views in ((a[:, :64], a[:, 64:]), (a[:4].reshape(8, 64)[::2], a[:4].reshape(8, 64)[1::2]),
+                  (a[:, ::2], a[:, 1::2])):
+        x1, x2 = arr(views[0].shape), arr(views[0].shape)
+        assert cp.rms_norm(x1, w, x2, out=views[0], residual_out=views[1])[0] is views[0]
+        assert cp.rms_norm(views[0], w, out=views[1]) is views[1]
+        cp.clip_by_global_norm(list(views), 1.0)
+        cp.clip_by_global_norm([x1, x2], 1.0, out=list(views), norm_out=arr(()))
+    r = arr((4, 3))
+    out = cp.TokenLogProb(r[:, 0], r[:, 1], r[:, 2], None, None)
+    assert cp.token_log_prob(x, ids, entropy=True, out=out).lse is out.lse
+    flat = arr(20)
+    cp.clip_by_global_norm([flat[::2]], 1.0, norm_out=flat[5:6].reshape(()))
+    cp.clip_by_global_norm([flat[::9], flat[1:9]], 1.0)
+    # those that do share elements are refused still
+    for views in ((a[:, :65], a[:, 64:]), (a[::2], a[::3]), (a[:, ::2], a[:, 2::2])):
+        with pytest.raises(ValueError):
+            cp.clip_by_global_norm(list(views), 1.0)
+    with pytest.raises(ValueError):
+        cp.rms_norm(arr((8, 64)), w, arr((8, 64)), out=a[:, :64], residual_out=a[:, 63:127])
+    with pytest.raises(ValueError):
+        cp.token_log_prob(x, ids, out=cp.TokenLogProb(r[:, 0], r[:, :2].T[0], None, None, None))
+
+
+@dry
+def test_inputs_beside_an_output_are_not_copied():
+    a, w = arr((8, 128)), arr(64)
+    _dryrun.launches.clear()
+    cp.rms_norm(a[:, :64], w, out=a[:, 64:])
+    assert [l[0] for l in _dryrun.launches] == ['cupy_rms_norm']
+    _dryrun.launches.clear()
+    cp.rms_norm(a[:, :64], w, out=a[:, 63:127])
+    assert len(_dryrun.launches) == 2
+
+
+def test_inputs_inside_the_ranges_of_several_outputs():
+    """Each input of the one is looked for among outputs that lie inside each other's
+    ranges of addresses."""
+    flat = arr(100)
+    src = [flat[90:95], flat[40:50], arr(4)]
+    dst = [flat[0:100:20], flat[1:81:8], flat[60:64]]
+    arrays, targets = [a.ravel() for a in src], dst
+    ranges = [_global_norm._ranges(v, _global_norm._describe(v, 'v')) for v in (arrays, targets)]
+    assert list(_global_norm._hit_by(*ranges)) == [1]
+    assert list(_global_norm._hit_by(ranges[1], ranges[1])) == [0, 1, 2]
+
+
 def test_descriptions():
     a = arr((6, 4), 'float16')
     arrays = [a, a.T, a[:, ::2], arr((), 'float64'), arr((0, 3)), arr(3, 'int32')]

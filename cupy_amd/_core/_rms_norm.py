@@ -8,15 +8,42 @@ reduces, and writes from the same registers.  The reference has no such
 function; in its terms it is the row-wise fusion of
 cupy/_core/_fusion_kernel.pyx:99-115, which takes one kernel per reduction.
 """
+import math
+
 import numpy
 
 from cupy_amd._core import _op_calls as _oc
 from cupy_amd._core._op_calls import Ref
 from cupy_amd._core.core import ndarray
 
-_SOURCE = _oc.Source(r'''
+# Squares of float32 elements leave the range of float32 at 2^64 and 2^-75, and the
+# gradient's powers of r before that.  With RANGED, a row whose sum of squares lies
+# outside what is safe for all of them is taken again, times a power of two: the
+# factor is exact, so that rows of any size have the digits of those in between.
+# (Sums in 64 bits would cost every row what this costs those few: two compares are
+# all that other rows see of it.)  float16 rows never leave the range.
+_RANGE = r'''
 #include <cupy/rows.cuh>
 typedef cupy::acc_of<X_T>::type A;
+
+#ifdef RANGED
+// `low`: 0 where eps is large enough for small sums to have no say in r.  (False for a
+// NaN.)
+_CUPY_DEV bool out_of_range(float square, float low) {
+  return (square > 0x1p80f) | (square < low);
+}
+// The power of two that brings the larger of `top`, the row's largest magnitude, and
+// `root`, the root of eps, near 1; an infinity stays one.
+_CUPY_DEV float scale_for(float top, float root) {
+  const unsigned int b = __builtin_bit_cast(unsigned int, __builtin_fmaxf(top, root)) >> 23;
+  return cupy::from_bits((254u - (b < 1 ? 1 : b > 253 ? 253 : b)) << 23);
+}
+// eps for a row times f
+_CUPY_DEV float scaled_eps(double eps, float f) { return static_cast<float>(eps * f * f); }
+#endif
+'''
+
+_SOURCE = _oc.Source(_RANGE + r'''
 typedef cupy::bits_of<A>::type Bits;
 
 struct Stat { A square; Bits top; };
@@ -35,7 +62,8 @@ typedef signed char Y_T;
 typedef X_T Y_T;
 #endif
 
-// What a row's statistics turn its elements h * weight into.
+// What a row's statistics turn its elements h * weight into (f * h * weight with the
+// statistics of the row times f).
 struct Finish {
   A r, inv, lift;
   A scale;
@@ -77,13 +105,131 @@ _CUPY_DEV void sums_of(const cupy::Vec<X_T, N>& x, const cupy::Vec<R_T, N>& res,
   }
 }
 
+// Rows walked twice, the second time out of the cache, by kLanes lanes each, from the
+// workgroup's row `base` on.  Every element is written by the thread that read it, in
+// the second walk only, so outputs may lie on inputs here too.  A lane adds up what
+// it would add up of a row in registers, in that order.
+// A row that is out of range is walked for its largest magnitude and again, times f,
+// for its statistics.
+template <int kLanes>
+_CUPY_DEV void walk_rows(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
+                         long long base, const long long rows, const int width, const long long px,
+                         const long long pr, const long long py, const long long ps,
+                         const double eps, const float low, const float root,
+                         Stat (&lds)[2][BLOCK / 64], int flip) {
+  constexpr int kRows = BLOCK / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  for (; base < rows; base += (long long)gridDim.x * kRows) {
+    const long long at = base + threadIdx.x / kLanes;
+    const bool valid = kRows == 1 || at < rows;
+    const long long row = valid ? at : rows - 1;
+    A f = A(1), row_eps = static_cast<A>(eps);
+    Stat s;
+    for (bool again = false;; again = true) {
+      s.square = A(0);
+      s.top = 0;
+      for (long long c = lane * VEC; c < width; c += kLanes * VEC) {
+        const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+        const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+        cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+        rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
+#endif
+        A h[VEC];
+        sums_of<VEC>(xv, rv, h);
+        cupy::Vec<W_T, VEC> wv;
+#if defined(INT8) && defined(WEIGHT)
+        wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+#ifdef RANGED
+          h[e] *= f;
+#endif
+          s.square = cupy::fma_(h[e], h[e], s.square);
+#ifdef INT8
+#ifdef WEIGHT
+          const Bits b = cupy::abs_bits(h[e] * static_cast<A>(wv.v[e]));
+#else
+          const Bits b = cupy::abs_bits(h[e]);
+#endif
+          s.top = b > s.top ? b : s.top;
+#endif
+        }
+      }
+      s = cupy::row_allreduce<kLanes, BLOCK>(s, JoinStat(), lds[flip]);
+      flip ^= 1;
+#ifdef RANGED
+      if (again || !out_of_range(s.square, low)) break;
+      Stat t;
+      t.square = A(0);
+      t.top = 0;
+      for (long long c = lane; c < width; c += kLanes) {
+        A h = static_cast<A>(x[row * px + c]);
+#ifdef RESIDUAL
+        h += static_cast<A>(res[row * pr + c]);
+#endif
+        const Bits b = cupy::abs_bits(h);
+        t.top = b > t.top ? b : t.top;
+      }
+      t = cupy::row_allreduce<kLanes, BLOCK>(t, JoinStat(), lds[flip]);
+      flip ^= 1;
+      f = scale_for(cupy::from_bits(t.top), root);
+      row_eps = scaled_eps(eps, f);
+#else
+      break;
+#endif
+    }
+    const Finish fin(s, width, row_eps);
+    if (!valid) continue;
+    for (long long c = lane * VEC; c < width; c += kLanes * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+      rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
+#endif
+      A h[VEC];
+      sums_of<VEC>(xv, rv, h);
+#ifdef RESIDUAL
+      cupy::Vec<R_T, VEC> hv;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) hv.v[e] = static_cast<R_T>(h[e]);
+      cupy::store_part<R_T, VEC>(sum + row * ps + c, hv, have);
+#endif
+#ifdef RANGED
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[e] *= f;
+#endif
+      cupy::Vec<Y_T, VEC> yv;
+#ifdef WEIGHT
+      const cupy::Vec<W_T, VEC> wv = cupy::load_part<W_T, VEC>(w + c, have);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e] * static_cast<A>(wv.v[e]));
+#else
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e]);
+#endif
+      cupy::store_part<Y_T, VEC>(y + row * py + c, yv, have);
+    }
+#ifdef INT8
+    if (lane == 0) scale[row] = static_cast<float>(fin.scale);
+#endif
+  }
+}
+
 #if ITEMS > 0
 // Bound by memory (9001 x 2047 float32 with residual: 50.5 us, 5.8 TB/s; 4096 x
 // 8192 float16 to int8: 48 us, 4.9 TB/s, where two workgroups fill a unit).
+#ifdef WAVES
+extern "C" __global__ void __launch_bounds__(BLOCK, WAVES)
+#else
 extern "C" __global__ void __launch_bounds__(BLOCK)
+#endif
 cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
               const long long rows, const int width, const long long px, const long long pr,
-              const long long py, const long long ps, const double eps) {
+              const long long py, const long long ps, const double eps, const float low,
+              const float root) {
   constexpr int kRows = BLOCK / LANES;
   __shared__ Stat lds[2][BLOCK / 64];
   const cupy::RowShare<ITEMS, LANES, VEC, TINY> mine(threadIdx.x % LANES, width);
@@ -92,8 +238,8 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
   mine.load(wv, w);
 #endif
   int flip = 0;
-  for (long long base = (long long)blockIdx.x * kRows; base < rows;
-       base += (long long)gridDim.x * kRows) {
+  long long base = (long long)blockIdx.x * kRows;
+  for (; base < rows; base += (long long)gridDim.x * kRows) {
     const long long at = base + threadIdx.x / LANES;
     const bool valid = kRows == 1 || at < rows;
     const long long row = valid ? at : rows - 1;
@@ -127,6 +273,11 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
     }
     s = cupy::row_allreduce<LANES, BLOCK>(s, JoinStat(), lds[flip]);
     flip ^= 1;
+#ifdef RANGED
+    // (rows that share a wave go together, and so do all that the wave has left: a way
+    // back would cost the rows in range registers)
+    if (__ballot(out_of_range(s.square, low)) != 0) break;
+#endif
     const Finish fin(s, width, static_cast<A>(eps));
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
@@ -154,88 +305,26 @@ cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, 
     if (valid && threadIdx.x % LANES == 0) scale[row] = static_cast<float>(fin.scale);
 #endif
   }
+#ifdef RANGED
+  walk_rows<LANES>(x, res, w, y, scale, sum, base, rows, width, px, pr, py, ps, eps, low, root, lds,
+                   flip);
+#endif
 }
 #else
-// Rows longer than the registers hold: a workgroup walks its row twice, the
-// second time out of the cache.  Every element is written by the thread that
-// read it, in the second walk only, so outputs may lie on the inputs here too.
+// Rows longer than the registers hold.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_rms_norm(const X_T* x, const R_T* res, const W_T* w, Y_T* y, float* scale, R_T* sum,
               const long long rows, const int width, const long long px, const long long pr,
-              const long long py, const long long ps, const double eps) {
+              const long long py, const long long ps, const double eps, const float low,
+              const float root) {
   __shared__ Stat lds[2][BLOCK / 64];
-  int flip = 0;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    Stat s;
-    s.square = A(0);
-    s.top = 0;
-    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
-      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
-      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
-      cupy::Vec<R_T, VEC> rv;
-#ifdef RESIDUAL
-      rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
-#endif
-      A h[VEC];
-      sums_of<VEC>(xv, rv, h);
-      cupy::Vec<W_T, VEC> wv;
-#if defined(INT8) && defined(WEIGHT)
-      wv = cupy::load_part<W_T, VEC>(w + c, have);
-#endif
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        s.square = cupy::fma_(h[e], h[e], s.square);
-#ifdef INT8
-#ifdef WEIGHT
-        const Bits b = cupy::abs_bits(h[e] * static_cast<A>(wv.v[e]));
-#else
-        const Bits b = cupy::abs_bits(h[e]);
-#endif
-        s.top = b > s.top ? b : s.top;
-#endif
-      }
-    }
-    s = cupy::row_allreduce<BLOCK, BLOCK>(s, JoinStat(), lds[flip]);
-    flip ^= 1;
-    const Finish fin(s, width, static_cast<A>(eps));
-    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
-      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
-      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
-      cupy::Vec<R_T, VEC> rv;
-#ifdef RESIDUAL
-      rv = cupy::load_part<R_T, VEC>(res + row * pr + c, have);
-#endif
-      A h[VEC];
-      sums_of<VEC>(xv, rv, h);
-#ifdef RESIDUAL
-      cupy::Vec<R_T, VEC> hv;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) hv.v[e] = static_cast<R_T>(h[e]);
-      cupy::store_part<R_T, VEC>(sum + row * ps + c, hv, have);
-#endif
-      cupy::Vec<Y_T, VEC> yv;
-#ifdef WEIGHT
-      const cupy::Vec<W_T, VEC> wv = cupy::load_part<W_T, VEC>(w + c, have);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e] * static_cast<A>(wv.v[e]));
-#else
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) yv.v[e] = fin(h[e]);
-#endif
-      cupy::store_part<Y_T, VEC>(y + row * py + c, yv, have);
-    }
-#ifdef INT8
-    if (threadIdx.x == 0) scale[row] = static_cast<float>(fin.scale);
-#endif
-  }
+  walk_rows<BLOCK>(x, res, w, y, scale, sum, blockIdx.x, rows, width, px, pr, py, ps, eps, low, root,
+                   lds, 0);
 }
 #endif
 ''')
 
-_GRAD_SOURCE = _oc.Source(r'''
-#include <cupy/rows.cuh>
-typedef cupy::acc_of<X_T>::type A;
-
+_GRAD_SOURCE = _oc.Source(_RANGE + r'''
 struct Pair { A square, dot; };
 struct JoinPair {
   _CUPY_DEV Pair operator()(const Pair& a, const Pair& b) const {
@@ -249,7 +338,8 @@ struct JoinPair {
 // With n = x r, a = g w and m = mean(a n):  dx = r (a - n m) = r a - x k,
 // k = r^3 sum(a x) / width;  dw = sum over the rows of g n.  The sum is as large as
 // r is small: r is multiplied to it one by one, for r^3 alone leaves the range of
-// float32 from rows of 1e13 (and 1e-13) on, where k does not.
+// float32 from rows of 1e13 (and 1e-13) on, where k does not.  With the sums of a row
+// times f: dx = f (r a - f x k), n = f x r.
 struct Factors {
   A r, k;
   _CUPY_DEV Factors(const Pair& s, int width, A eps) {
@@ -258,13 +348,140 @@ struct Factors {
   }
 };
 
+// What a row's n is made of, in one word: x times r (with the sums of x), or, where
+// f r may be no number of the type, -(f r) 2^-64 or -(f r) 2^64, whichever f is far from.
+_CUPY_DEV A factor_of(A r, A f) {
+#ifdef RANGED
+  if (f > 0x1p100f) return -(f * 0x1p-64f * r);
+  if (f < 0x1p-100f) return -(f * 0x1p64f * r);
+#endif
+  return f * r;
+}
+_CUPY_DEV A normalised(X_T x, A factor) {
+#ifdef RANGED
+  const A by = factor < A(0) ? (factor > A(-1) ? A(0x1p-64f) : A(0x1p64f)) : A(1);
+  return static_cast<A>(x) * by * cupy::abs_(factor);
+#else
+  return static_cast<A>(x) * factor;
+#endif
+}
+
+#ifdef RANGED
+struct LargerSquare {
+  _CUPY_DEV Pair operator()(const Pair& a, const Pair& b) const {
+    return a.square > b.square ? a : b;
+  }
+};
+// (also where only the products with a are too large)
+_CUPY_DEV bool out_of_range(const Pair& s, float low) {
+  return out_of_range(s.square, low) | !(cupy::abs_(s.dot) < __builtin_inff());
+}
+#endif
+
+// Rows walked twice by the whole workgroup, from its row `base` on: a thread adds up
+// what it would of a row in registers, in that order, and writes what it read.  A row
+// that is out of range is walked for its largest magnitude and again, times f.
+// `factors` (if any) receives what the rows' n are made of, `dw` (if any) is added to.
+_CUPY_DEV void walk_rows(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
+                         A* factors, A* dw, long long base, const long long rows, const int width,
+                         const long long pg, const long long px, const long long pr,
+                         const long long pd, const double eps, const float low, const float root,
+                         Pair (&lds)[2][BLOCK / 64], int flip) {
+  for (long long row = base; row < rows; row += gridDim.x) {
+    A f = A(1), row_eps = static_cast<A>(eps);
+    Pair s;
+    for (bool again = false;; again = true) {
+      s.square = s.dot = A(0);
+      for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+        const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+        const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+        const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
+        cupy::Vec<W_T, VEC> wv;
+#ifdef WEIGHT
+        wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+#ifdef RANGED
+          const A xe = static_cast<A>(xv.v[e]) * f;
+#else
+          const A xe = static_cast<A>(xv.v[e]);
+#endif
+          A a = static_cast<A>(gv.v[e]);
+#ifdef WEIGHT
+          a *= static_cast<A>(wv.v[e]);
+#endif
+          s.square = cupy::fma_(xe, xe, s.square);
+          s.dot = cupy::fma_(a, xe, s.dot);
+        }
+      }
+      s = cupy::row_allreduce<BLOCK, BLOCK>(s, JoinPair(), lds[flip]);
+      flip ^= 1;
+#ifdef RANGED
+      if (again || !out_of_range(s, low)) break;
+      Pair t;
+      t.square = t.dot = A(0);
+      for (long long c = threadIdx.x; c < width; c += BLOCK) {
+        const A m = cupy::abs_(static_cast<A>(x[row * px + c]));
+        t.square = m > t.square ? m : t.square;
+      }
+      t = cupy::row_allreduce<BLOCK, BLOCK>(t, LargerSquare(), lds[flip]);
+      flip ^= 1;
+      f = scale_for(t.square, root);
+      row_eps = scaled_eps(eps, f);
+#else
+      break;
+#endif
+    }
+    const Factors fac(s, width, row_eps);
+    if (factors && threadIdx.x == 0) factors[row] = factor_of(fac.r, f);
+    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
+      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
+      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
+      const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
+      cupy::Vec<W_T, VEC> wv;
+#ifdef WEIGHT
+      wv = cupy::load_part<W_T, VEC>(w + c, have);
+#endif
+      cupy::Vec<R_T, VEC> rv;
+#ifdef RESIDUAL
+      rv = cupy::load_part<R_T, VEC>(dres + row * pr + c, have);
+#endif
+      cupy::Vec<X_T, VEC> d;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        A xe = static_cast<A>(xv.v[e]);
+        const A ge = static_cast<A>(gv.v[e]);
+        A a = ge;
+#ifdef WEIGHT
+        a *= static_cast<A>(wv.v[e]);
+#endif
+#ifdef RANGED
+        xe *= f;
+        if (dw && e < have) dw[c + e] = cupy::fma_(ge, xe * fac.r, dw[c + e]);
+#endif
+        A v = cupy::fma_(-xe, fac.k, a * fac.r);
+#ifdef RANGED
+        v *= f;
+#endif
+#ifdef RESIDUAL
+        v += static_cast<A>(rv.v[e]);
+#endif
+        d.v[e] = static_cast<X_T>(v);
+      }
+      cupy::store_part<X_T, VEC>(dx + row * pd + c, d, have);
+    }
+  }
+}
+
 #if ITEMS > 0
 // Bound by memory (16384 x 4096 float16 with residual: 97 us, 5.5 TB/s).
-// FEW: every row's r is kept, for dw by a kernel of its own.
+// FEW: what every row's n is made of is kept, for dw by a kernel of its own.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
                    A* partial, const long long rows, const int width, const long long pg,
-                   const long long px, const long long pr, const long long pd, const double eps) {
+                   const long long px, const long long pr, const long long pd, const double eps,
+                   const float low, const float root) {
   constexpr int kRows = BLOCK / LANES;
   __shared__ Pair lds[2][BLOCK / 64];
   const int lane = threadIdx.x % LANES;
@@ -281,8 +498,8 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
 #endif
 #endif
   int flip = 0;
-  for (long long base = (long long)blockIdx.x * kRows; base < rows;
-       base += (long long)gridDim.x * kRows) {
+  long long base = (long long)blockIdx.x * kRows;
+  for (; base < rows; base += (long long)gridDim.x * kRows) {
     const long long at = base + threadIdx.x / LANES;
     const bool valid = kRows == 1 || at < rows;
     const long long row = valid ? at : rows - 1;
@@ -310,8 +527,40 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
     }
     s = cupy::row_allreduce<LANES, BLOCK>(s, JoinPair(), lds[flip]);
     flip ^= 1;
+    A scale = A(1), row_eps = static_cast<A>(eps);
+#ifdef RANGED
+    if (LANES > 64) {
+      // (all that the workgroup has left is walked: a way back would cost the rows in
+      // range registers)
+      if (__ballot(out_of_range(s, low)) != 0) break;
+    } else if (__builtin_expect(out_of_range(s, low), 0)) {
+      // (a lane holds one vector of the row)
+      Pair t;
+      t.square = t.dot = A(0);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A m = mine.owns(0, e) ? cupy::abs_(static_cast<A>(xv[0].v[e])) : A(0);
+        t.square = m > t.square ? m : t.square;
+      }
+      t = cupy::row_allreduce<LANES, BLOCK>(t, LargerSquare(), lds[flip]);
+      scale = scale_for(t.square, root);
+      row_eps = scaled_eps(eps, scale);
+      s.square = s.dot = A(0);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const A xe = mine.owns(0, e) ? static_cast<A>(xv[0].v[e]) * scale : A(0);
+        A a = mine.owns(0, e) ? static_cast<A>(gv[0].v[e]) : A(0);
+#ifdef WEIGHT
+        a = mine.owns(0, e) ? a * static_cast<A>(wv[0].v[e]) : A(0);
+#endif
+        s.square = cupy::fma_(xe, xe, s.square);
+        s.dot = cupy::fma_(a, xe, s.dot);
+      }
+      s = cupy::row_allreduce<LANES, BLOCK>(s, JoinPair(), lds[flip]);
+    }
+#endif
     if (!valid) continue;
-    const Factors f(s, width, static_cast<A>(eps));
+    const Factors f(s, width, row_eps);
 #ifdef FEW
     if (threadIdx.x == 0) partial[row] = f.r;
 #endif
@@ -321,7 +570,11 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
       cupy::Vec<X_T, VEC> d;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const A xe = static_cast<A>(xv[k].v[e]), ge = static_cast<A>(gv[k].v[e]);
+        A xe = static_cast<A>(xv[k].v[e]);
+        const A ge = static_cast<A>(gv[k].v[e]);
+#ifdef RANGED
+        if (LANES <= 64) xe *= scale;
+#endif
         A a = ge;
 #ifdef WEIGHT
         a *= static_cast<A>(wv[k].v[e]);
@@ -330,6 +583,9 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
 #endif
 #endif
         A v = cupy::fma_(-xe, f.k, a * f.r);
+#ifdef RANGED
+        if (LANES <= 64) v *= scale;
+#endif
 #ifdef RESIDUAL
         v += static_cast<A>(rv[k].v[e]);
 #endif
@@ -367,78 +623,37 @@ cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_
     }
   }
 #endif
+#ifdef RANGED
+  if (LANES > 64) {
+#if defined(FEW)
+    A *factors = partial, *sums = nullptr;
+#elif defined(WEIGHT)
+    // (every column's sum is one thread's, here and above)
+    A *factors = nullptr, *sums = partial + (long long)blockIdx.x * width;
+#else
+    A *factors = nullptr, *sums = nullptr;
+#endif
+    walk_rows(g, x, w, dres, dx, factors, sums, base, rows, width, pg, px, pr, pd, eps, low, root,
+              lds, flip);
+  }
+#endif
 }
 #else
-// Rows longer than the registers hold: walked twice; every row's r is kept
-// for the sums down the columns, which a kernel of their own makes.
+// Rows longer than the registers hold; what their n are made of is kept for the sums
+// down the columns, which a kernel of their own makes.
 extern "C" __global__ void __launch_bounds__(BLOCK)
 cupy_rms_norm_grad(const X_T* g, const X_T* x, const W_T* w, const R_T* dres, X_T* dx,
-                   A* row_r, const long long rows, const int width, const long long pg,
-                   const long long px, const long long pr, const long long pd, const double eps) {
+                   A* factors, const long long rows, const int width, const long long pg,
+                   const long long px, const long long pr, const long long pd, const double eps,
+                   const float low, const float root) {
   __shared__ Pair lds[2][BLOCK / 64];
-  int flip = 0;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    Pair s;
-    s.square = s.dot = A(0);
-    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
-      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
-      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
-      const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
-      cupy::Vec<W_T, VEC> wv;
-#ifdef WEIGHT
-      wv = cupy::load_part<W_T, VEC>(w + c, have);
-#endif
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const A xe = static_cast<A>(xv.v[e]);
-        A a = static_cast<A>(gv.v[e]);
-#ifdef WEIGHT
-        a *= static_cast<A>(wv.v[e]);
-#endif
-        s.square = cupy::fma_(xe, xe, s.square);
-        s.dot = cupy::fma_(a, xe, s.dot);
-      }
-    }
-    s = cupy::row_allreduce<BLOCK, BLOCK>(s, JoinPair(), lds[flip]);
-    flip ^= 1;
-    const Factors f(s, width, static_cast<A>(eps));
-#ifdef WEIGHT
-    if (threadIdx.x == 0) row_r[row] = f.r;
-#endif
-    for (long long c = (long long)threadIdx.x * VEC; c < width; c += BLOCK * VEC) {
-      const int have = width - c < VEC ? static_cast<int>(width - c) : VEC;
-      const cupy::Vec<X_T, VEC> xv = cupy::load_part<X_T, VEC>(x + row * px + c, have);
-      const cupy::Vec<X_T, VEC> gv = cupy::load_part<X_T, VEC>(g + row * pg + c, have);
-      cupy::Vec<W_T, VEC> wv;
-#ifdef WEIGHT
-      wv = cupy::load_part<W_T, VEC>(w + c, have);
-#endif
-      cupy::Vec<R_T, VEC> rv;
-#ifdef RESIDUAL
-      rv = cupy::load_part<R_T, VEC>(dres + row * pr + c, have);
-#endif
-      cupy::Vec<X_T, VEC> d;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const A xe = static_cast<A>(xv.v[e]);
-        A a = static_cast<A>(gv.v[e]);
-#ifdef WEIGHT
-        a *= static_cast<A>(wv.v[e]);
-#endif
-        A v = cupy::fma_(-xe, f.k, a * f.r);
-#ifdef RESIDUAL
-        v += static_cast<A>(rv.v[e]);
-#endif
-        d.v[e] = static_cast<X_T>(v);
-      }
-      cupy::store_part<X_T, VEC>(dx + row * pd + c, d, have);
-    }
-  }
+  walk_rows(g, x, w, dres, dx, factors, nullptr, blockIdx.x, rows, width, pg, px, pr, pd, eps, low,
+            root, lds, 0);
 }
 #endif
 
 // Partial sum of dw over the p-th run of rows, a thread per column: the first
-// `skip` words of `temp` are the rows' r, the partial sums follow.
+// `skip` words of `temp` are what the rows' n are made of, the partial sums follow.
 extern "C" __global__ void __launch_bounds__(256)
 cupy_rms_norm_columns(const X_T* g, const X_T* x, A* temp, const long long rows,
                       const int width, const long long pg, const long long px,
@@ -449,15 +664,15 @@ cupy_rms_norm_columns(const X_T* g, const X_T* x, A* temp, const long long rows,
   const long long r1 = r0 + run < rows ? r0 + run : rows;
   A t = A(0);
   for (long long r = r0; r < r1; ++r)
-    t = cupy::fma_(static_cast<A>(g[r * pg + c]), static_cast<A>(x[r * px + c]) * temp[r], t);
+    t = cupy::fma_(static_cast<A>(g[r * pg + c]), normalised(x[r * px + c], temp[r]), t);
   temp[skip + (long long)blockIdx.y * width + c] = t;
 }
 
 // dw of few rows from what the rows were made of, which the caches still hold, and
-// their r: 64 columns by 16 slices of the rows to a workgroup, each slice in order,
+// their factors: 64 columns by 16 slices of the rows to a workgroup, each slice in order,
 // the slices by a tree (300 x 12000 float16: 14.7 us in all; 27 with partial rows).
 extern "C" __global__ void __launch_bounds__(1024)
-cupy_rms_norm_few(const X_T* g, const X_T* x, const A* row_r, W_T* dw, const int rows,
+cupy_rms_norm_few(const X_T* g, const X_T* x, const A* factors, W_T* dw, const int rows,
                   const int width, const long long pg, const long long px) {
   constexpr int kAhead = 8, kSlices = 16;
   __shared__ A lds[kSlices][64];
@@ -472,12 +687,12 @@ cupy_rms_norm_few(const X_T* g, const X_T* x, const A* row_r, W_T* dw, const int
       const int r = r0 + kSlices * k < rows ? r0 + kSlices * k : rows - 1;
       gv[k] = g[r * pg + from];
       xv[k] = x[r * px + from];
-      rv[k] = row_r[r];
+      rv[k] = factors[r];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (r0 + kSlices * k < rows)
-        t = cupy::fma_(static_cast<A>(gv[k]), static_cast<A>(xv[k]) * rv[k], t);
+        t = cupy::fma_(static_cast<A>(gv[k]), normalised(xv[k], rv[k]), t);
   }
   lds[slice][lane] = t;
   __syncthreads();
@@ -546,6 +761,11 @@ def _geometry(width, itemsize, most_items):
     if items > most_items:
         return 1024, 1024, 0, vec
     return lanes, lanes, items, vec
+
+
+def _range_of(eps):
+    """(smallest sum of squares that is safe, root of eps) for the kernels of float32 rows."""
+    return 2.0 ** -60 if eps < 2.0 ** -40 else 0.0, min(math.sqrt(eps), 1e38) if eps > 0 else 0.0
 
 
 def _check(x, weight, residual, what):
@@ -655,10 +875,20 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
                    ITEMS=items, VEC=vec, TINY=width < vec, NT_IN=nt_in, NT_OUT=nt_out,
                    # (8 bits fit the cache where the rest does not)
                    NT_Y=nt_out and not int8)
+    ranged = 'f' in (x.dtype.char, defines['R_T'].char)
     for name, on in (('INT8', int8), ('WEIGHT', weight is not None),
-                     ('RESIDUAL', residual is not None)):
+                     ('RESIDUAL', residual is not None), ('RANGED', ranged)):
         if on:
             defines[name] = 1
+    # The walks may not cost the rows in registers the second workgroup on a unit: the
+    # compiler is asked for two where a lane holds few enough words of x, the weight and
+    # the residual (16384 x 4096 float32 to int8: 134 us, 156 unasked; 300 x 12000: 10.6
+    # and 11.1; but 400 x 16384 with residual, 48 words: 19.5 and 18.5, for some spill).
+    held = items * vec * (x.dtype.itemsize
+                          + (weight.dtype.itemsize if weight is not None else 0)
+                          + (residual.dtype.itemsize if residual is not None else 0)) // 4
+    if ranged and block > 512 and 0 < held <= 40:
+        defines['WAVES'] = -(-2 * block // 256)
     fn = _SOURCE.function('cupy_rms_norm', **defines)
     # A workgroup per row (or 256 / lanes of them): stores run fastest without a
     # loop around them.  Of those of more than 512 threads a unit holds two: they
@@ -670,10 +900,10 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
     if block > 512 and grid >= 0.95 * rounds * resident:
         grid = min(grid, resident)
     grid = min(grid, 0xffffffff // block)
-    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
+    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqdff',
                 Ref(0), Ref(i_r) if i_r is not None else 0, Ref(i_w) if i_w is not None else 0,
                 Ref(i_y), Ref(i_s) if int8 else 0, Ref(i_h) if i_h is not None else 0,
-                rows, width, px, pr, py, ps, eps)
+                rows, width, px, pr, py, ps, eps, *_range_of(eps))
     out = call.finish(ret if len(ret) > 1 else ret[0])
     return out
 
@@ -684,6 +914,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, *, out=None, residual_out=
     ``y = h / sqrt(mean(h * h) + eps) * weight`` with ``h = x + residual``
     (``h = x`` without a residual).  Sums are held in 32 bits for float16 and
     float32 (64 for float64); ``y`` is rounded once, from the unrounded ``h``.
+    Finite rows of float16 and float32 may be of any size; the squares of float64
+    rows have to stay in its range.
 
     Args:
         x (cupy.ndarray): float16, float32 or float64, of one dimension or more.
@@ -731,7 +963,8 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     ``dx = (a - n * mean(a * n)) / sqrt(mean(x * x) + eps) + residual_grad`` and
     ``dw = sum of grad * n`` over all rows, in an order that does not change
     from call to call (``dx`` in the place of ``grad`` or ``x`` may have another
-    order than ``dx`` elsewhere).
+    order than ``dx`` elsewhere).  Rows may be as large and small as in the forward
+    call.
 
     Args:
         grad (cupy.ndarray): gradient of ``y``, of the shape and type of ``x``.
@@ -833,7 +1066,8 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     defines = dict(X_T=x.dtype, R_T=x.dtype if residual_grad is None else residual_grad.dtype,
                    W_T=x.dtype if weight is None else weight.dtype, LANES=lanes, BLOCK=block,
                    ITEMS=items, VEC=vec, TINY=width < vec, NT_IN=nt_in, NT_OUT=nt_out)
-    for name, on in (('WEIGHT', weight is not None), ('RESIDUAL', residual_grad is not None)):
+    for name, on in (('WEIGHT', weight is not None), ('RESIDUAL', residual_grad is not None),
+                     ('RANGED', x.dtype.char == 'f')):
         if on:
             defines[name] = 1
     acc = _oc.acc_dtype(x.dtype).itemsize
@@ -841,7 +1075,7 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
         defines['FEW'] = 1
     grid = max(1, min(-(-rows // (block // lanes)), most))
     fn = _GRAD_SOURCE.function('cupy_rms_norm_grad', **defines)
-    # the temporary: the rows' r (walked rows only), then the partial sums of dw
+    # the temporary: a word for each row (walked rows only), then the partial sums of dw
     n_partial, skip, run = grid, 0, 0
     i_t = None
     if weight is not None:
@@ -851,10 +1085,10 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
             run = -(-rows // max(1, min(rows, -(-_oc.compute_units() * 8 // blocks), 65535)))
             n_partial, skip = -(-rows // run), rows
         i_t = call.temp((rows if few else skip + n_partial * width) * acc)
-    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqd',
+    call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqdff',
                 Ref(0), Ref(1), Ref(i_w) if i_w is not None else 0,
                 Ref(i_r) if i_r is not None else 0, Ref(i_d), Ref(i_t) if i_t is not None else 0,
-                rows, width, pg, px, pr, pd, eps)
+                rows, width, pg, px, pr, pd, eps, *_range_of(eps))
     if few:
         fn = _GRAD_SOURCE.function('cupy_rms_norm_few', **defines)
         call.launch(fn, (-(-width // 64), 1, 1), 1024, 'PPPPiiqq',

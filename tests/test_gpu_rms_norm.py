@@ -153,13 +153,15 @@ def test_gradient(shape, dtype):
 
 # a row shorter than a vector, rows that share a wave, dw from the inputs, partial rows
 # of dw, rows walked twice
-FORMS = [(3, 5), (300, 64), (7, 1000), (600, 4100), (2, 40001)]
+FORMS = [(4, 1), (4, 3), (3, 5), (300, 64), (7, 1000), (600, 4100), (2, 40001)]
 
 
 def check_scaled_gradient(shape, dtype, power, eps):
     """Rows of the size 2**power against the formula at the size 1, where nothing
     leaves the range of float64: dx(s x, eps) = dx(x, eps / s^2) / s, and dw is the
-    same.  ``dx`` is rounded by half a subnormal more where it is one."""
+    same.  dx is compared times s, for where it is subnormal it is off by half of the
+    smallest subnormal more (and the bound has room for as much again): in float64
+    2^-1075, which float64 itself holds only times s."""
     s = 2.0 ** power
     g, x, w = inputs(shape, dtype, 1), inputs(shape, dtype, 2, 2.0), inputs(shape[-1:], dtype, 3)
     rows = x.size // shape[-1]
@@ -174,8 +176,8 @@ def check_scaled_gradient(shape, dtype, power, eps):
             got, got_w = got
             bound = out * np.abs(dw) + (rows + off) * u * dw_size + tiny(dtype)
             assert np.all(np.abs(got_w.get().astype(np.float64) - dw) <= bound)
-        bound = (out * np.abs(dx) + off * u * size) / s + 2 * tiny(dtype)
-        assert np.all(np.abs(got.get().astype(np.float64) - dx / s) <= bound)
+        bound = out * np.abs(dx) + off * u * size + float(np.finfo(dtype).smallest_subnormal) * s
+        assert np.all(np.abs(np.ldexp(got.get().astype(np.float64), power) - dx) <= bound)
 
 
 @pytest.mark.parametrize('shape', FORMS)
@@ -186,6 +188,121 @@ def test_gradient_of_large_and_small_rows(shape, dtype, power, eps):
     """Powers of the inverse root of the mean square (the third enters dx) leave the
     type's range long before that root, its square and dx do."""
     check_scaled_gradient(shape, dtype, power, eps)
+
+
+@pytest.mark.parametrize('shape', FORMS)
+@pytest.mark.parametrize('dtype,power,eps', [
+    ('float32', 40, 1e-6), ('float32', 70, 1e-6), ('float32', 124, 1e-6), ('float32', -35, 0.0),
+    ('float32', -80, 0.0), ('float32', -80, 1e-40), ('float32', -80, 1e-60), ('float32', -120, 0.0)])
+def test_gradient_of_rows_of_any_size(shape, dtype, power, eps):
+    """The squares themselves leave the type's range."""
+    check_scaled_gradient(shape, dtype, power, eps)
+
+
+@pytest.mark.parametrize('shape', FORMS + [(9, 2047)])
+@pytest.mark.parametrize('dtype,power,eps', [
+    ('float32', 70, 1e-6), ('float32', 124, 1e-6), ('float32', -80, 0.0), ('float32', -80, 1e-40),
+    ('float32', -80, 1e-60), ('float32', -130, 0.0), ('float32', -30, 0.0)])
+def test_rows_of_any_size(shape, dtype, power, eps):
+    """y of rows times s and eps times s^2 is y of the rows; the scale of the 8 bits as
+    well.  Rows of every size side by side, zeros and an infinity among them."""
+    s = 2.0 ** power
+    x, w, r = inputs(shape, dtype, 1), inputs(shape[-1:], dtype, 2), inputs(shape, dtype, 3)
+    plain = np.arange(shape[0]) % 5 == 3                    # rows of the ordinary size
+    powers = np.where(plain, 0, power)[:, None]
+    xs, rs = np.ldexp(x, powers), np.ldexp(r, powers)
+    one = np.ldexp(1.0, -powers)
+    h64 = xs.astype(np.float64) * one + rs.astype(np.float64) * one
+    eps64 = np.where(plain, eps, eps / s / s)[:, None]
+    want = norm64(h64, w, eps64)
+    xd, rd, wd = cp.asarray(xs), cp.asarray(rs), cp.asarray(w)
+    y, h = cp.rms_norm(xd, wd, rd, eps)
+    check_norm(y.get(), want, shape[-1], dtype)
+    assert np.all(np.abs(h.get().astype(np.float64) * one - h64)
+                  <= half_step(dtype) * np.abs(h64) * 1.001 + tiny(dtype) * one)
+    h64 = xs.astype(np.float64) * one
+    check_norm(cp.rms_norm(xd, wd, eps=eps).get(), norm64(h64, w, eps64), shape[-1], dtype)
+    q, s_, _ = (a.get().astype(np.float64) for a in cp.rms_norm_int8(xd, wd, rd, eps))
+    step = np.abs(want).max(-1) / 127
+    off = (terms(shape[-1]) / 2 + 10) * acc_step(dtype)
+    assert np.all(np.abs(s_ - step) <= (off + half_step('float32')) * step)
+    assert np.all(np.abs(q - want / step[:, None]) <= 0.5 + 127 * off)
+    assert np.all(np.abs(q).max(-1) == 127)
+
+
+@pytest.mark.parametrize('shape', [(1030, 3), (5000, 64), (3000, 1003), (1536, 4096), (300, 12000), (700, 33000)])
+def test_rows_of_all_sizes_side_by_side(shape):
+    """Few rows in between that leave the range, where workgroups take several: the
+    others have the bits that they have among themselves, and dw holds all of them."""
+    rng = np.random.default_rng(5)
+    powers = np.where(rng.random(shape[0]) < 0.02, rng.choice([-80, 40, 70, 120], shape[0]), 0)
+    powers[[0, -1]] = 70, -80
+    plain, s = powers == 0, np.ldexp(1.0, powers)[:, None]
+    x, g, d = (inputs(shape, 'float32', k) for k in range(3))
+    w = inputs(shape[-1:], 'float32', 3)
+    xs, ds = np.ldexp(x, powers[:, None]), np.ldexp(d, powers[:, None])
+    wd, eps = cp.asarray(w), 1e-60
+    # in the place of the inputs
+    for q8 in (False, True):
+        want = cp.rms_norm(cp.asarray(x), wd, cp.asarray(d), eps)[0].get()
+        xd, dd = cp.asarray(xs), cp.asarray(ds)
+        if q8:
+            want = [a.get() for a in cp.rms_norm_int8(cp.asarray(x), wd, cp.asarray(d), eps)]
+            q, sc, h = cp.rms_norm_int8(xd, wd, dd, eps, residual_out=dd)
+            assert np.array_equal(q.get()[plain], want[0][plain])
+            assert np.array_equal(sc.get()[plain], want[1][plain])
+            # (every step is exact but the sum's own rounding: the same 8 bits)
+            assert np.array_equal(q.get(), want[0])
+        else:
+            y, h = cp.rms_norm(xd, wd, dd, eps, out=xd, residual_out=dd)
+            assert y is xd and h is dd
+            assert np.array_equal(y.get()[plain], want[plain])
+            h64 = (xs.astype(np.float64) + ds.astype(np.float64)) / s
+            check_norm(y.get(), norm64(h64, w, eps / s / s), shape[-1], 'float32')
+    u, off = acc_step('float32'), 1.5 * terms(shape[-1]) + 10
+    dx, dw, size, dw_size = grad64(g, x, w, eps / s / s)
+    want, _ = (a.get() for a in cp.rms_norm_grad(cp.asarray(g), cp.asarray(x), wd, eps))
+    for place in range(3):
+        gd, xd = cp.asarray(g), cp.asarray(xs)
+        got, got_w = cp.rms_norm_grad(gd, xd, wd, eps, out=(None, gd, xd)[place])
+        if not place:
+            assert np.array_equal(got.get()[plain], want[plain])
+        bound = u * np.abs(dx) + off * u * size + s * 2.0 ** -149
+        assert np.all(np.abs(got.get() * s - dx) <= bound)
+        bound = u * np.abs(dw) + (shape[0] + off) * u * dw_size + tiny('float32')
+        assert np.all(np.abs(got_w.get() - dw) <= bound)
+
+
+@pytest.mark.parametrize('shape', [(4, 5), (4, 64), (4, 1000), (4, 40001)])
+def test_rows_of_zeros_infinities_and_nan_without_eps(shape):
+    """As with one: what has no value is NaN, and the rows beside it keep theirs."""
+    x, g, w = inputs(shape, 'float32', 1), inputs(shape, 'float32', 2), inputs(shape[-1:], 'float32', 3)
+    x[0], x[1, 2], x[2, 3] = 0, np.inf, np.nan
+    x[3] *= np.float32(1e30)
+    y = cp.rms_norm(cp.asarray(x), cp.asarray(w), eps=0.0).get()
+    assert np.all(np.isnan(y[0])) and np.isnan(y[1, 2]) and not np.delete(y[1], 2).any()
+    assert np.all(np.isnan(y[2]))
+    check_norm(y[3], norm64(x[3], w, 0.0), shape[-1], 'float32')
+    q, s = (a.get() for a in cp.rms_norm_int8(cp.asarray(x), cp.asarray(w), eps=0.0))
+    assert np.all(np.isnan(s[:3])) and np.isfinite(s[3]) and np.abs(q[3]).max() == 127
+    dx = cp.rms_norm_grad(cp.asarray(g), cp.asarray(x), eps=0.0).get()
+    assert np.isnan(dx[0]).all() and np.isnan(dx[1, 2]) and np.isnan(dx[2]).all()
+    # (rows of zeros with an eps, however small)
+    z = cp.zeros(shape, 'float32')
+    assert not cp.rms_norm(z, cp.asarray(w), eps=1e-40).get().any()
+    q, s = cp.rms_norm_int8(z, cp.asarray(w), eps=1e-40)
+    assert not q.get().any() and not s.get().any()
+
+
+def test_float32_residual_of_any_size_with_float16():
+    for power in (100, -100):
+        x, w = inputs((6, 300), 'float16', 1), inputs((300,), 'float16', 2)
+        r = np.ldexp(inputs((6, 300), 'float32', 3), power)
+        if power < 0:
+            x[:] = 0
+        y, h = cp.rms_norm(cp.asarray(x), cp.asarray(w), cp.asarray(r), 0.0)
+        h64 = np.ldexp(x.astype(np.float64), -power) + np.ldexp(r.astype(np.float64), -power)
+        check_norm(y.get(), norm64(h64, w, 0.0), 300, 'float16')
 
 
 @pytest.mark.parametrize('shape', [(4, 7), (3, 300), (2, 9000)])

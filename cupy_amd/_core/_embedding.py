@@ -690,7 +690,8 @@ def embedding(table, ids, scale=1.0, *, out=None):
     Args:
         table (cupy.ndarray): float16, float32 or float64 matrix.
         ids: integers of any shape.
-        scale (float): factor; the product is rounded once.
+        scale (float): factor, of 32 bits (64 for float64 tables); the product is
+            rounded once.
         out (cupy.ndarray): receives the result, of shape
             ``ids.shape + (table.shape[1],)`` and the table's type.
     """
@@ -767,8 +768,9 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, *, dtype=None, out=None):
 
     ``out[v] = scale * (sum of grad[t] over all t with ids[t] == v)``; rows
     that no id selects are zeros, ids outside ``[0, num_rows)`` have no part.
-    The sums are held in 32 bits (64 for float64), their order is fixed:
-    repeated calls give the same bits.  Under ``cuda.memory.static_scratch``
+    The sums are held in 32 bits (64 for float64), their order follows from the
+    sizes, the ids and whether the rows of the result are stored one after the
+    other: repeated calls give the same bits.  Under ``cuda.memory.static_scratch``
     about 8 million ids can be taken (16 bytes for each, and the partial sums).
 
     Args:

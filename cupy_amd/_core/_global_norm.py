@@ -383,6 +383,9 @@ def global_norm(arrays, *, norm_out=None):
             of no arrays the norm is 0.
         norm_out (cupy.ndarray): receives the result, of shape ``()``.
 
+    Elements are added up as they are stored, by 16-byte vectors: arrays stored in
+    another order, or that start elsewhere modulo 16 bytes, may give other last bits.
+
     Returns:
         cupy.ndarray: of shape ``()``; float32, or float64 if any array is.
         Nothing waits for it: it is on the device.

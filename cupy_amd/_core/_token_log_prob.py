@@ -713,9 +713,12 @@ def token_log_prob(logits, tokens, *, entropy=False, top=0, out=None):
             likely ones the lower token comes first.
         out (TokenLogProb): arrays that receive the results.
 
-    Sums are held in 32 bits (64 for float64) and joined in 64.  A row whose
-    elements are all -inf has log probabilities of -inf and the entropy 0; a
-    row with a NaN or +inf has NaN everywhere and -1 for its likeliest tokens.
+    Sums are held and joined in 32 bits (64 for float64), what follows from a row's
+    sums is computed in 64.  They are grouped by 16-byte vectors: rows that start
+    elsewhere modulo 16 bytes may differ in the last bits.  A row whose elements are
+    all -inf has log probabilities of -inf and the entropy 0; a row with a NaN or
+    +inf has NaN for all of them and -1 for its likeliest tokens (a token out of range
+    has the log probability 0 there too).
 
     Returns:
         TokenLogProb: ``log_prob``, ``lse`` (the logarithm of the sum of

@@ -204,3 +204,56 @@ def test_captured_at_training_sizes():
             work()
         stream.synchronize()
         want = [a.get() for a in outs]
+
+
+@pytest.mark.parametrize('dtype', ['float16', 'float32'])
+def test_the_same_bits_from_arrays_laid_out_alike(dtype):
+    """What fixes the order of a sum: sizes, strides, storage order and the address
+    modulo 16, and nothing else.  Where only the address differs modulo 16, results
+    are compared to the bound that holds for either: both are off by at most n
+    roundings of 2^-24 relative to the sum of the sizes, n the elements a lane adds up."""
+    rng = np.random.default_rng(7)
+    item = np.dtype(dtype).itemsize
+    n, width = 70, 1003
+    x, g = (rng.standard_normal((n, width)).astype(dtype) for _ in range(2))
+    w = (1 + rng.random(width)).astype(dtype)
+    ids, tokens = cp.asarray(rng.integers(-1, 900, n)), cp.asarray(rng.integers(0, width, n))
+    grad = cp.asarray(rng.standard_normal(n).astype('float32'))
+
+    def at(a, start):
+        """``a`` at ``start`` elements behind a 256-byte border, other things around it."""
+        store = cp.full(a.size + 64, 3, dtype)
+        assert store.data.ptr % 256 == 0
+        view = store[start:start + a.size].reshape(a.shape)
+        view[...] = cp.asarray(a)
+        return view
+
+    def everything(start):
+        xd, gd, wd = at(x, start), at(g, start), at(w, start)
+        r = cp.token_log_prob(xd, tokens, entropy=True, top=3)
+        out = [r.log_prob, r.lse, r.entropy, r.top_log_prob,
+               cp.token_log_prob_grad(grad, xd, tokens, r.lse), cp.global_norm([xd, gd, wd])]
+        out += [*cp.rms_norm_grad(gd, xd, wd), *cp.rms_norm(xd, wd, gd), *cp.rms_norm_int8(xd, wd)]
+        out += [cp.embedding_grad(gd, ids, 900), cp.embedding(xd, ids, 1.5)]
+        return r.top_token.get(), [a.get().astype(np.float64) for a in out]
+    best, first = everything(0)
+    for start in (0, 16 // item, 48 // item):                # the same modulo 16
+        again, same = everything(start)
+        assert np.array_equal(again, best)
+        for a, b in zip(same, first):
+            assert np.array_equal(a, b)
+    # logits of about 4 at most: lse, entropies and log probabilities of 3 to 11, whose
+    # exponentials are summed in chains of at most 16 and 6 joins and rounded once
+    for start in (1, 3, 5):
+        again, other = everything(start)
+        assert np.array_equal(again, best)
+        for a, b in zip(other[:4], first[:4]):
+            assert np.all(np.abs(a - b) <= 2 * 2.0 ** -24 * (16 + 6 + 2 * 16))
+        # (its exponential: one lse for another, and the result's rounding)
+        p = np.abs(first[4]) + np.abs(grad.get())[:, None]
+        step = np.finfo(dtype).eps
+        assert np.all(np.abs(other[4] - first[4]) <= step * np.abs(first[4]) + 2.0 ** -17 * p + 1e-7)
+        # (32 elements in 32 bits, or 64 bits throughout; half of it in the root)
+        assert abs(other[5] - first[5]) <= 40 * 2.0 ** -24 * first[5]
+        for a, b in zip(other[6:], first[6:]):               # rows as their elements lie
+            assert np.array_equal(a, b)

@@ -768,6 +768,12 @@ def _range_of(eps):
     return 2.0 ** -60 if eps < 2.0 ** -40 else 0.0, min(math.sqrt(eps), 1e38) if eps > 0 else 0.0
 
 
+def _held_eps(dtype, ranged, eps):
+    """eps for kernels that hold it in 32 bits: above 0 there too.  (The mean square of
+    float16 rows is 0 or far above 1e-38; RANGED kernels take it as it is.)"""
+    return 1e-38 if dtype.char != 'd' and not ranged and 0 < eps < 1e-38 else eps
+
+
 def _check(x, weight, residual, what):
     _oc.check_float(x, 'x')
     if x.ndim == 0:
@@ -903,7 +909,7 @@ def _norm(plans, int8, x, weight, residual, eps, out, scale_out, residual_out):
     call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqdff',
                 Ref(0), Ref(i_r) if i_r is not None else 0, Ref(i_w) if i_w is not None else 0,
                 Ref(i_y), Ref(i_s) if int8 else 0, Ref(i_h) if i_h is not None else 0,
-                rows, width, px, pr, py, ps, eps, *_range_of(eps))
+                rows, width, px, pr, py, ps, _held_eps(x.dtype, ranged, eps), *_range_of(eps))
     out = call.finish(ret if len(ret) > 1 else ret[0])
     return out
 
@@ -1088,7 +1094,8 @@ def rms_norm_grad(grad, x, weight=None, eps=1e-6, *, residual_grad=None, out=Non
     call.launch(fn, (grid, 1, 1), block, 'PPPPPPqiqqqqdff',
                 Ref(0), Ref(1), Ref(i_w) if i_w is not None else 0,
                 Ref(i_r) if i_r is not None else 0, Ref(i_d), Ref(i_t) if i_t is not None else 0,
-                rows, width, pg, px, pr, pd, eps, *_range_of(eps))
+                rows, width, pg, px, pr, pd, _held_eps(x.dtype, x.dtype.char == 'f', eps),
+                *_range_of(eps))
     if few:
         fn = _GRAD_SOURCE.function('cupy_rms_norm_few', **defines)
         call.launch(fn, (-(-width // 64), 1, 1), 1024, 'PPPPiiqq',

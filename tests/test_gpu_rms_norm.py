@@ -288,10 +288,13 @@ def test_rows_of_zeros_infinities_and_nan_without_eps(shape):
     dx = cp.rms_norm_grad(cp.asarray(g), cp.asarray(x), eps=0.0).get()
     assert np.isnan(dx[0]).all() and np.isnan(dx[1, 2]) and np.isnan(dx[2]).all()
     # (rows of zeros with an eps, however small)
-    z = cp.zeros(shape, 'float32')
-    assert not cp.rms_norm(z, cp.asarray(w), eps=1e-40).get().any()
-    q, s = cp.rms_norm_int8(z, cp.asarray(w), eps=1e-40)
-    assert not q.get().any() and not s.get().any()
+    for dtype, eps in (('float32', 1e-40), ('float32', 1e-70), ('float16', 1e-70), ('float64', 1e-300)):
+        z, wd = cp.zeros(shape, dtype), cp.asarray(w.astype(dtype))
+        assert not cp.rms_norm(z, wd, eps=eps).get().any()
+        q, s = cp.rms_norm_int8(z, wd, eps=eps)
+        assert not q.get().any() and not s.get().any()
+        _, dw = cp.rms_norm_grad(cp.asarray(g.astype(dtype)), z, wd, eps)
+        assert not dw.get().any()
 
 
 def test_float32_residual_of_any_size_with_float16():

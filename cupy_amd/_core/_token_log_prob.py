@@ -533,7 +533,7 @@ cupy_token_log_prob(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A
 
 // The parts of a row joined: a workgroup per row, at most 64 parts.  A chain of
 // waits: all that does not depend on a result is requested at the start (8 rows of
-// 64 parts, 20 alternatives: 5.6 us).
+// 64 parts, 20 alternatives: about 5 us).
 extern "C" __global__ void __launch_bounds__(256)
 cupy_token_log_prob_join(const X_T* logits, const I_T* tokens, A* log_prob, A* lse, A* entropy,
                          A* top, long long* index, const A* runs, const long long rows,
@@ -806,31 +806,34 @@ def _geometry(rows, vecs, top):
     block, parts = 256, 1
     if rows < units * 3 // 8 and vecs > 14336:
         # Long rows, too few to fill the device, are cut into parts; a second
-        # launch joins them, which costs about 5 us (64 rows of 128000 float16: 15
-        # us in parts, 16.3 in one launch; 64 of 200000 float32: 19 and 24; 8 of
-        # 131072 float32: 12.5 and 18; but 100 of 64000 float32: 15.8 and 12.5, 32
-        # of 50257: 14 and 11).
+        # launch joins them, which costs about 5 us (with 5 alternatives: 64 rows of
+        # 128000 float16: 13.6 us in parts, 14.0 in one launch; 64 of 200000 float32:
+        # 18.0 and 21.2; 8 of 131072 float32: 12.8 and 14.7; but 100 of 64000 float32:
+        # 14.4 and 11.4, 32 of 50257: 11.7 and 10.1; with the entropy alone: 12.2 and
+        # 12.1, 13.6 and 19.7, 11.8 and 12.7, 12.0 and 9.1, 12.3 and 7.4).
         parts = min(64, max(1, 4 * units // rows), -(-vecs // (2 * block)))
     elif rows <= units and vecs > 2048:
-        # (190 rows of 100000 float16: 16.4 us; 17.6 with 512 threads to a row, 24
-        # with 256)
+        # (190 rows of 100000 float16 with entropy: 11.0 us; 11.8 with 512 threads to a
+        # row, 15.6 with 256; with 5 alternatives: 13.6, 14.0, 18.0)
         block = 1024
     elif rows < 4 * units:
-        # (300 rows of 100000 float16: 23 us with 512 threads to a row, 25 with 256,
-        # 27 with 1024; 1000 rows of 16000 float16: 22.9 and 19.7)
+        # (300 rows of 100000 float16 with entropy: 17.7 us with 512 threads to a row,
+        # 19.8 with 256, 19.5 with 1024; with 5 alternatives: 19.8, 21.3, 24.8; 1000 rows
+        # of 16000 float16: 9.9 and 9.3 with entropy, 15.7 and 12.5 with alternatives)
         block = 512 if vecs > 2048 else 256
     elif vecs <= 512 or (top > 1 and vecs <= 1024):
         # Short rows: one wave to each, whose reductions meet no barrier (16384
-        # rows of 1500 float16: 17.5 us; 22.5 with two waves, 30 with four).  What
-        # is done for alternatives is done by every wave, so that fewer are best
-        # there (8000 rows of 8000 float16, 5 of them: 37 us; 45 with two waves, 57
-        # with four).
+        # rows of 1500 float16 with entropy: 15.8 us; 20.5 with two waves, 27.8 with
+        # four).  What is done for alternatives is done by every wave, so that fewer are
+        # best there (8000 rows of 8000 float16, 5 of them: 35.3 us; 40.2 with two waves,
+        # 52.2 with four).
         block = 64
     elif top > 1 and vecs <= 2048:
-        # (4000 rows of 8000 float32, 5 of them: 32 us; 32 with one wave, 37 with four)
+        # (4000 rows of 8000 float32, 5 of them: 32.2 us; 32.0 with one wave, 37.3 with
+        # four)
         block = 128
     # Long ones: four waves, so that a unit holds eight rows (8192 rows of 50257
-    # float16 with entropy: 140 us; 175 with eight waves, 220 with sixteen).
+    # float16 with entropy: 131 us; 142 with eight waves, 197 with sixteen).
     return block, 4, parts
 
 

@@ -397,8 +397,8 @@ def clip_by_global_norm(arrays, max_norm, *, eps=1e-6, out=None, norm_out=None):
     """Scales arrays down so that their :func:`global_norm` is ``max_norm`` at most.
 
     Every array is multiplied by ``min(1, max_norm / (norm + eps))``, a factor of 64
-    bits (rounded to 32 for float16 arrays), and rounded once.  Where the norm is infinite the factor is 0, where it is NaN the
-    factor is NaN.  Arrays whose norm plus ``eps`` does not exceed ``max_norm``,
+    bits (rounded to 32 for float16 arrays), and rounded once.  Where the norm is
+    infinite the factor is 0, where it is NaN the factor is NaN.  Arrays whose norm plus ``eps`` does not exceed ``max_norm``,
     which may be infinite, keep their bits.
 
     Args:

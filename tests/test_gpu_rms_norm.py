@@ -230,7 +230,7 @@ def test_rows_of_any_size(shape, dtype, power, eps):
     assert np.all(np.abs(q).max(-1) == 127)
 
 
-@pytest.mark.parametrize('shape', [(1030, 3), (5000, 64), (3000, 1003), (1536, 4096), (300, 12000), (700, 33000)])
+@pytest.mark.parametrize('shape', [(1030, 3), (5000, 64), (3000, 127), (2000, 250), (3000, 1003), (1536, 4096), (300, 12000), (700, 33000)])
 def test_rows_of_all_sizes_side_by_side(shape):
     """Few rows in between that leave the range, where workgroups take several: the
     others have the bits that they have among themselves, and dw holds all of them."""
@@ -271,6 +271,31 @@ def test_rows_of_all_sizes_side_by_side(shape):
         assert np.all(np.abs(got.get() * s - dx) <= bound)
         bound = u * np.abs(dw) + (shape[0] + off) * u * dw_size + tiny('float32')
         assert np.all(np.abs(got_w.get() - dw) <= bound)
+
+
+@pytest.mark.parametrize('shape', [(600, 100), (2000, 1003), (200, 8192), (50, 33000)])
+def test_gradients_without_a_value_stay_in_their_row(shape):
+    """An infinity and a NaN among the gradients, products too large for float32: the
+    other rows have their bits, the other columns of dw their value."""
+    g, x, w = inputs(shape, 'float32', 1), inputs(shape, 'float32', 2), inputs(shape[-1:], 'float32', 3)
+    want, _ = (a.get() for a in cp.rms_norm_grad(cp.asarray(g), cp.asarray(x), cp.asarray(w)))
+    rows = [3, shape[0] // 2, shape[0] - 1]
+    g[rows[0], 7], g[rows[1], 8], g[rows[2], 9:12] = np.inf, np.nan, 3e38
+    x[rows[2], 9:12] = 9.0
+    with np.errstate(invalid='ignore'):
+        _, dw, _, dw_size = grad64(g, x, w, 1e-6)
+    for into in (False, True):
+        gd = cp.asarray(g)
+        got, got_w = (a.get() for a in cp.rms_norm_grad(gd, cp.asarray(x), cp.asarray(w),
+                                                        out=gd if into else None))
+        if not into:
+            assert np.array_equal(np.delete(got, rows, 0), np.delete(want, rows, 0))
+        assert np.isnan(got[rows[1]]).all() and not np.isfinite(got[rows[0]]).any()
+        columns = np.arange(shape[1])
+        columns = columns[(columns < 7) | (columns > 11)]
+        off = (shape[0] + 1.5 * terms(shape[-1]) + 10) * acc_step('float32')
+        assert np.all(np.abs(got_w[columns] - dw[columns])
+                      <= 2.0 ** -24 * np.abs(dw[columns]) + off * dw_size[columns])
 
 
 @pytest.mark.parametrize('shape', [(4, 5), (4, 64), (4, 1000), (4, 40001)])
